@@ -297,6 +297,131 @@ WR_API wr_status_t wr_naive_moe(const wr_moe_desc_t* desc, const void* x,
                          void* workspace, size_t workspace_bytes,
                          wr_stream_t stream);
 
+/* ---- paged key/value cache --------------------------------------------- */
+
+/* A paged key/value cache: k and v are [num_pages][num_kv_heads][page_size]
+ * [head_dim] arrays of `dtype`, strides in elements and the same for both,
+ * head_dim contiguous (so pages of [page_size][num_kv_heads][head_dim] are
+ * the same cache with other strides).  Slot s of the cache is row
+ * s % page_size of page s / page_size.  head_dim: a multiple of 8 in
+ * [16, 256]; k, v and every stride 16-byte aligned.  No counterpart in
+ * warp-route, whose decode step begins at the MoE layer's input. */
+typedef struct wr_paged_kv {
+  void* k;
+  void* v;
+  int64_t page_stride;
+  int64_t head_stride;
+  int64_t slot_stride;
+  int32_t num_pages;
+  int32_t num_kv_heads;
+  int32_t page_size;
+  int32_t head_dim;
+  int32_t dtype; /* wr_dtype_t */
+  int32_t reserved;
+} wr_paged_kv_t;
+
+/* The [num_tokens][heads][head_dim] rows of a call, strides in elements and
+ * 16-byte aligned (so the parts of a fused projection go in as they are). */
+typedef struct wr_rows {
+  const void* ptr;
+  int64_t token_stride;
+  int64_t head_stride;
+} wr_rows_t;
+
+/* Writes the keys and values of num_tokens tokens into the cache: token t
+ * goes to slot slots[t]; a token whose slot is negative or outside the cache
+ * is not written (the padding of a batch).  Two tokens of a call with one
+ * slot leave that slot's content undefined.  With positions and inv_freq
+ * [rot_dim / 2] the first rot_dim columns of each key turn by the angles
+ * positions[t] * inv_freq[i] on the way: columns (i, i + rot_dim / 2), or
+ * (2i, 2i + 1) when interleaved is not 0; angles by a 64-bit product, so far
+ * positions keep theirs.  With q (num_q_heads heads) and q_out, contiguous
+ * [num_tokens][num_q_heads][head_dim], the queries of all tokens, those
+ * without a slot too, turn by the same angles into q_out, which must not
+ * overlap q.  rot_dim: even, in [0, head_dim]; positions and inv_freq may be
+ * NULL when it is 0.  No counterpart in warp-route. */
+WR_API wr_status_t wr_append_paged_kv(const wr_paged_kv_t* cache, int32_t num_tokens,
+                                      const wr_rows_t* k, const wr_rows_t* v,
+                                      const int64_t* slots, const int64_t* positions,
+                                      const float* inv_freq, int32_t rot_dim,
+                                      int32_t interleaved, int32_t num_q_heads,
+                                      const wr_rows_t* q, void* q_out, wr_stream_t stream);
+
+/* Attention of a batch over the cache.  All sequences see the same prefix,
+ * prefix_len keys in the pages prefix_pages[0 .. ceil(prefix_len/page_size));
+ * sequence b then sees context_lens[b] keys of its own, in the pages of row b
+ * of block_tables (table_width entries, rows table_stride apart).  The rest
+ * of a last page is not read, whatever it holds.  Without q_start (NULL)
+ * sequence b asks with token b (num_tokens = num_seqs), and sees all of its
+ * keys; with q_start [num_seqs + 1], non-decreasing, it asks with tokens
+ * q_start[b] .. q_start[b+1] - 1, which stand for its last own keys: the
+ * i-th of n sees the prefix and the first context_lens[b] - n + i + 1 of the
+ * own keys.  Query head h reads key head h / (num_q_heads / num_kv_heads).
+ *
+ *   out = sum_j softmax_j(scale * q . k_j) v_j,   lse = log sum_j e^(scale q . k_j)
+ *
+ * out: contiguous [num_tokens][num_q_heads][head_dim] of the cache's type;
+ * lse: fp32 [num_tokens][num_q_heads], or NULL.  A row that sees no key, and
+ * a token that belongs to no sequence, gets out = 0 and lse = -inf.  A page
+ * index outside the cache hides its keys.  Lengths, tables and q_start are
+ * read on the device, so a captured graph follows them; prefix_len is fixed
+ * in the call.  The workspace needs no initial content; calls that share one
+ * must not overlap on the GPU.  No counterpart in warp-route. */
+typedef struct wr_attn_desc {
+  int32_t num_tokens;
+  int32_t num_seqs;
+  int32_t num_q_heads;
+  int32_t table_width;
+  int64_t table_stride;
+  int32_t prefix_len;
+  float scale;
+} wr_attn_desc_t;
+
+WR_API size_t wr_shared_prefix_attention_workspace_size(const wr_paged_kv_t* cache,
+                                                        const wr_attn_desc_t* desc,
+                                                        int32_t has_q_start);
+WR_API wr_status_t wr_shared_prefix_attention(const wr_paged_kv_t* cache,
+                                              const wr_attn_desc_t* desc, const wr_rows_t* q,
+                                              const int32_t* block_tables,
+                                              const int32_t* context_lens,
+                                              const int32_t* q_start,
+                                              const int32_t* prefix_pages, void* out, float* lse,
+                                              void* workspace, size_t workspace_bytes,
+                                              wr_stream_t stream);
+
+/* ---- sampling ---------------------------------------------------------- */
+
+/* Settings of wr_sample_tokens: one number for all rows, or, where the
+ * pointer is not NULL, one per row on the device. */
+typedef struct wr_sampling {
+  float temperature; /* 0 or less: the maximum */
+  float top_p;       /* 1 or more: off */
+  float min_p;       /* 0: off */
+  int32_t top_k;     /* below 1: off */
+  const float* temperatures;
+  const float* top_ps;
+  const float* min_ps;
+  const int32_t* top_ks;
+} wr_sampling_t;
+
+/* A token for each of num_rows rows of logits [vocab] (dtype fp32 or bf16,
+ * rows row_stride elements apart):
+ *   w_i = e^((x_i - max) / temperature), ordered by x descending, equal ones
+ *   by index ascending; kept are the first top_k of the order, of these the
+ *   ones whose preceding sum of w is below top_p times the sum of those
+ *   top_k, of these the ones with w_i >= min_p, and always the first;
+ *   ids[r] = lowest index whose running sum of kept w (by index) exceeds
+ *   uniforms[r] * (sum of kept w), uniforms in [0, 1).
+ * w is held in whole numbers of 2^-45, so a call's result does not depend on
+ * the order of its sums; a NaN counts as -inf; a row with nothing above -inf
+ * gets -1; where the maximum is +inf only such values are sampled.  ids:
+ * int64.  vocab at most 262144.  No counterpart in warp-route (its top-K
+ * over router logits is wr_router_topk). */
+WR_API wr_status_t wr_sample_tokens(int64_t num_rows, int32_t vocab, int32_t dtype,
+                                    const void* logits, int64_t row_stride,
+                                    const float* uniforms, const wr_sampling_t* sampling,
+                                    int64_t* ids, wr_stream_t stream);
+
 /* ---- device status ----------------------------------------------------- */
 
 /* Reads (and clears) the status word a fused call left in its workspace:

@@ -1,0 +1,166 @@
+"""GPU: sample_tokens against a 64-bit form, token by token.
+
+The tokens have to be equal.  The kernel holds weights in whole numbers of
+2^-45 of the largest, the reference in 64-bit floating point: with V values
+their running sums differ by at most V * 2^-46, which moves a border past the
+given number in a row with probability about 2 V * V * 2^-46 at most
+(V = 50000: 7e-5) were all weights equal to the largest, and far less for
+weights that fall off; the seeds are fixed, so a pass is a pass.
+"""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+import warp_route
+from decode_reference import sample
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _need_cuda():
+    if not torch.cuda.is_available():
+        pytest.skip("needs a CUDA device")
+
+
+def _f(v, r):
+    return float(v[r]) if isinstance(v, torch.Tensor) else float(np.float32(v))
+
+
+def check(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    ids = warp_route.sample_tokens(logits, u, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
+    assert ids.dtype == torch.int64 and ids.shape == (logits.shape[0],)
+    got = ids.cpu().numpy()
+    x = logits.double().cpu().numpy()
+    un = u.cpu().numpy()
+    for r in range(x.shape[0]):
+        k = int(top_k[r]) if isinstance(top_k, torch.Tensor) else top_k
+        want = sample(x[r], un[r], _f(temperature, r), k, _f(top_p, r), _f(min_p, r))
+        assert got[r] == want, (r, got[r], want, x[r].max())
+    return ids
+
+
+def rows(n, v, dtype=torch.float32, seed=0, spread=2.5):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    x = (torch.randn(n, v, generator=g, device="cuda") * spread).to(dtype)
+    return x, torch.rand(n, generator=g, device="cuda")
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("v", [1, 2, 5, 2047, 2048, 2049, 32000, 50001, 131072])
+@pytest.mark.parametrize("kw", [
+    dict(), dict(temperature=0.0), dict(temperature=0.3), dict(top_k=1), dict(top_k=7), dict(top_k=1000),
+    dict(top_p=0.0), dict(top_p=0.5), dict(top_p=0.999), dict(min_p=0.05), dict(min_p=1.0),
+    dict(temperature=1.7, top_k=50, top_p=0.9, min_p=0.01), dict(temperature=0.6, top_k=40000, top_p=0.97),
+])
+def test_matches_plain(v, kw, dtype):
+    x, u = rows(5, v, dtype, seed=v)
+    check(x, u, **kw)
+
+
+@pytest.mark.parametrize("n", [1, 18, 19, 200])
+def test_rows_with_settings_of_their_own(n):
+    x, u = rows(n, 30011, seed=n)
+    r = torch.arange(n, device="cuda")
+    check(x, u, temperature=torch.where(r % 4 == 0, 0.0, 0.5 + (r % 5) / 4).float(),
+          top_k=torch.where(r % 3 == 0, 0, r * 7 + 1).int(),
+          top_p=torch.where(r % 2 == 0, 1.0, 0.05 + (r % 9) / 10).float(),
+          min_p=torch.where(r % 5 == 1, 0.1, 0.0).float())
+
+
+@pytest.mark.parametrize("u", [0.0, 1e-30, 0.25, 0.5, 1 - 2.0 ** -24])
+def test_ends_of_the_uniform_numbers(u):
+    x, _ = rows(3, 5003)
+    check(x, torch.full((3,), u, device="cuda"))
+    check(x, torch.full((3,), u, device="cuda"), top_p=0.7)
+
+
+@pytest.mark.parametrize("kw", [dict(top_k=k) for k in (1, 2, 3, 2500, 4999, 5000)] +
+                         [dict(top_p=p) for p in (0.0, 1e-4, 0.5, 0.7501, 1.0)] +
+                         [dict(top_k=3000, top_p=0.3), dict(temperature=0.0), dict(min_p=1.0)])
+def test_equal_values_go_by_index(kw):
+    u = torch.tensor([0.0, 0.3, 0.77, 0.9999], device="cuda")
+    check(torch.full((4, 5000), 1.25, device="cuda"), u, **kw)
+    x = torch.zeros(4, 5000, device="cuda")
+    x[:, ::3] = 2.0   # two values, each many times
+    x[:, 1] = -0.0
+    check(x, u, **kw)
+
+
+def test_ties_across_the_border_of_a_large_row():
+    x, u = rows(4, 100000, torch.bfloat16, seed=3)
+    for k in (10, 100, 1000, 30000):
+        check(x, u, top_k=k)
+    for p in (0.1, 0.6, 0.95):
+        check(x, u, top_p=p)
+    check((x.float() / 4).round().bfloat16(), u, top_k=777, top_p=0.8)
+
+
+def test_infinities_and_nan():
+    inf, nan = float("inf"), float("nan")
+    x, u = rows(6, 3001)
+    x[0] = -inf                      # nothing to sample
+    x[1, 100:] = -inf
+    x[2, ::2] = nan
+    x[3, 7] = inf
+    x[3, 2000] = inf                 # these two alone, evenly
+    x[4] = nan
+    x[5, :3000] = -inf               # one value left
+    for kw in (dict(), dict(top_k=50), dict(top_p=0.9), dict(temperature=0.0), dict(top_k=500, top_p=0.5, min_p=0.1)):
+        ids = check(x, u, **kw)
+        assert ids[0] == -1 and ids[4] == -1 and ids[5] == 3000
+    lowest = torch.full((2, 40), torch.finfo(torch.float32).min, device="cuda")
+    lowest[1, 5] = torch.finfo(torch.float32).max
+    check(lowest, u[:2])
+    check(lowest, u[:2], top_p=0.5)
+    check(lowest, u[:2], top_k=30, top_p=0.5)
+
+
+def test_strided_and_unaligned_rows():
+    x, u = rows(4, 4003)
+    base = torch.zeros(4, 4100, device="cuda")
+    for off in (0, 1, 4):
+        v = base[:, off:off + 4003]
+        v.copy_(x)
+        check(v, u, top_k=20)
+    b = base.bfloat16()[:, 3:3 + 4003]
+    check(b, u, top_p=0.8)
+    check(x[:1].expand(4, -1), u)
+
+
+def test_largest_vocabulary_and_no_rows():
+    x, u = rows(2, 262144, seed=9)
+    check(x, u, top_p=0.9)
+    check(x, u, top_k=5000)
+    assert warp_route.sample_tokens(x[:0], u[:0]).shape == (0,)
+
+
+def test_in_a_graph():
+    x, u = rows(3, 20000)
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=st):
+        ids = warp_route.sample_tokens(x, u, top_k=40, top_p=0.9)
+    for seed in (1, 2):
+        y, w = rows(3, 20000, seed=seed)
+        x.copy_(y)
+        u.copy_(w)
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(ids, check(y, w, top_k=40, top_p=0.9))
+
+
+def test_frequencies_follow_the_probabilities():
+    """65536 evenly spaced numbers hit each kept token as often as its share
+    says, to within one (sums of shares move each end by at most one)."""
+    n = 65536
+    x = torch.tensor([0.0, 1.0, -1.0, 2.0, 0.5, -3.0], device="cuda")
+    u = (torch.arange(n, device="cuda") + 0.5) / n
+    ids = warp_route.sample_tokens(x.expand(n, -1), u, top_k=5)
+    share = torch.softmax(torch.where(x == -3.0, float("-inf"), x).double(), 0)
+    count = torch.bincount(ids, minlength=6).double()
+    assert ((count - share * n).abs() <= 1.0 + 1e-6).all()

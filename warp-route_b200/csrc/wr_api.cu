@@ -166,6 +166,56 @@ wr_status_t run_layer(const Problem& p, const void* x, const void* gate_w, const
   return WR_OK;
 }
 
+// Checks a paged cache; strides to bytes must stay 16-byte aligned.
+wr_status_t make_cache(const wr_paged_kv_t* d, PagedKv* c) {
+  if (!d) return fail(WR_ERR_INVALID, "cache must not be NULL");
+  if (d->dtype != WR_DTYPE_F32 && d->dtype != WR_DTYPE_BF16)
+    return fail(WR_ERR_INVALID, "dtype must be float32 or bfloat16, got code %d", d->dtype);
+  if (d->num_pages < 1 || d->num_kv_heads < 1 || d->page_size < 1)
+    return fail(WR_ERR_INVALID, "num_pages, num_kv_heads and page_size must be positive, got %d, %d, %d",
+                d->num_pages, d->num_kv_heads, d->page_size);
+  if (d->head_dim < 16 || d->head_dim > 256 || d->head_dim % 8 != 0)
+    return fail(WR_ERR_UNSUPPORTED, "head_dim must be a multiple of 8 in [16, 256], got %d", d->head_dim);
+  if (!d->k || !d->v) return fail(WR_ERR_INVALID, "cache k and v must not be NULL");
+  const int vec = d->dtype == WR_DTYPE_BF16 ? 8 : 4;
+  if (!aligned16(d->k) || !aligned16(d->v) || d->page_stride % vec || d->head_stride % vec ||
+      d->slot_stride % vec)
+    return fail(WR_ERR_UNSUPPORTED, "cache k, v and their strides must be 16-byte aligned");
+  if (d->page_stride < 0 || d->head_stride < 0 || d->slot_stride < 0)
+    return fail(WR_ERR_INVALID, "cache strides must not be negative");
+  *c = PagedKv{d->k, d->v, d->page_stride, d->head_stride, d->slot_stride,
+               d->num_pages, d->num_kv_heads, d->page_size, d->head_dim, d->dtype};
+  return WR_OK;
+}
+
+wr_status_t check_rows(const wr_rows_t* r, const char* name, int dtype) {
+  const int vec = dtype == WR_DTYPE_BF16 ? 8 : 4;
+  if (!r || !r->ptr) return fail(WR_ERR_INVALID, "%s must not be NULL", name);
+  if (!aligned16(r->ptr) || r->token_stride % vec || r->head_stride % vec)
+    return fail(WR_ERR_UNSUPPORTED, "%s and its strides must be 16-byte aligned", name);
+  return WR_OK;
+}
+
+wr_status_t make_attn(const wr_paged_kv_t* cache, const wr_attn_desc_t* d, AttnProblem* p) {
+  wr_status_t st = make_cache(cache, &p->c);
+  if (st != WR_OK) return st;
+  if (!d) return fail(WR_ERR_INVALID, "desc must not be NULL");
+  if (d->num_tokens < 0 || d->num_seqs < 0 || d->prefix_len < 0 || d->table_width < 0)
+    return fail(WR_ERR_INVALID, "num_tokens, num_seqs, table_width and prefix_len must be >= 0, got %d, %d, %d, %d",
+                d->num_tokens, d->num_seqs, d->table_width, d->prefix_len);
+  if (d->num_q_heads < 1 || d->num_q_heads % p->c.hkv != 0)
+    return fail(WR_ERR_INVALID, "num_q_heads must be a positive multiple of num_kv_heads %d, got %d",
+                p->c.hkv, d->num_q_heads);
+  if (d->table_stride < 0) return fail(WR_ERR_INVALID, "table_stride must not be negative");
+  if ((int64_t)d->table_width * p->c.page_size + d->prefix_len > (int64_t)1 << 30 ||
+      (int64_t)d->num_tokens * d->num_q_heads > (int64_t)1 << 30)
+    return fail(WR_ERR_UNSUPPORTED, "more than 2^30 keys a sequence, or rows of queries");
+  p->T = d->num_tokens; p->B = d->num_seqs; p->hq = d->num_q_heads;
+  p->table_width = d->table_width; p->table_stride = d->table_stride;
+  p->prefix_len = d->prefix_len; p->scale = d->scale;
+  return WR_OK;
+}
+
 }  // namespace
 }  // namespace wr
 
@@ -323,6 +373,100 @@ wr_status_t wr_naive_moe(const wr_moe_desc_t* desc, const void* x, const void* g
   if ((st = check_ws(workspace, workspace_bytes, naive_workspace_bytes(p))) != WR_OK) return st;
   return launch_naive(p, x, gate_w, weight_buf, out, nullptr, nullptr, workspace,
                       static_cast<cudaStream_t>(stream));
+}
+
+wr_status_t wr_append_paged_kv(const wr_paged_kv_t* cache, int32_t num_tokens, const wr_rows_t* k,
+                               const wr_rows_t* v, const int64_t* slots, const int64_t* positions,
+                               const float* inv_freq, int32_t rot_dim, int32_t interleaved,
+                               int32_t num_q_heads, const wr_rows_t* q, void* q_out,
+                               wr_stream_t stream) {
+  AppendProblem p{};
+  wr_status_t st = make_cache(cache, &p.c);
+  if (st != WR_OK) return st;
+  if (num_tokens < 0) return fail(WR_ERR_INVALID, "num_tokens must be >= 0, got %d", num_tokens);
+  if (rot_dim < 0 || rot_dim > p.c.dim || rot_dim % 2 != 0)
+    return fail(WR_ERR_INVALID, "rot_dim must be even and in [0, head_dim=%d], got %d", p.c.dim, rot_dim);
+  if (rot_dim > 0 && (!positions || !inv_freq))
+    return fail(WR_ERR_INVALID, "positions and inv_freq must not be NULL when rot_dim > 0");
+  if ((q == nullptr) != (q_out == nullptr))
+    return fail(WR_ERR_INVALID, "q and q_out go together");
+  if (q && num_q_heads < 1) return fail(WR_ERR_INVALID, "num_q_heads must be positive, got %d", num_q_heads);
+  if ((int64_t)(q ? num_q_heads : 0) + 2 * (int64_t)p.c.hkv > 16384)
+    return fail(WR_ERR_UNSUPPORTED, "more than 16384 heads");
+  if (num_tokens == 0) return WR_OK;
+  if ((st = check_rows(k, "k", p.c.dtype)) != WR_OK) return st;
+  if ((st = check_rows(v, "v", p.c.dtype)) != WR_OK) return st;
+  if (q && (st = check_rows(q, "q", p.c.dtype)) != WR_OK) return st;
+  if (!slots) return fail(WR_ERR_INVALID, "slots must not be NULL");
+  if (q && !aligned16(q_out)) return fail(WR_ERR_UNSUPPORTED, "q_out must be 16-byte aligned");
+  if (q && q_out == q->ptr) return fail(WR_ERR_INVALID, "q_out must not alias q");
+  p.T = num_tokens; p.rot = rot_dim; p.interleaved = interleaved != 0;
+  p.k = k->ptr; p.k_ts = k->token_stride; p.k_hs = k->head_stride;
+  p.v = v->ptr; p.v_ts = v->token_stride; p.v_hs = v->head_stride;
+  if (q) {
+    p.hq = num_q_heads;
+    p.q = q->ptr; p.q_ts = q->token_stride; p.q_hs = q->head_stride;
+  }
+  p.slots = slots; p.positions = positions; p.inv_freq = inv_freq; p.q_out = q_out;
+  return launch_append(p, static_cast<cudaStream_t>(stream));
+}
+
+size_t wr_shared_prefix_attention_workspace_size(const wr_paged_kv_t* cache,
+                                                 const wr_attn_desc_t* desc, int32_t has_q_start) {
+  AttnProblem p{};
+  static const int32_t some = 0;
+  if (make_attn(cache, desc, &p) != WR_OK) return 0;
+  if (has_q_start) p.q_start = &some;  // its presence counts here, not its content
+  return attn_workspace_bytes(p) + 256;  // never 0 for a valid description
+}
+
+wr_status_t wr_shared_prefix_attention(const wr_paged_kv_t* cache, const wr_attn_desc_t* desc,
+                                       const wr_rows_t* q, const int32_t* block_tables,
+                                       const int32_t* context_lens, const int32_t* q_start,
+                                       const int32_t* prefix_pages, void* out, float* lse,
+                                       void* workspace, size_t workspace_bytes, wr_stream_t stream) {
+  AttnProblem p{};
+  wr_status_t st = make_attn(cache, desc, &p);
+  if (st != WR_OK) return st;
+  if (!q_start && p.T != p.B)
+    return fail(WR_ERR_INVALID, "without q_start num_tokens must equal num_seqs, got %d and %d", p.T, p.B);
+  if (p.T == 0) return WR_OK;
+  if (p.B == 0) return fail(WR_ERR_INVALID, "num_seqs must be positive when there are tokens");
+  if ((st = check_rows(q, "q", p.c.dtype)) != WR_OK) return st;
+  if (!context_lens || !out) return fail(WR_ERR_INVALID, "context_lens and out must not be NULL");
+  if (p.table_width > 0 && !block_tables) return fail(WR_ERR_INVALID, "block_tables must not be NULL");
+  if (p.prefix_len > 0 && !prefix_pages) return fail(WR_ERR_INVALID, "prefix_pages must not be NULL");
+  if (!aligned16(out)) return fail(WR_ERR_UNSUPPORTED, "out must be 16-byte aligned");
+  p.q = q->ptr; p.q_ts = q->token_stride; p.q_hs = q->head_stride;
+  p.tables = block_tables; p.lens = context_lens; p.q_start = q_start; p.prefix_pages = prefix_pages;
+  p.out = out; p.lse = lse;
+  if ((st = check_ws(workspace, workspace_bytes, attn_workspace_bytes(p))) != WR_OK) return st;
+  return launch_attn(p, workspace, static_cast<cudaStream_t>(stream));
+}
+
+wr_status_t wr_sample_tokens(int64_t num_rows, int32_t vocab, int32_t dtype, const void* logits,
+                             int64_t row_stride, const float* uniforms,
+                             const wr_sampling_t* sampling, int64_t* ids, wr_stream_t stream) {
+  if (dtype != WR_DTYPE_F32 && dtype != WR_DTYPE_BF16)
+    return fail(WR_ERR_INVALID, "dtype must be float32 or bfloat16, got code %d", dtype);
+  if (num_rows < 0 || num_rows > (1 << 27))
+    return fail(WR_ERR_INVALID, "num_rows must be in [0, 2^27], got %lld", (long long)num_rows);
+  if (vocab < 1) return fail(WR_ERR_INVALID, "vocab must be positive, got %d", vocab);
+  if (vocab > kSampleMaxVocab)
+    return fail(WR_ERR_UNSUPPORTED, "vocab %d exceeds %d", vocab, kSampleMaxVocab);
+  if (row_stride < 0) return fail(WR_ERR_INVALID, "row_stride must not be negative");
+  if (num_rows == 0) return WR_OK;
+  if (!logits || !uniforms || !sampling || !ids)
+    return fail(WR_ERR_INVALID, "logits, uniforms, sampling and ids must not be NULL");
+  SampleProblem p{};
+  p.rows = num_rows; p.vocab = vocab; p.dtype = dtype; p.logits = logits; p.row_stride = row_stride;
+  p.uniforms = uniforms;
+  p.temperatures = sampling->temperatures; p.top_ps = sampling->top_ps; p.min_ps = sampling->min_ps;
+  p.top_ks = sampling->top_ks;
+  p.temperature = sampling->temperature; p.top_p = sampling->top_p; p.min_p = sampling->min_p;
+  p.top_k = sampling->top_k;
+  p.ids = ids;
+  return launch_sample(p, static_cast<cudaStream_t>(stream));
 }
 
 wr_status_t wr_workspace_status(void* workspace, wr_stream_t stream) {

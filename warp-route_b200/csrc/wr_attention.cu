@@ -1,0 +1,1012 @@
+// wr_attention.cu — attention of a batch over a paged cache, with a prefix
+// shared by all sequences.
+//
+//   s_j = scale * q . k_j over the prefix and the sequence's own keys up to
+//         the token's own;   out = sum_j e^(s_j - m) v_j / sum_j e^(s_j - m)
+//
+// by the running maximum m and sum l, in units of log2 (2^(s log2(e) - m));
+// scores, m, l and the sums O are fp32, the weights 2^(s - m) are rounded to
+// the cache's type for the second product (bf16: half a step of 2^-8, as the
+// output itself), l adds them before that rounding.
+//
+// Own keys: each sequence's few rows meet its own keys, one byte of cache for
+// a few operations, so HBM bounds it.  k_attn_stream: a warp works alone on
+// 16 keys at a time, which it brings with 16-byte asynchronous copies into
+// a ring of its own in shared memory (no barrier between warps anywhere), and
+// multiplies with its 16 rows by mma.sync (the M of tcgen05 is 128 rows, of
+// which these segments fill 1 to 16; nothing here comes near the tensor
+// rate).  The units of all sequences are dealt to the warps evenly (see
+// wr_attention.cuh), so one long sequence and hundreds of short ones fill the
+// GPU alike.  k_attn_stream_f32: the same ring and split with fp32 products
+// on the CUDA cores, 8 rows a warp.
+//
+// Prefix: its rows are the tokens of all sequences.  With one sequence, or a
+// prefix short enough, each sequence reads it with its own keys; else it is a
+// segment of its own, whose partial results k_attn_combine joins to those of
+// the own keys: m = max m_s, l = sum l_s 2^(m_s - m), O = sum O_s 2^(m_s - m),
+// in the order of the pieces, so that a call's result is the same each time.
+#include "wr_attention.cuh"
+
+namespace wr {
+namespace {
+
+constexpr int kStreamWarps = 4;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+#define WR_NEG_INF (-__int_as_float(0x7f800000))
+
+WR_DEVINL float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+WR_DEVINL void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes)
+               : "memory");
+}
+WR_DEVINL void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+WR_DEVINL void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+WR_DEVINL void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+WR_DEVINL void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+WR_DEVINL void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+WR_DEVINL uint32_t pack_bf16(float lo, float hi) {
+  __nv_bfloat162 b = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<uint32_t*>(&b);
+}
+
+// ---------------------------------------------------------------------------
+// The split, computed by each CTA from the lengths
+// ---------------------------------------------------------------------------
+constexpr int kScanThreads = kStreamWarps * 32;
+
+struct ScanSmem {
+  int64_t chunk[kScanThreads + 1];  // units before each thread's run of sequences
+};
+
+// All threads of the CTA (NT of them).  Fills sm.chunk; CTA 0 of an own
+// launch also writes seq_unit, all CTAs together token_seq.
+template <int MR, int NT>
+WR_DEVINL int64_t scan_units(const AttnArgs& a, ScanSmem& sm) {
+  const int per = (a.B + NT - 1) / NT;
+  const int b0 = min(a.B, (int)threadIdx.x * per), b1 = min(a.B, b0 + per);
+  int64_t sum = 0;
+  for (int b = b0; b < b1; ++b) {
+    const SeqInfo s = seq_info(a, b);
+    sum += (int64_t)a.hkv * row_tiles<MR>(a, s) * key_units(a, s);
+  }
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int64_t incl = sum;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int64_t u = __shfl_up_sync(0xffffffffu, incl, d);
+    if (lane >= d) incl += u;
+  }
+  __shared__ int64_t warp_sum[NT / 32];
+  if (lane == 31) warp_sum[warp] = incl;
+  __syncthreads();
+  for (int w = 0; w < warp; ++w) incl += warp_sum[w];
+  sm.chunk[threadIdx.x + 1] = incl;
+  if (threadIdx.x == 0) sm.chunk[0] = 0;
+  __syncthreads();
+  if (a.own) {
+    if (blockIdx.x == 0) {
+      int64_t at = sm.chunk[threadIdx.x];
+      for (int b = b0; b < b1; ++b) {
+        const SeqInfo s = seq_info(a, b);
+        a.seq_unit[b] = at;
+        at += (int64_t)a.hkv * row_tiles<MR>(a, s) * key_units(a, s);
+      }
+      if (threadIdx.x == 0) a.seq_unit[a.B] = sm.chunk[NT];
+    }
+    if (a.q_start)
+      for (int t = blockIdx.x * NT + threadIdx.x; t < a.T; t += gridDim.x * NT) {
+        int lo = 0, hi = a.B;  // last b with q_start[b] <= t
+        while (hi - lo > 1) {
+          const int mid = (lo + hi) >> 1;
+          if (__ldg(a.q_start + mid) <= t) lo = mid; else hi = mid;
+        }
+        const SeqInfo s = seq_info(a, lo);
+        a.token_seq[t] = t >= s.q0 && t < s.q0 + s.nq ? lo : -1;
+      }
+  }
+  return sm.chunk[NT];
+}
+
+// A position in the order of the units.
+template <int MR>
+struct Cursor {
+  int b, h, rt, u;   // sequence, key head, row tile, unit
+  int rts, us;       // row tiles and units of the sequence
+  SeqInfo s;
+
+  WR_DEVINL void load(const AttnArgs& a) {
+    s = seq_info(a, b);
+    rts = row_tiles<MR>(a, s);
+    us = key_units(a, s);
+  }
+  // To unit `at` (< units of the launch).
+  template <int NT>
+  WR_DEVINL void seek(const AttnArgs& a, const ScanSmem& sm, int64_t at) {
+    int lo = 0, hi = NT;  // last run that starts at or before `at`
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (sm.chunk[mid] <= at) lo = mid; else hi = mid;
+    }
+    int64_t left = at - sm.chunk[lo];
+    b = lo * ((a.B + NT - 1) / NT);
+    for (;;) {
+      load(a);
+      const int64_t n = (int64_t)a.hkv * rts * us;
+      if (left < n) break;
+      left -= n;
+      ++b;
+    }
+    const int64_t tile = left / us;
+    u = (int)(left - tile * us);
+    h = (int)(tile / rts);
+    rt = (int)(tile - (int64_t)h * rts);
+  }
+  // Never called past the launch's last unit.
+  WR_DEVINL void next(const AttnArgs& a) {
+    if (++u < us) return;
+    u = 0;
+    if (++rt < rts) return;
+    rt = 0;
+    if (++h < a.hkv) return;
+    h = 0;
+    do {
+      ++b;
+      load(a);
+    } while (rts == 0 && b + 1 < a.B);
+  }
+};
+
+// The page of this lane's key of a unit, read ahead of the copies.
+template <int MR>
+WR_DEVINL int lane_page(const AttnArgs& a, const Cursor<MR>& c, int lane) {
+  const int j = c.u * kUnitTokens + (lane & 15);
+  int page, row;
+  if (j < a.prefix) {
+    split_page(j, a.page_size, a.page_shift, page, row);
+    return __ldg(a.prefix_pages + page);
+  }
+  const int jj = j - a.prefix;
+  if (jj >= c.s.len) return -1;
+  split_page(jj, a.page_size, a.page_shift, page, row);
+  return __ldg(a.tables + c.b * a.table_stride + page);
+}
+
+// Offset (elements) of this lane's key in the cache; its valid bit.  A page
+// outside the cache makes its keys invisible.
+template <int MR>
+WR_DEVINL int64_t lane_offset(const AttnArgs& a, const Cursor<MR>& c, int page, int lane, bool& ok) {
+  const int j = c.u * kUnitTokens + (lane & 15);
+  int p, row;
+  split_page(j < a.prefix ? j : j - a.prefix, a.page_size, a.page_shift, p, row);
+  ok = page >= 0 && page < a.num_pages;
+  return ok ? page * a.page_stride + c.h * a.head_stride + row * a.slot_stride : 0;
+}
+
+// Number of keys that row (token i of the sequence) sees of the segment.
+template <int MR>
+WR_DEVINL int row_limit(const AttnArgs& a, const Cursor<MR>& c, int i) {
+  return a.prefix + max(0, c.s.len - c.s.nq + i + 1);
+}
+
+// Where a finished piece goes: out (whole and final), home or a warp's slot.
+struct PieceDst {
+  float* o;
+  float2* ml;
+  int64_t row0;  // row r of the tile is row0 + r of (o, ml), home and out rows excepted
+  bool home, final;
+};
+
+// ---------------------------------------------------------------------------
+// bf16
+// ---------------------------------------------------------------------------
+constexpr int kStages = 3;
+template <int DP>
+struct StreamCfg {
+  static constexpr int kRowBytes = DP * 2;
+  static constexpr int kTile = kUnitTokens * kRowBytes;  // K (or V) of a unit
+  static constexpr bool kQSmem = DP > 128;  // the fragments of 256 columns do not fit beside O
+  static constexpr int kWarpBytes = kStages * 2 * kTile + (kQSmem ? kTile : 0);
+  static constexpr int kSmem = kStreamWarps * kWarpBytes;
+};
+
+template <int DP>
+__global__ void __launch_bounds__(kStreamWarps * 32) k_attn_stream(const AttnArgs a) {
+  using C = StreamCfg<DP>;
+  constexpr int MR = 16, CPR = DP / 8, RPP = 32 / CPR;  // chunks a row, rows a pass of the warp
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ ScanSmem sm;
+  __shared__ uint32_t s_bits[kStreamWarps][kStages];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  griddep_launch_dependents();
+  AttnSplit sp;
+  sp.units = scan_units<MR, kStreamWarps * 32>(a, sm);
+  sp.ranges = min((int64_t)gridDim.x * kStreamWarps, sp.units);
+  const int64_t w = (int64_t)warp * gridDim.x + blockIdx.x;
+  if (w < sp.ranges) {
+    const int64_t u0 = range_start(sp, w), u1 = range_start(sp, w + 1);
+    uint8_t* ring = smem + warp * C::kWarpBytes;
+    const uint32_t ring_s = smem_u32(ring);
+    const uint32_t q_s = ring_s + kStages * 2 * C::kTile;
+    Cursor<MR> cl, cc;  // the copies' and the products' position
+    cl.seek<kStreamWarps * 32>(a, sm, u0);
+    cc = cl;
+    const int n = (int)(u1 - u0);
+    int page = lane_page(a, cl, lane);
+    int loaded = 0;
+    auto load = [&]() {
+      if (loaded < n) {
+        const int st = loaded % kStages;
+        bool ok;
+        const int64_t off = lane_offset(a, cl, page, lane, ok);
+        const uint32_t bits = __ballot_sync(0xffffffffu, ok) & 0xffffu;
+        if (lane == 0) s_bits[warp][st] = bits;
+        const uint32_t base = ring_s + st * 2 * C::kTile;
+        const int c = lane % CPR;
+        const bool in = c * 8 < a.dim;
+#pragma unroll
+        for (int i = 0; i < kUnitTokens / RPP; ++i) {
+          const int r = i * RPP + lane / CPR;
+          const int64_t o = __shfl_sync(0xffffffffu, off, r) + (in ? c * 8 : 0);
+          const uint32_t bytes = in && ((bits >> r) & 1) ? 16 : 0;  // 0: the chunk is filled with zeros
+          const uint32_t d = base + r * C::kRowBytes + ((c ^ (r & 7)) << 4);
+          cp_async16(d, static_cast<const uint16_t*>(a.kc) + o, bytes);
+          cp_async16(d + C::kTile, static_cast<const uint16_t*>(a.vc) + o, bytes);
+        }
+        ++loaded;
+        if (loaded < n) {
+          cl.next(a);
+          page = lane_page(a, cl, lane);
+        }
+      }
+      cp_async_commit();
+    };
+#pragma unroll
+    for (int s = 0; s < kStages - 1; ++s) load();
+
+    uint32_t qf[C::kQSmem ? 1 : DP / 16][4];
+    float o[DP / 8][4];
+    float m0 = WR_NEG_INF, m1 = WR_NEG_INF, l0 = 0.f, l1 = 0.f;
+    int lim0 = 0, lim1 = 0, first = 0;
+    const int g8 = lane >> 2, c2 = (lane & 3) * 2;
+    for (int it = 0; it < n; ++it) {
+      __syncwarp();  // every lane has read what the next copies overwrite
+      load();
+      if (it == 0 || cc.u == 0) {  // a new piece
+        first = cc.u;
+        m0 = m1 = WR_NEG_INF;
+        l0 = l1 = 0.f;
+#pragma unroll
+        for (int d = 0; d < DP / 8; ++d) o[d][0] = o[d][1] = o[d][2] = o[d][3] = 0.f;
+        const int r0 = cc.rt * MR + g8, r1 = r0 + 8, rows = cc.s.nq * a.group;
+        const int i0 = r0 / a.group, i1 = r1 / a.group;
+        lim0 = row_limit(a, cc, i0);
+        lim1 = row_limit(a, cc, i1);
+        const uint16_t* qb = static_cast<const uint16_t*>(a.q);
+        const uint16_t* q0 = qb + (int64_t)(cc.s.q0 + i0) * a.q_ts +
+                             (int64_t)(cc.h * a.group + r0 - i0 * a.group) * a.q_hs;
+        const uint16_t* q1 = qb + (int64_t)(cc.s.q0 + i1) * a.q_ts +
+                             (int64_t)(cc.h * a.group + r1 - i1 * a.group) * a.q_hs;
+        if constexpr (C::kQSmem) {
+          for (int i = lane; i < MR * CPR; i += 32) {
+            const int r = i / CPR, c = i % CPR, rr = cc.rt * MR + r, ii = rr / a.group;
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (rr < rows && c * 8 < a.dim)
+              v = *reinterpret_cast<const uint4*>(qb + (int64_t)(cc.s.q0 + ii) * a.q_ts +
+                                                  (int64_t)(cc.h * a.group + rr - ii * a.group) * a.q_hs +
+                                                  c * 8);
+            *reinterpret_cast<uint4*>(ring + kStages * 2 * C::kTile + r * C::kRowBytes +
+                                      ((c ^ (r & 7)) << 4)) = v;
+          }
+          __syncwarp();
+        } else {
+#pragma unroll
+          for (int k = 0; k < DP / 16; ++k) {
+            const int d0 = k * 16 + c2, d1 = d0 + 8;
+            auto at = [&](const uint16_t* p, int r, int d) {
+              return r < rows && d < a.dim ? *reinterpret_cast<const uint32_t*>(p + d) : 0u;
+            };
+            qf[k][0] = at(q0, r0, d0);
+            qf[k][1] = at(q1, r1, d0);
+            qf[k][2] = at(q0, r0, d1);
+            qf[k][3] = at(q1, r1, d1);
+          }
+        }
+      }
+      cp_async_wait<kStages - 1>();
+      __syncwarp();
+      const int st = it % kStages;
+      const uint32_t kb = ring_s + st * 2 * C::kTile, vb = kb + C::kTile;
+      const uint32_t bits = s_bits[warp][st];
+      float s[2][4] = {};
+      {
+        const int r = ((lane >> 4) << 3) + (lane & 7);
+        const uint32_t row = kb + r * C::kRowBytes;
+#pragma unroll
+        for (int k = 0; k < DP / 16; ++k) {
+          uint32_t f[4];
+          ldsm4(f, row + (((2 * k + ((lane >> 3) & 1)) ^ (r & 7)) << 4));
+          if constexpr (C::kQSmem) {
+            uint32_t qq[4];
+            const int qr = lane & 15;
+            ldsm4(qq, q_s + qr * C::kRowBytes + (((2 * k + (lane >> 4)) ^ (qr & 7)) << 4));
+            mma16816(s[0], qq, f[0], f[1]);
+            mma16816(s[1], qq, f[2], f[3]);
+          } else {
+            mma16816(s[0], qf[k], f[0], f[1]);
+            mma16816(s[1], qf[k], f[2], f[3]);
+          }
+        }
+      }
+      const int j0 = cc.u * kUnitTokens;
+      float mx0 = WR_NEG_INF, mx1 = WR_NEG_INF;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int j = h * 8 + c2 + e;
+          const bool vis = (bits >> j) & 1;
+          s[h][e] = vis && j0 + j < lim0 ? s[h][e] * a.scale_log2 : WR_NEG_INF;
+          s[h][2 + e] = vis && j0 + j < lim1 ? s[h][2 + e] * a.scale_log2 : WR_NEG_INF;
+          mx0 = fmaxf(mx0, s[h][e]);
+          mx1 = fmaxf(mx1, s[h][2 + e]);
+        }
+#pragma unroll
+      for (int d = 1; d < 4; d <<= 1) {
+        mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, d));
+        mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, d));
+      }
+      if (__any_sync(0xffffffffu, mx0 > m0 || mx1 > m1)) {
+        const float n0 = fmaxf(m0, mx0), n1 = fmaxf(m1, mx1);
+        const float f0 = m0 == n0 ? 1.f : ex2(m0 - n0), f1 = m1 == n1 ? 1.f : ex2(m1 - n1);
+        m0 = n0;
+        m1 = n1;
+        l0 *= f0;
+        l1 *= f1;
+#pragma unroll
+        for (int d = 0; d < DP / 8; ++d) {
+          o[d][0] *= f0; o[d][1] *= f0;
+          o[d][2] *= f1; o[d][3] *= f1;
+        }
+      }
+      const float b0 = m0 == WR_NEG_INF ? 0.f : m0, b1 = m1 == WR_NEG_INF ? 0.f : m1;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          s[h][e] = ex2(s[h][e] - b0);
+          s[h][2 + e] = ex2(s[h][2 + e] - b1);
+          l0 += s[h][e];
+          l1 += s[h][2 + e];
+        }
+      const uint32_t p[4] = {pack_bf16(s[0][0], s[0][1]), pack_bf16(s[0][2], s[0][3]),
+                             pack_bf16(s[1][0], s[1][1]), pack_bf16(s[1][2], s[1][3])};
+      {
+        const int r = (((lane >> 3) & 1) << 3) + (lane & 7);
+        const uint32_t row = vb + r * C::kRowBytes;
+#pragma unroll
+        for (int c = 0; c < CPR; c += 2) {
+          uint32_t f[4];
+          ldsm4_t(f, row + (((c + (lane >> 4)) ^ (r & 7)) << 4));
+          mma16816(o[c], p, f[0], f[1]);
+          mma16816(o[c + 1], p, f[2], f[3]);
+        }
+      }
+      const bool tile_end = cc.u == cc.us - 1;
+      if (tile_end || it == n - 1) {  // the piece ends
+        float t0 = l0, t1 = l1;
+#pragma unroll
+        for (int d = 1; d < 4; d <<= 1) {
+          t0 += __shfl_xor_sync(0xffffffffu, t0, d);
+          t1 += __shfl_xor_sync(0xffffffffu, t1, d);
+        }
+        const bool whole = tile_end && first == 0;
+        const int rows = cc.s.nq * a.group;
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const int rl = g8 + half * 8, r = cc.rt * MR + rl;
+          if (r >= rows) continue;
+          const float mm = half ? m1 : m0, ll = half ? t1 : t0;
+          const int i = r / a.group;
+          const int64_t orow = (int64_t)(cc.s.q0 + i) * a.hq + cc.h * a.group + (r - i * a.group);
+          if (whole && a.direct) {
+            const float inv = ll > 0.f ? 1.f / ll : (ll == 0.f ? 0.f : ll);  // NaN stays
+            uint16_t* op = static_cast<uint16_t*>(a.out) + orow * a.dim;
+#pragma unroll
+            for (int d = 0; d < DP / 8; ++d)
+              if (d * 8 + c2 < a.dim)
+                *reinterpret_cast<uint32_t*>(op + d * 8 + c2) =
+                    pack_bf16(o[d][2 * half] * inv, o[d][2 * half + 1] * inv);
+            if (a.lse && (lane & 3) == 0) a.lse[orow] = ll == 0.f ? WR_NEG_INF : (mm + log2f(ll)) * kLn2;
+          } else {
+            const int64_t prow = (w * 2 + (first == 0 ? 1 : 0)) * MR + rl;
+            float* op = whole ? a.home + orow * a.dim : a.part.piece + prow * a.dim;
+#pragma unroll
+            for (int d = 0; d < DP / 8; ++d)
+              if (d * 8 + c2 < a.dim)
+                *reinterpret_cast<float2*>(op + d * 8 + c2) = make_float2(o[d][2 * half], o[d][2 * half + 1]);
+            if ((lane & 3) == 0) (whole ? a.home_ml + orow : a.part.piece_ml + prow)[0] = make_float2(mm, ll);
+          }
+        }
+      }
+      if (it + 1 < n) cc.next(a);
+    }
+    cp_async_wait<0>();
+  }
+  griddep_wait();  // this launch counts as complete only after the one before it
+}
+
+// ---------------------------------------------------------------------------
+// fp32
+// ---------------------------------------------------------------------------
+template <int DP>
+struct StreamF32Cfg {
+  static constexpr int kMR = 8;
+  static constexpr int kWarps = DP > 128 ? 2 : 4;
+  static constexpr int kRowBytes = DP * 4;
+  static constexpr int kTile = kUnitTokens * kRowBytes;
+  static constexpr int kQBytes = kMR * kRowBytes;
+  static constexpr int kPBytes = kUnitTokens * kMR * 4;
+  static constexpr int kWarpBytes = kStages * 2 * kTile + kQBytes + kPBytes;
+  static constexpr int kSmem = kWarps * kWarpBytes;
+};
+
+// Lane (t, half) of the first product: key t of the unit, half the columns;
+// of the second: DP / 32 columns, all keys.  K chunks are swizzled by key, so
+// that the 8 lanes of a 16-byte read phase meet 8 different banks; Q and the
+// weights are read by all lanes at once.
+template <int DP>
+__global__ void __launch_bounds__(StreamF32Cfg<DP>::kWarps * 32) k_attn_stream_f32(const AttnArgs a) {
+  using C = StreamF32Cfg<DP>;
+  constexpr int MR = C::kMR, CPR = DP / 4, NT = C::kWarps * 32;
+  constexpr int VC = DP / 32;  // columns of O a lane has
+  constexpr int VW = VC < 4 ? VC : 4;  // ... in runs of VW
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ ScanSmem sm;
+  __shared__ uint32_t s_bits[C::kWarps][kStages];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  griddep_launch_dependents();
+  AttnSplit sp;
+  sp.units = scan_units<MR, NT>(a, sm);
+  sp.ranges = min((int64_t)gridDim.x * C::kWarps, sp.units);
+  const int64_t w = (int64_t)warp * gridDim.x + blockIdx.x;
+  if (w < sp.ranges) {
+    const int64_t u0 = range_start(sp, w), u1 = range_start(sp, w + 1);
+    uint8_t* ring = smem + warp * C::kWarpBytes;
+    const uint32_t ring_s = smem_u32(ring);
+    float* qs = reinterpret_cast<float*>(ring + kStages * 2 * C::kTile);
+    float* ps = qs + MR * DP;
+    Cursor<MR> cl, cc;
+    cl.template seek<NT>(a, sm, u0);
+    cc = cl;
+    const int n = (int)(u1 - u0);
+    int page = lane_page(a, cl, lane);
+    int loaded = 0;
+    auto load = [&]() {
+      if (loaded < n) {
+        const int st = loaded % kStages;
+        bool ok;
+        const int64_t off = lane_offset(a, cl, page, lane, ok);
+        const uint32_t bits = __ballot_sync(0xffffffffu, ok) & 0xffffu;
+        if (lane == 0) s_bits[warp][st] = bits;
+        const uint32_t base = ring_s + st * 2 * C::kTile;
+#pragma unroll
+        for (int i = 0; i < kUnitTokens * CPR / 32; ++i) {
+          const int x = i * 32 + lane, r = x / CPR, c = x % CPR;
+          const bool in = c * 4 < a.dim;
+          const int64_t o = __shfl_sync(0xffffffffu, off, r) + (in ? c * 4 : 0);
+          const uint32_t bytes = in && ((bits >> r) & 1) ? 16 : 0;
+          const uint32_t row = base + r * C::kRowBytes;
+          cp_async16(row + ((c ^ (r & 7)) << 4), static_cast<const float*>(a.kc) + o, bytes);
+          cp_async16(row + (c << 4) + C::kTile, static_cast<const float*>(a.vc) + o, bytes);
+        }
+        ++loaded;
+        if (loaded < n) {
+          cl.next(a);
+          page = lane_page(a, cl, lane);
+        }
+      }
+      cp_async_commit();
+    };
+#pragma unroll
+    for (int s = 0; s < kStages - 1; ++s) load();
+
+    const int t = lane & 15, hf = lane >> 4;
+    float o[MR][VC], m[4], l[4];  // m, l: rows hf * 4 + 0..3
+    int lim[4], first = 0;
+    for (int it = 0; it < n; ++it) {
+      __syncwarp();
+      load();
+      const int rows = cc.s.nq * a.group;
+      if (it == 0 || cc.u == 0) {
+        first = cc.u;
+#pragma unroll
+        for (int r = 0; r < MR; ++r)
+#pragma unroll
+          for (int c = 0; c < VC; ++c) o[r][c] = 0.f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          m[e] = WR_NEG_INF;
+          l[e] = 0.f;
+          lim[e] = row_limit(a, cc, (cc.rt * MR + hf * 4 + e) / a.group);
+        }
+        for (int x = lane; x < MR * CPR; x += 32) {
+          const int r = x / CPR, c = x % CPR, rr = cc.rt * MR + r, ii = rr / a.group;
+          float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (rr < rows && c * 4 < a.dim)
+            v = *reinterpret_cast<const float4*>(static_cast<const float*>(a.q) +
+                                                 (int64_t)(cc.s.q0 + ii) * a.q_ts +
+                                                 (int64_t)(cc.h * a.group + rr - ii * a.group) * a.q_hs +
+                                                 c * 4);
+          *reinterpret_cast<float4*>(qs + r * DP + c * 4) = v;
+        }
+      }
+      cp_async_wait<kStages - 1>();
+      __syncwarp();
+      const int st = it % kStages;
+      const uint8_t* kb = ring + st * 2 * C::kTile;
+      const uint8_t* vb = kb + C::kTile;
+      const uint32_t bits = s_bits[warp][st];
+      float s[MR] = {};
+      {
+        const uint8_t* row = kb + t * C::kRowBytes;
+#pragma unroll 4
+        for (int c = 0; c < CPR / 2; ++c) {
+          const int cc2 = hf * (CPR / 2) + c;
+          const float4 k = *reinterpret_cast<const float4*>(row + ((cc2 ^ (t & 7)) << 4));
+#pragma unroll
+          for (int r = 0; r < MR; ++r) {
+            const float4 q = *reinterpret_cast<const float4*>(qs + r * DP + cc2 * 4);
+            s[r] = fmaf(q.x, k.x, s[r]);
+            s[r] = fmaf(q.y, k.y, s[r]);
+            s[r] = fmaf(q.z, k.z, s[r]);
+            s[r] = fmaf(q.w, k.w, s[r]);
+          }
+        }
+      }
+      // each half keeps its four rows
+      const int j = cc.u * kUnitTokens + t;
+      const bool vis = (bits >> t) & 1;
+      float x[4], mx[4];
+      bool up = false;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float give = hf ? s[e] : s[e + 4], keep = hf ? s[e + 4] : s[e];
+        const float sum = keep + __shfl_xor_sync(0xffffffffu, give, 16);
+        x[e] = vis && j < lim[e] ? sum * a.scale_log2 : WR_NEG_INF;
+        mx[e] = x[e];
+#pragma unroll
+        for (int d = 1; d < 16; d <<= 1) mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], d));
+        up |= mx[e] > m[e];
+      }
+      if (__any_sync(0xffffffffu, up)) {
+        float f[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float nm = fmaxf(m[e], mx[e]);
+          f[e] = nm == m[e] ? 1.f : ex2(m[e] - nm);
+          m[e] = nm;
+          l[e] *= f[e];
+        }
+#pragma unroll
+        for (int r = 0; r < MR; ++r) {
+          const float fr = __shfl_sync(0xffffffffu, f[r & 3], (r >> 2) << 4);
+#pragma unroll
+          for (int c = 0; c < VC; ++c) o[r][c] *= fr;
+        }
+      }
+      float4 pw;
+      float* pv = &pw.x;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        pv[e] = ex2(x[e] - (m[e] == WR_NEG_INF ? 0.f : m[e]));
+        l[e] += pv[e];
+      }
+      *reinterpret_cast<float4*>(ps + t * MR + hf * 4) = pw;
+      __syncwarp();
+#pragma unroll 4
+      for (int k = 0; k < kUnitTokens; ++k) {
+        const float4 pa = *reinterpret_cast<const float4*>(ps + k * MR);
+        const float4 pb = *reinterpret_cast<const float4*>(ps + k * MR + 4);
+        const float p[8] = {pa.x, pa.y, pa.z, pa.w, pb.x, pb.y, pb.z, pb.w};
+        float v[VC];
+#pragma unroll
+        for (int g = 0; g < VC; g += VW) {
+          const uint8_t* src = vb + k * C::kRowBytes + (g * 32 + lane * VW) * 4;
+          if constexpr (VW == 4) {
+            const float4 f = *reinterpret_cast<const float4*>(src);
+            v[g] = f.x; v[g + 1] = f.y; v[g + 2] = f.z; v[g + 3] = f.w;
+          } else {
+            const float2 f = *reinterpret_cast<const float2*>(src);
+            v[g] = f.x; v[g + 1] = f.y;
+          }
+        }
+#pragma unroll
+        for (int r = 0; r < MR; ++r)
+#pragma unroll
+          for (int c = 0; c < VC; ++c) o[r][c] = fmaf(p[r], v[c], o[r][c]);
+      }
+      const bool tile_end = cc.u == cc.us - 1;
+      if (tile_end || it == n - 1) {
+        float ls[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          ls[e] = l[e];
+#pragma unroll
+          for (int d = 1; d < 16; d <<= 1) ls[e] += __shfl_xor_sync(0xffffffffu, ls[e], d);
+        }
+        const bool whole = tile_end && first == 0;
+#pragma unroll
+        for (int r = 0; r < MR; ++r) {
+          const float mm = __shfl_sync(0xffffffffu, m[r & 3], (r >> 2) << 4);
+          const float ll = __shfl_sync(0xffffffffu, ls[r & 3], (r >> 2) << 4);
+          const int rr = cc.rt * MR + r;
+          if (rr >= rows) continue;
+          const int i = rr / a.group;
+          const int64_t orow = (int64_t)(cc.s.q0 + i) * a.hq + cc.h * a.group + (rr - i * a.group);
+          const int64_t prow = (w * 2 + (first == 0 ? 1 : 0)) * MR + r;
+          const bool fin = whole && a.direct;
+          const float inv = !fin ? 1.f : (ll > 0.f ? 1.f / ll : (ll == 0.f ? 0.f : ll));
+          float* op = fin ? static_cast<float*>(a.out) + orow * a.dim
+                          : (whole ? a.home + orow * a.dim : a.part.piece + prow * a.dim);
+#pragma unroll
+          for (int g = 0; g < VC; g += VW) {
+            const int d = g * 32 + lane * VW;
+            if (d < a.dim)
+#pragma unroll
+              for (int c = 0; c < VW; ++c) op[d + c] = o[r][g + c] * inv;
+          }
+          if (lane == 0) {
+            if (!fin) (whole ? a.home_ml + orow : a.part.piece_ml + prow)[0] = make_float2(mm, ll);
+            else if (a.lse) a.lse[orow] = ll == 0.f ? WR_NEG_INF : (mm + log2f(ll)) * kLn2;
+          }
+        }
+      }
+      if (it + 1 < n) cc.next(a);
+    }
+    cp_async_wait<0>();
+  }
+  griddep_wait();
+}
+
+// ---------------------------------------------------------------------------
+// Joining the pieces
+// ---------------------------------------------------------------------------
+struct CombineArgs {
+  AttnArgs own;       // the launch over the sequences' own keys
+  int64_t own_warps;
+  AttnArgs pre;       // the launch over the prefix (pre_kind == 1)
+  int64_t pre_warps;
+  int pre_kind;       // 0: none, 1: k_attn_stream*, 2: splits [splits][rows of all tokens][dim]
+  const float* split;
+  const float2* split_ml;
+  int splits;
+  int64_t split_rows;
+};
+
+// The pieces of a row of one launch: piece i of `n` lies at row(i).
+struct PieceList {
+  int64_t w0;
+  int n, rl, mr;
+  bool whole;
+};
+template <int MR>
+WR_DEVINL PieceList piece_list(const AttnSplit& sp, int64_t unit0, int us, int r) {
+  PieceList p;
+  const int64_t w0 = range_of(sp, unit0), w1 = range_of(sp, unit0 + us - 1);
+  p.whole = w0 == w1;
+  p.w0 = w0;
+  p.n = (int)(w1 - w0) + 1;
+  p.rl = r % MR;
+  p.mr = MR;
+  return p;
+}
+
+template <typename T, int MR, int DP, int kWarps>
+__global__ void __launch_bounds__(kWarps == 1 ? 128 : kWarps * 32) k_attn_combine(const CombineArgs c) {
+  constexpr int VC = DP / 32;
+  constexpr int VW = VC < 4 ? VC : 4;
+  constexpr int kRowsCta = kWarps == 1 ? 4 : 1;
+  __shared__ float s_o[kWarps > 1 ? kWarps : 1][DP];
+  __shared__ float2 s_ml[kWarps > 1 ? kWarps : 1];
+  const AttnArgs& a = c.own;
+  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
+  const int64_t row = (int64_t)blockIdx.x * kRowsCta + (kWarps == 1 ? wid : 0);
+  griddep_wait();
+  if (row >= (int64_t)a.T * a.hq) return;  // uniform over a row's warps
+  const int t = (int)(row / a.hq), hq = (int)(row - (int64_t)t * a.hq);
+  const int h = hq / a.group, g = hq - h * a.group;
+  const int b = a.q_start ? a.token_seq[t] : t;
+  PieceList po{}, pp{};
+  bool done = false;
+  if (b >= 0) {
+    const SeqInfo s = seq_info(a, b);
+    const int us = key_units(a, s), rts = row_tiles<MR>(a, s);
+    AttnSplit sp;
+    sp.units = a.seq_unit[a.B];
+    sp.ranges = min(c.own_warps, sp.units);
+    const int r = (t - s.q0) * a.group + g;
+    po = piece_list<MR>(sp, a.seq_unit[b] + ((int64_t)h * rts + r / MR) * us, us, r);
+    done = po.whole && a.direct;
+  }
+  if (done) return;  // written by the first kernel
+  if (c.pre_kind == 1 && b >= 0) {
+    const SeqInfo s = seq_info(c.pre, 0);
+    const int us = key_units(c.pre, s), rts = row_tiles<MR>(c.pre, s);
+    AttnSplit sp;
+    sp.units = (int64_t)a.hkv * rts * us;
+    sp.ranges = min(c.pre_warps, sp.units);
+    const int r = t * a.group + g;
+    pp = piece_list<MR>(sp, ((int64_t)h * rts + r / MR) * us, us, r);
+  } else if (c.pre_kind == 2 && b >= 0) {
+    pp.n = c.splits;
+  }
+  const int total = po.n + pp.n;
+  float m = WR_NEG_INF, l = 0.f, o[VC];
+#pragma unroll
+  for (int i = 0; i < VC; ++i) o[i] = 0.f;
+  const int64_t prow = (int64_t)h * c.split_rows + (int64_t)t * a.group + g;
+#pragma unroll 4
+  for (int i = kWarps == 1 ? 0 : wid; i < total; i += kWarps) {
+    const float* src;
+    float2 ml;
+    if (i < po.n || c.pre_kind == 1) {
+      const bool mine = i < po.n;
+      const PieceList& p = mine ? po : pp;
+      const AttnArgs& x = mine ? a : c.pre;
+      const int k = mine ? i : i - po.n;
+      if (p.whole) {
+        src = x.home + row * a.dim;
+        ml = x.home_ml[row];
+      } else {
+        const int64_t at = ((p.w0 + k) * 2 + (k == 0 ? 1 : 0)) * MR + p.rl;
+        src = x.part.piece + at * a.dim;
+        ml = x.part.piece_ml[at];
+      }
+    } else {
+      const int64_t at = (int64_t)(i - po.n) * a.hkv * c.split_rows + prow;
+      src = c.split + at * a.dim;
+      ml = c.split_ml[at];
+    }
+    const float nm = fmaxf(m, ml.x);
+    const float base = nm == WR_NEG_INF ? 0.f : nm;
+    const float fo = ex2(m - base), fn = ex2(ml.x - base);
+    m = nm;
+    l = l * fo + ml.y * fn;
+#pragma unroll
+    for (int q = 0; q < VC; q += VW) {
+      const int d = q * 32 + lane * VW;
+#pragma unroll
+      for (int e = 0; e < VW; ++e) o[q + e] = o[q + e] * fo + (d < a.dim ? src[d + e] : 0.f) * fn;
+    }
+  }
+  if constexpr (kWarps > 1) {
+#pragma unroll
+    for (int q = 0; q < VC; q += VW)
+#pragma unroll
+      for (int e = 0; e < VW; ++e) s_o[wid][q * 32 + lane * VW + e] = o[q + e];
+    if (lane == 0) s_ml[wid] = make_float2(m, l);
+    __syncthreads();
+    if (wid) return;
+    m = WR_NEG_INF;
+    for (int i = 0; i < kWarps; ++i) m = fmaxf(m, s_ml[i].x);
+    const float base = m == WR_NEG_INF ? 0.f : m;
+    l = 0.f;
+#pragma unroll
+    for (int q = 0; q < VC; ++q) o[q] = 0.f;
+    for (int i = 0; i < kWarps; ++i) {
+      const float f = ex2(s_ml[i].x - base);
+      l += s_ml[i].y * f;
+#pragma unroll
+      for (int q = 0; q < VC; q += VW)
+#pragma unroll
+        for (int e = 0; e < VW; ++e) o[q + e] += s_o[i][q * 32 + lane * VW + e] * f;
+    }
+  }
+  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+#pragma unroll
+  for (int q = 0; q < VC; q += VW) {
+    const int d = q * 32 + lane * VW;
+    if (d >= a.dim) continue;
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+      for (int e = 0; e < VW; e += 2)
+        *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.out) + row * a.dim + d + e) =
+            pack_bf16(o[q + e] * inv, o[q + e + 1] * inv);
+    } else {
+#pragma unroll
+      for (int e = 0; e < VW; ++e) static_cast<float*>(a.out)[row * a.dim + d + e] = o[q + e] * inv;
+    }
+  }
+  if (a.lse && lane == 0) a.lse[row] = l == 0.f ? WR_NEG_INF : (m + log2f(l)) * kLn2;
+}
+
+// ---------------------------------------------------------------------------
+// Host
+// ---------------------------------------------------------------------------
+struct Plan {
+  int dp, mr, warps_cta, smem;
+  int own_grid, pre_grid;
+  int pre_kind;      // see CombineArgs
+  int inline_prefix; // each sequence reads the prefix with its own keys
+  int64_t rows;      // T * hq
+  size_t off_piece, off_piece_ml, off_home, off_home_ml, off_seq, off_tok;
+  size_t off_ppiece, off_ppiece_ml, off_phome, off_phome_ml;
+  size_t bytes;
+};
+
+Plan make_plan(const AttnProblem& p) {
+  Plan pl{};
+  const bool f32 = p.c.dtype == WR_DTYPE_F32;
+  pl.dp = p.c.dim <= 64 ? 64 : (p.c.dim <= 128 ? 128 : 256);
+  pl.mr = f32 ? 8 : 16;
+  pl.warps_cta = f32 && pl.dp > 128 ? 2 : kStreamWarps;
+  pl.smem = f32 ? (pl.dp == 64 ? StreamF32Cfg<64>::kSmem : pl.dp == 128 ? StreamF32Cfg<128>::kSmem : StreamF32Cfg<256>::kSmem)
+                : (pl.dp == 64 ? StreamCfg<64>::kSmem : pl.dp == 128 ? StreamCfg<128>::kSmem : StreamCfg<256>::kSmem);
+  const int per_sm = 228 * 1024 / (pl.smem + 4096) < 1 ? 1 : (228 * 1024 / (pl.smem + 4096) > 4 ? 4 : 228 * 1024 / (pl.smem + 4096));
+  const int64_t most = (int64_t)device_sm_count() * per_sm;
+  const int group = p.hq / p.c.hkv;
+  pl.rows = (int64_t)p.T * p.hq;
+  pl.inline_prefix = p.prefix_len > 0 && p.B == 1;
+  pl.pre_kind = p.prefix_len > 0 && !pl.inline_prefix ? 1 : 0;
+  // An upper bound of the units: the lengths are on the device.
+  const int64_t keys = (int64_t)p.table_width * p.c.page_size + (pl.inline_prefix ? p.prefix_len : 0);
+  const int64_t tiles = ((int64_t)p.T * group + pl.mr - 1) / pl.mr + (p.B > 0 ? p.B : 0);
+  const int64_t units = (tiles * p.c.hkv) * ((keys + kUnitTokens - 1) / kUnitTokens + 1);
+  const int64_t ctas = (units + pl.warps_cta - 1) / pl.warps_cta;
+  pl.own_grid = (int)(ctas < most ? (ctas < 1 ? 1 : ctas) : most);
+  size_t at = 0;
+  auto take = [&](size_t n) {
+    const size_t o = at;
+    at += (n + 255) & ~(size_t)255;
+    return o;
+  };
+  const size_t own_rows = (size_t)pl.own_grid * pl.warps_cta * 2 * pl.mr;
+  pl.off_piece = take(own_rows * p.c.dim * 4);
+  pl.off_piece_ml = take(own_rows * 8);
+  if (pl.pre_kind) {
+    pl.off_home = take((size_t)pl.rows * p.c.dim * 4);
+    pl.off_home_ml = take((size_t)pl.rows * 8);
+  }
+  pl.off_seq = take((size_t)(p.B + 1) * 8);
+  pl.off_tok = take((size_t)(p.q_start ? p.T : 0) * 4);
+  if (pl.pre_kind == 1) {
+    const int64_t pu = (int64_t)p.c.hkv * (((int64_t)p.T * group + pl.mr - 1) / pl.mr) *
+                       ((p.prefix_len + kUnitTokens - 1) / kUnitTokens);
+    const int64_t pc = (pu + pl.warps_cta - 1) / pl.warps_cta;
+    pl.pre_grid = (int)(pc < most ? pc : most);
+    const size_t pre_rows = (size_t)pl.pre_grid * pl.warps_cta * 2 * pl.mr;
+    pl.off_ppiece = take(pre_rows * p.c.dim * 4);
+    pl.off_ppiece_ml = take(pre_rows * 8);
+    pl.off_phome = take((size_t)pl.rows * p.c.dim * 4);
+    pl.off_phome_ml = take((size_t)pl.rows * 8);
+  }
+  pl.bytes = at;
+  return pl;
+}
+
+template <typename K>
+cudaError_t launch_one(K kernel, int64_t grid, int threads, int smem, bool pdl, cudaStream_t stream,
+                       const void* args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = pdl ? 1 : 0;
+  void* ptrs[1] = {const_cast<void*>(args)};
+  if (smem > 0) {
+    const cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                               cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+  }
+  return cudaLaunchKernelExC(&cfg, reinterpret_cast<const void*>(kernel), ptrs);
+}
+
+cudaError_t launch_stream(const Plan& pl, bool f32, const AttnArgs& a, int grid, bool pdl, cudaStream_t s) {
+  const int th = pl.warps_cta * 32;
+  if (f32) {
+    if (pl.dp == 64) return launch_one(k_attn_stream_f32<64>, grid, th, pl.smem, pdl, s, &a);
+    if (pl.dp == 128) return launch_one(k_attn_stream_f32<128>, grid, th, pl.smem, pdl, s, &a);
+    return launch_one(k_attn_stream_f32<256>, grid, th, pl.smem, pdl, s, &a);
+  }
+  if (pl.dp == 64) return launch_one(k_attn_stream<64>, grid, th, pl.smem, pdl, s, &a);
+  if (pl.dp == 128) return launch_one(k_attn_stream<128>, grid, th, pl.smem, pdl, s, &a);
+  return launch_one(k_attn_stream<256>, grid, th, pl.smem, pdl, s, &a);
+}
+
+template <typename T, int MR, int W>
+cudaError_t launch_combine_dp(int dp, const CombineArgs& c, int64_t grid, cudaStream_t s) {
+  constexpr int th = W == 1 ? 128 : W * 32;
+  if (dp == 64) return launch_one(k_attn_combine<T, MR, 64, W>, grid, th, 0, true, s, &c);
+  if (dp == 128) return launch_one(k_attn_combine<T, MR, 128, W>, grid, th, 0, true, s, &c);
+  return launch_one(k_attn_combine<T, MR, 256, W>, grid, th, 0, true, s, &c);
+}
+
+}  // namespace
+
+size_t attn_workspace_bytes(const AttnProblem& p) { return make_plan(p).bytes; }
+
+wr_status_t launch_attn(const AttnProblem& p, void* ws, cudaStream_t stream) {
+  const Plan pl = make_plan(p);
+  const bool f32 = p.c.dtype == WR_DTYPE_F32;
+  uint8_t* base = static_cast<uint8_t*>(ws);
+  AttnArgs a{};
+  a.q = p.q; a.kc = p.c.k; a.vc = p.c.v;
+  a.q_ts = p.q_ts; a.q_hs = p.q_hs;
+  a.page_stride = p.c.page_stride; a.head_stride = p.c.head_stride; a.slot_stride = p.c.slot_stride;
+  a.tables = p.tables; a.table_stride = p.table_stride; a.lens = p.lens; a.q_start = p.q_start;
+  a.prefix_pages = p.prefix_pages;
+  a.num_pages = p.c.num_pages; a.page_size = p.c.page_size;
+  a.page_shift = (p.c.page_size & (p.c.page_size - 1)) == 0 ? __builtin_ctz(p.c.page_size) : -1;
+  a.T = p.T; a.B = p.B; a.hq = p.hq; a.hkv = p.c.hkv; a.group = p.hq / p.c.hkv; a.dim = p.c.dim;
+  a.table_width = p.table_width;
+  a.prefix = pl.inline_prefix ? p.prefix_len : 0;
+  a.own = 1;
+  a.direct = pl.pre_kind == 0;
+  a.scale_log2 = p.scale * kLog2e;
+  a.part.piece = reinterpret_cast<float*>(base + pl.off_piece);
+  a.part.piece_ml = reinterpret_cast<float2*>(base + pl.off_piece_ml);
+  a.home = reinterpret_cast<float*>(base + pl.off_home);
+  a.home_ml = reinterpret_cast<float2*>(base + pl.off_home_ml);
+  a.seq_unit = reinterpret_cast<int64_t*>(base + pl.off_seq);
+  a.token_seq = reinterpret_cast<int32_t*>(base + pl.off_tok);
+  a.out = p.out; a.lse = p.lse;
+  CombineArgs c{};
+  c.own = a;
+  c.own_warps = (int64_t)pl.own_grid * pl.warps_cta;
+  c.pre_kind = pl.pre_kind;
+  cudaError_t e;
+  if (pl.pre_kind == 1) {
+    AttnArgs x = a;
+    x.B = 1; x.own = 0; x.prefix = p.prefix_len; x.direct = 0; x.q_start = nullptr;
+    x.part.piece = reinterpret_cast<float*>(base + pl.off_ppiece);
+    x.part.piece_ml = reinterpret_cast<float2*>(base + pl.off_ppiece_ml);
+    x.home = reinterpret_cast<float*>(base + pl.off_phome);
+    x.home_ml = reinterpret_cast<float2*>(base + pl.off_phome_ml);
+    c.pre = x;
+    c.pre_warps = (int64_t)pl.pre_grid * pl.warps_cta;
+    e = launch_stream(pl, f32, x, pl.pre_grid, false, stream);
+    if (e != cudaSuccess) return cuda_fail(e, "shared_prefix_attention (prefix) launch");
+  }
+  e = launch_stream(pl, f32, a, pl.own_grid, pl.pre_kind != 0, stream);
+  if (e != cudaSuccess) return cuda_fail(e, "shared_prefix_attention launch");
+  // Few rows: 8 warps a row read its many pieces; many rows: a warp each.
+  const bool wide = pl.rows <= (int64_t)device_sm_count() * 8;
+  const int64_t grid = wide ? pl.rows : (pl.rows + 3) / 4;
+  if (f32)
+    e = wide ? launch_combine_dp<float, 8, 8>(pl.dp, c, grid, stream)
+             : launch_combine_dp<float, 8, 1>(pl.dp, c, grid, stream);
+  else
+    e = wide ? launch_combine_dp<uint16_t, 16, 8>(pl.dp, c, grid, stream)
+             : launch_combine_dp<uint16_t, 16, 1>(pl.dp, c, grid, stream);
+  return e == cudaSuccess ? WR_OK : cuda_fail(e, "shared_prefix_attention (join) launch");
+}
+
+}  // namespace wr

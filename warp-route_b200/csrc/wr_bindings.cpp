@@ -15,6 +15,7 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 
+#include <algorithm>
 #include <map>
 #include <mutex>
 #include <tuple>
@@ -406,6 +407,202 @@ torch::Tensor pack_experts(const std::vector<torch::Tensor>& gate,
   return buf;
 }
 
+// ---- paged cache, shared-prefix attention, sampling --------------------------
+
+void check_on(const torch::Tensor& t, const char* name, const torch::Tensor& ref, const char* ref_name) {
+  TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor");
+  TORCH_CHECK(t.device() == ref.device(), name, " and ", ref_name, " must be on the same device");
+}
+
+void check_list(const torch::Tensor& t, const char* name, torch::ScalarType type, int64_t n,
+                const torch::Tensor& ref, const char* ref_name) {
+  check_on(t, name, ref, ref_name);
+  TORCH_CHECK(t.scalar_type() == type, name, " must be ", type, ", got ", t.scalar_type());
+  TORCH_CHECK(t.dim() == 1 && t.size(0) == n, name, " must have shape [", n, "], got shape ", t.sizes());
+  TORCH_CHECK(t.is_contiguous(), name, " must be contiguous");
+}
+
+// A length of one has no stride that counts: 0 is as good as any.
+int64_t stride_of(const torch::Tensor& t, int d) { return t.size(d) > 1 ? t.stride(d) : 0; }
+
+int32_t narrow(int64_t v, const char* what) {
+  TORCH_CHECK(v >= 0 && v <= INT32_MAX, what, " is out of range: ", v);
+  return (int32_t)v;
+}
+
+wr_paged_kv_t make_cache(const torch::Tensor& k, const torch::Tensor& v) {
+  TORCH_CHECK(k.is_cuda(), "k_cache must be a CUDA tensor");
+  TORCH_CHECK(k.scalar_type() == torch::kFloat32 || k.scalar_type() == torch::kBFloat16,
+              "k_cache must be float32 or bfloat16");
+  TORCH_CHECK(k.dim() == 4, "k_cache must have shape [num_pages, num_kv_heads, page_size, head_dim], got shape ",
+              k.sizes());
+  check_same(k, v, "k_cache", "v_cache");
+  TORCH_CHECK(v.sizes() == k.sizes() && v.strides() == k.strides(),
+              "v_cache must have k_cache's shape and strides, got shape ", v.sizes(), " and ", k.sizes());
+  TORCH_CHECK(k.stride(3) == 1 || k.size(3) == 1, "the caches' last dimension must be contiguous");
+  wr_paged_kv_t c{};
+  c.k = k.data_ptr();
+  c.v = v.data_ptr();
+  c.page_stride = stride_of(k, 0);
+  c.head_stride = stride_of(k, 1);
+  c.slot_stride = stride_of(k, 2);
+  c.num_pages = narrow(k.size(0), "num_pages");
+  c.num_kv_heads = narrow(k.size(1), "num_kv_heads");
+  c.page_size = narrow(k.size(2), "page_size");
+  c.head_dim = narrow(k.size(3), "head_dim");
+  c.dtype = dtype_code(k);
+  return c;
+}
+
+wr_rows_t make_rows(const torch::Tensor& t, const char* name, int64_t tokens, int64_t heads,
+                    const torch::Tensor& cache) {
+  check_on(t, name, cache, "k_cache");
+  TORCH_CHECK(t.scalar_type() == cache.scalar_type(), name, " and k_cache must have the same dtype, got ",
+              t.scalar_type(), " and ", cache.scalar_type());
+  TORCH_CHECK(t.dim() == 3 && t.size(0) == tokens && (heads < 0 || t.size(1) == heads) &&
+                  t.size(2) == cache.size(3),
+              name, " must have shape [", tokens, ", ", heads < 0 ? std::string("heads") : std::to_string(heads),
+              ", ", cache.size(3), "], got shape ", t.sizes());
+  TORCH_CHECK(t.stride(2) == 1, name, "'s last dimension must be contiguous");
+  return wr_rows_t{t.data_ptr(), stride_of(t, 0), stride_of(t, 1)};
+}
+
+// Writes k and v into the caches, in place; returns the rotated q or None.
+c10::optional<torch::Tensor> append_paged_kv(torch::Tensor k, torch::Tensor v, torch::Tensor k_cache,
+                                             torch::Tensor v_cache, torch::Tensor slots,
+                                             c10::optional<torch::Tensor> positions,
+                                             c10::optional<torch::Tensor> inv_freq,
+                                             c10::optional<torch::Tensor> q, bool interleaved) {
+  const wr_paged_kv_t cache = make_cache(k_cache, v_cache);
+  TORCH_CHECK(k.dim() == 3, "k must have shape [tokens, heads, head_dim], got shape ", k.sizes());
+  const int64_t T = k.size(0);
+  const wr_rows_t kr = make_rows(k, "k", T, k_cache.size(1), k_cache);
+  const wr_rows_t vr = make_rows(v, "v", T, k_cache.size(1), k_cache);
+  check_list(slots, "slots", torch::kInt64, T, k_cache, "k_cache");
+  TORCH_CHECK(positions.has_value() == inv_freq.has_value(), "positions and inv_freq go together");
+  int32_t rot = 0;
+  if (positions.has_value()) {
+    check_list(*positions, "positions", torch::kInt64, T, k_cache, "k_cache");
+    TORCH_CHECK(inv_freq->dim() == 1, "inv_freq must have shape [rot_dim / 2], got shape ", inv_freq->sizes());
+    check_list(*inv_freq, "inv_freq", torch::kFloat32, inv_freq->size(0), k_cache, "k_cache");
+    rot = narrow(2 * inv_freq->size(0), "rot_dim");
+  }
+  const c10::cuda::CUDAGuard guard(k_cache.device());
+  cudaStream_t stream = at::cuda::getCurrentCUDAStream(k_cache.device().index()).stream();
+  wr_rows_t qr{};
+  torch::Tensor out;
+  int32_t hq = 0;
+  if (q.has_value()) {
+    qr = make_rows(*q, "q", T, -1, k_cache);
+    hq = narrow(q->size(1), "num_q_heads");
+    out = torch::empty({T, hq, k_cache.size(3)}, k_cache.options());
+    if (out.numel() == 0) return out;
+  }
+  check_status(wr_append_paged_kv(&cache, narrow(T, "num_tokens"), &kr, &vr, slots.data_ptr<int64_t>(),
+                                  rot ? positions->data_ptr<int64_t>() : nullptr,
+                                  rot ? inv_freq->data_ptr<float>() : nullptr, rot, interleaved ? 1 : 0, hq,
+                                  q.has_value() ? &qr : nullptr, q.has_value() ? out.data_ptr() : nullptr,
+                                  stream));
+  if (!q.has_value()) return c10::nullopt;
+  return out;
+}
+
+std::tuple<torch::Tensor, c10::optional<torch::Tensor>> shared_prefix_attention(
+    torch::Tensor q, torch::Tensor k_cache, torch::Tensor v_cache, torch::Tensor block_tables,
+    torch::Tensor context_lens, c10::optional<torch::Tensor> prefix_pages, int64_t prefix_len,
+    c10::optional<torch::Tensor> q_start, double scale, bool want_lse) {
+  const wr_paged_kv_t cache = make_cache(k_cache, v_cache);
+  TORCH_CHECK(q.dim() == 3, "q must have shape [tokens, heads, head_dim], got shape ", q.sizes());
+  const int64_t T = q.size(0);
+  const wr_rows_t qr = make_rows(q, "q", T, -1, k_cache);
+  check_on(block_tables, "block_tables", k_cache, "k_cache");
+  TORCH_CHECK(block_tables.scalar_type() == torch::kInt32, "block_tables must be ", torch::kInt32, ", got ",
+              block_tables.scalar_type());
+  TORCH_CHECK(block_tables.dim() == 2, "block_tables must have shape [num_seqs, pages], got shape ",
+              block_tables.sizes());
+  TORCH_CHECK(block_tables.size(1) <= 1 || block_tables.stride(1) == 1,
+              "block_tables' last dimension must be contiguous");
+  const int64_t B = block_tables.size(0);
+  check_list(context_lens, "context_lens", torch::kInt32, B, k_cache, "k_cache");
+  if (q_start.has_value()) check_list(*q_start, "q_start", torch::kInt32, B + 1, k_cache, "k_cache");
+  else TORCH_CHECK(T == B, "without q_start q must have one token a sequence, got ", T, " tokens and ", B,
+                   " sequences");
+  TORCH_CHECK(prefix_len >= 0, "prefix_len must be >= 0, got ", prefix_len);
+  if (prefix_len > 0) {
+    TORCH_CHECK(prefix_pages.has_value(), "prefix_pages must be given when prefix_len > 0");
+    check_list(*prefix_pages, "prefix_pages", torch::kInt32, prefix_pages->size(0), k_cache, "k_cache");
+    TORCH_CHECK(prefix_pages->size(0) * k_cache.size(2) >= prefix_len, "prefix_pages holds ",
+                prefix_pages->size(0), " pages of ", k_cache.size(2), ", too few for prefix_len ", prefix_len);
+  }
+  wr_attn_desc_t d{};
+  d.num_tokens = narrow(T, "num_tokens");
+  d.num_seqs = narrow(B, "num_seqs");
+  d.num_q_heads = narrow(q.size(1), "num_q_heads");
+  d.table_width = narrow(block_tables.size(1), "table_width");
+  d.table_stride = stride_of(block_tables, 0);
+  d.prefix_len = narrow(prefix_len, "prefix_len");
+  d.scale = (float)scale;
+  const c10::cuda::CUDAGuard guard(k_cache.device());
+  cudaStream_t stream = at::cuda::getCurrentCUDAStream(k_cache.device().index()).stream();
+  torch::Tensor out = torch::empty({T, q.size(1), q.size(2)}, k_cache.options());
+  c10::optional<torch::Tensor> lse;
+  if (want_lse) lse = torch::empty({T, q.size(1)}, k_cache.options().dtype(torch::kFloat32));
+  const size_t need = wr_shared_prefix_attention_workspace_size(&cache, &d, q_start.has_value() ? 1 : 0);
+  TORCH_CHECK(need > 0, wr_last_error_string());
+  if (T == 0) return {out, lse};
+  // From torch's allocator for this call alone: in a captured graph it is the
+  // graph's own memory, so two graphs never share one.
+  torch::Tensor ws = torch::empty({(int64_t)need}, k_cache.options().dtype(torch::kUInt8));
+  check_status(wr_shared_prefix_attention(
+      &cache, &d, &qr, block_tables.data_ptr<int32_t>(), context_lens.data_ptr<int32_t>(),
+      q_start.has_value() ? q_start->data_ptr<int32_t>() : nullptr,
+      prefix_len > 0 ? prefix_pages->data_ptr<int32_t>() : nullptr, out.data_ptr(),
+      want_lse ? lse->data_ptr<float>() : nullptr, ws.data_ptr(), need, stream));
+  return {out, lse};
+}
+
+// Each setting: its number, or a tensor with one for each row.
+torch::Tensor sample_tokens(torch::Tensor logits, torch::Tensor uniforms, double temperature,
+                            c10::optional<torch::Tensor> temperatures, int64_t top_k,
+                            c10::optional<torch::Tensor> top_ks, double top_p,
+                            c10::optional<torch::Tensor> top_ps, double min_p,
+                            c10::optional<torch::Tensor> min_ps) {
+  CHECK_CUDA(logits);
+  CHECK_DTYPE(logits);
+  TORCH_CHECK(logits.dim() == 2, "logits must have shape [rows, vocab], got shape ", logits.sizes());
+  TORCH_CHECK(logits.stride(1) == 1 || logits.size(1) == 1, "logits' last dimension must be contiguous");
+  const int64_t R = logits.size(0);
+  check_list(uniforms, "uniforms", torch::kFloat32, R, logits, "logits");
+  wr_sampling_t s{};
+  s.temperature = (float)temperature;
+  s.top_p = (float)top_p;
+  s.min_p = (float)min_p;
+  s.top_k = (int32_t)std::min<int64_t>(std::max<int64_t>(top_k, 0), INT32_MAX);
+  if (temperatures.has_value()) {
+    check_list(*temperatures, "temperature", torch::kFloat32, R, logits, "logits");
+    s.temperatures = temperatures->data_ptr<float>();
+  }
+  if (top_ps.has_value()) {
+    check_list(*top_ps, "top_p", torch::kFloat32, R, logits, "logits");
+    s.top_ps = top_ps->data_ptr<float>();
+  }
+  if (min_ps.has_value()) {
+    check_list(*min_ps, "min_p", torch::kFloat32, R, logits, "logits");
+    s.min_ps = min_ps->data_ptr<float>();
+  }
+  if (top_ks.has_value()) {
+    check_list(*top_ks, "top_k", torch::kInt32, R, logits, "logits");
+    s.top_ks = top_ks->data_ptr<int32_t>();
+  }
+  const c10::cuda::CUDAGuard guard(logits.device());
+  cudaStream_t stream = at::cuda::getCurrentCUDAStream(logits.device().index()).stream();
+  torch::Tensor ids = torch::empty({R}, logits.options().dtype(torch::kInt64));
+  check_status(wr_sample_tokens(R, narrow(logits.size(1), "vocab"), dtype_code(logits), logits.data_ptr(),
+                                stride_of(logits, 0), uniforms.data_ptr<float>(), &s,
+                                ids.data_ptr<int64_t>(), stream));
+  return ids;
+}
+
 int64_t workspace_status(torch::Tensor hidden) {
   // Reads and clears the status word of this device/stream's cached workspace.
   const c10::cuda::CUDAGuard guard(hidden.device());
@@ -456,6 +653,21 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("pack_experts", &pack_experts,
         "Pack one rank's shard (experts, intermediate slice) of per-expert weights on the "
         "device");
+  m.def("append_paged_kv", &append_paged_kv,
+        "Keys and values into a paged cache, rotated by position; returns the rotated q",
+        py::arg("k"), py::arg("v"), py::arg("k_cache"), py::arg("v_cache"), py::arg("slots"),
+        py::arg("positions") = py::none(), py::arg("inv_freq") = py::none(),
+        py::arg("q") = py::none(), py::arg("interleaved") = false);
+  m.def("shared_prefix_attention", &shared_prefix_attention,
+        "Attention of a batch over a paged cache with a prefix shared by all: (out, lse or None)",
+        py::arg("q"), py::arg("k_cache"), py::arg("v_cache"), py::arg("block_tables"),
+        py::arg("context_lens"), py::arg("prefix_pages"), py::arg("prefix_len"),
+        py::arg("q_start"), py::arg("scale"), py::arg("return_lse"));
+  m.def("sample_tokens", &sample_tokens,
+        "A token for each row of logits by temperature, top-k, top-p and min-p",
+        py::arg("logits"), py::arg("uniforms"), py::arg("temperature"), py::arg("temperatures"),
+        py::arg("top_k"), py::arg("top_ks"), py::arg("top_p"), py::arg("top_ps"),
+        py::arg("min_p"), py::arg("min_ps"));
   m.def("workspace_status", &workspace_status,
         "Read and clear the device status word of the current stream's workspace");
   m.def("version", []() { return std::string(wr_version()); });

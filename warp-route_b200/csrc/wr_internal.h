@@ -95,6 +95,59 @@ wr_status_t launch_naive(const Problem& p, const void* x, const void* gate_w,
                          const void* wbuf, float* out, int32_t* ids, float* w,
                          void* ws, cudaStream_t stream);
 
+// ---- paged key/value cache (wr_kvcache.cu, wr_attention.cu) ----
+// A checked wr_paged_kv: strides in elements.
+struct PagedKv {
+  void *k, *v;
+  int64_t page_stride, head_stride, slot_stride;
+  int num_pages, hkv, page_size, dim, dtype;
+};
+
+struct AppendProblem {
+  PagedKv c;
+  int T, hq, rot, interleaved;
+  const void *k, *v, *q;
+  int64_t k_ts, k_hs, v_ts, v_hs, q_ts, q_hs;  // token and head strides, elements
+  const int64_t* slots;
+  const int64_t* positions;  // null: no rotation (rot = 0)
+  const float* inv_freq;
+  void* q_out;
+};
+wr_status_t launch_append(const AppendProblem& p, cudaStream_t stream);
+
+struct AttnProblem {
+  PagedKv c;
+  int T, B, hq, table_width, prefix_len;
+  float scale;
+  const void* q;
+  int64_t q_ts, q_hs;
+  const int32_t* tables;  // [B, table_width], rows table_stride apart
+  int64_t table_stride;
+  const int32_t* lens;         // [B]
+  const int32_t* q_start;      // [B + 1], or null: one token a sequence
+  const int32_t* prefix_pages; // [ceil(prefix_len / page_size)]
+  void* out;                   // [T, hq, dim] in the cache's type
+  float* lse;                  // [T, hq], or null
+};
+size_t attn_workspace_bytes(const AttnProblem& p);
+wr_status_t launch_attn(const AttnProblem& p, void* ws, cudaStream_t stream);
+
+// ---- sampling (wr_sample.cu) ----
+constexpr int kSampleMaxVocab = 8 * 512 * 64;  // what a cluster of 8 CTAs of 512 threads keeps, 64 values a thread
+struct SampleProblem {
+  int64_t rows;
+  int vocab, dtype;
+  const void* logits;
+  int64_t row_stride;  // elements
+  const float* uniforms;
+  const float *temperatures, *top_ps, *min_ps;  // [rows], or null: the numbers
+  const int32_t* top_ks;
+  float temperature, top_p, min_p;
+  int32_t top_k;
+  int64_t* ids;
+};
+wr_status_t launch_sample(const SampleProblem& p, cudaStream_t stream);
+
 // Number of SMs of the current device (cached per device).
 int device_sm_count();
 

@@ -14,6 +14,7 @@ import torch.nn as nn
 from .functional import (
     _expert_stride_elems,
     _pack_expert_weights,
+    append_paged_kv,
     batched_fused_moe,
     fused_moe,
     fused_moe_batched,
@@ -22,6 +23,8 @@ from .functional import (
     naive_moe,
     pack_expert_shard,
     router_topk,
+    sample_tokens,
+    shared_prefix_attention,
 )
 
 __all__ = [
@@ -35,6 +38,9 @@ __all__ = [
     "router_topk",
     "pack_expert_shard",
     "_pack_expert_weights",
+    "append_paged_kv",
+    "shared_prefix_attention",
+    "sample_tokens",
 ]
 
 

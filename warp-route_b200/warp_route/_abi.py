@@ -51,7 +51,57 @@ class ExpertOffsets(ctypes.Structure):
     ]
 
 
+class PagedKv(ctypes.Structure):
+    _fields_ = [
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("page_stride", ctypes.c_int64),
+        ("head_stride", ctypes.c_int64),
+        ("slot_stride", ctypes.c_int64),
+        ("num_pages", ctypes.c_int32),
+        ("num_kv_heads", ctypes.c_int32),
+        ("page_size", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+    ]
+
+
+class Rows(ctypes.Structure):
+    _fields_ = [
+        ("ptr", ctypes.c_void_p),
+        ("token_stride", ctypes.c_int64),
+        ("head_stride", ctypes.c_int64),
+    ]
+
+
+class AttnDesc(ctypes.Structure):
+    _fields_ = [
+        ("num_tokens", ctypes.c_int32),
+        ("num_seqs", ctypes.c_int32),
+        ("num_q_heads", ctypes.c_int32),
+        ("table_width", ctypes.c_int32),
+        ("table_stride", ctypes.c_int64),
+        ("prefix_len", ctypes.c_int32),
+        ("scale", ctypes.c_float),
+    ]
+
+
+class Sampling(ctypes.Structure):
+    _fields_ = [
+        ("temperature", ctypes.c_float),
+        ("top_p", ctypes.c_float),
+        ("min_p", ctypes.c_float),
+        ("top_k", ctypes.c_int32),
+        ("temperatures", ctypes.c_void_p),
+        ("top_ps", ctypes.c_void_p),
+        ("min_ps", ctypes.c_void_p),
+        ("top_ks", ctypes.c_void_p),
+    ]
+
+
 _D = ctypes.POINTER(MoeDesc)
+_KV, _R, _A, _S = (ctypes.POINTER(c) for c in (PagedKv, Rows, AttnDesc, Sampling))
 SIGNATURES = {
     "wr_expert_offsets": (_i32, [_i32, _i32, _i32, ctypes.POINTER(ExpertOffsets)]),
     "wr_total_weight_bytes": (_i64, [_i32, _i32, _i32, _i32]),
@@ -81,6 +131,10 @@ SIGNATURES = {
                                       _vp]),
     "wr_moe_decode_layer": (_i32, [_D, _i32, _vp, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _sz,
                                    _vp, _vp]),
+    "wr_append_paged_kv": (_i32, [_KV, _i32, _R, _R, _vp, _vp, _vp, _i32, _i32, _i32, _R, _vp, _vp]),
+    "wr_shared_prefix_attention_workspace_size": (_sz, [_KV, _A, _i32]),
+    "wr_shared_prefix_attention": (_i32, [_KV, _A, _R, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "wr_sample_tokens": (_i32, [_i64, _i32, _i32, _vp, _i64, _vp, _S, _vp, _vp]),
 }
 
 _lib = None

@@ -18,7 +18,7 @@ There is no CPU fallback: without the compiled extension every call raises.
 from __future__ import annotations
 
 import functools
-from typing import List, Optional, Tuple
+from typing import List, Optional, Tuple, Union
 
 import torch
 
@@ -236,6 +236,102 @@ def router_topk(
     """Router only: (logits fp32 [T,E], ids int32 [T,K], weights fp32 [T,K])."""
     _C = _load_extension()
     return _C.router_topk(x, gate_w, num_experts, hidden_dim, top_k, router_bias)
+
+
+def append_paged_kv(
+    k: torch.Tensor,
+    v: torch.Tensor,
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    slots: torch.Tensor,
+    *,
+    positions: Optional[torch.Tensor] = None,
+    inv_freq: Optional[torch.Tensor] = None,
+    q: Optional[torch.Tensor] = None,
+    interleaved: bool = False,
+) -> Optional[torch.Tensor]:
+    """Keys and values of new tokens into a paged cache, in place.
+
+    k, v [T, num_kv_heads, head_dim] (views of a fused projection will do)
+    go to slots [T] (int64; slot s is row s % page_size of page
+    s // page_size) of k_cache, v_cache [num_pages, num_kv_heads, page_size,
+    head_dim] (any strides of multiples of 16 bytes, the same for both).  A
+    slot that is negative or outside the cache drops its token: the padding
+    of a batch.  Two tokens with one slot leave its content undefined.
+
+    With positions [T] (int64) and inv_freq [rot_dim / 2] (float32) the first
+    rot_dim columns of every key turn by the angles position * inv_freq:
+    columns (i, i + rot_dim/2), or (2i, 2i+1) if interleaved.  The queries q
+    [T, num_q_heads, head_dim] turn by the same angles (those of dropped
+    tokens too) and are returned as a new tensor; None without q."""
+    _C = _load_extension()
+    return _C.append_paged_kv(k, v, k_cache, v_cache, slots, positions, inv_freq, q, interleaved)
+
+
+def shared_prefix_attention(
+    q: torch.Tensor,
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    block_tables: torch.Tensor,
+    context_lens: torch.Tensor,
+    *,
+    prefix_pages: Optional[torch.Tensor] = None,
+    prefix_len: int = 0,
+    q_start: Optional[torch.Tensor] = None,
+    scale: Optional[float] = None,
+    return_lse: bool = False,
+):
+    """Attention of a batch over a paged cache, where all sequences share a
+    prefix, whose keys and values are read once for all of them.
+
+    Every sequence sees the prefix_len keys in the pages prefix_pages (int32)
+    and then its own context_lens[b] (int32 [B]) keys in the pages of row b
+    of block_tables (int32 [B, pages]; entries behind its keys are not read).
+    q [T, num_q_heads, head_dim], num_q_heads a multiple of the caches'
+    heads.  Without q_start sequence b asks with token b and sees all its
+    keys; with q_start (int32 [B + 1]) it asks with tokens q_start[b] to
+    q_start[b+1] - 1, its last own ones: each sees the own keys up to itself.
+    scale defaults to head_dim ** -0.5.
+
+    Returns out [T, num_q_heads, head_dim] in q's dtype, or (out, lse) with
+    the fp32 log of the sum of exponentials [T, num_q_heads].  A row that
+    sees no key (and a token of no sequence) gets 0 and -inf.  Lengths and
+    tables are read on the device: a captured graph follows them."""
+    _C = _load_extension()
+    out, lse = _C.shared_prefix_attention(q, k_cache, v_cache, block_tables, context_lens,
+                                          prefix_pages, prefix_len, q_start,
+                                          q.shape[-1] ** -0.5 if scale is None else scale,
+                                          return_lse)
+    return (out, lse) if return_lse else out
+
+
+def sample_tokens(
+    logits: torch.Tensor,
+    uniforms: torch.Tensor,
+    *,
+    temperature: Union[float, torch.Tensor] = 1.0,
+    top_k: Union[int, torch.Tensor] = 0,
+    top_p: Union[float, torch.Tensor] = 1.0,
+    min_p: Union[float, torch.Tensor] = 0.0,
+) -> torch.Tensor:
+    """A token (int64 [rows]) for each row of logits [rows, vocab] (float32 or
+    bfloat16), from the uniform numbers uniforms (float32 [rows], in [0, 1)).
+
+    w_i = exp((x_i - max) / temperature); kept are the top_k largest (equal
+    ones: lowest index first), of these the ones whose preceding sum is below
+    top_p of their sum, of these the ones with w_i >= min_p, and always the
+    largest; the token is the first whose running sum of kept w, by index,
+    exceeds uniform * sum.  Each setting is a number or a tensor with one for
+    each row (float32, top_k int32); temperature 0 takes the maximum, top_k
+    0, top_p 1 and min_p 0 are off.  The result is the same every time.  NaN
+    counts as -inf; a row with nothing above -inf gets -1."""
+    _C = _load_extension()
+
+    def split(value, off):
+        return (off, value) if isinstance(value, torch.Tensor) else (value, None)
+
+    return _C.sample_tokens(logits, uniforms, *split(temperature, 1.0), *split(top_k, 0),
+                            *split(top_p, 1.0), *split(min_p, 0.0))
 
 
 def exchange_handles(mine: bytes, group=None) -> bytes:
