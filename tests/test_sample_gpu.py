@@ -99,6 +99,21 @@ def test_ties_across_the_border_of_a_large_row():
     check((x.float() / 4).round().bfloat16(), u, top_k=777, top_p=0.8)
 
 
+def test_top_p_stays_within_what_top_k_cut():
+    """Equal values across the border of top_k: top_p must not bring back the
+    ones that top_k cut off, whichever of its ways it takes."""
+    u = torch.tensor([0.0, 0.4, 0.6, 0.9999], device="cuda")
+    for v in (300, 5000, 50000):
+        x, _ = rows(4, v, torch.bfloat16, seed=v)
+        x[:, 11::v // 7] = 12.5
+        for k in (1, 2, 5):
+            for p in (0.1, 0.5, 0.99):
+                check(x, u, top_k=k, top_p=p)
+        x[:, ::2] = 13.0  # more equal ones than are sorted
+        for k in (1, 20, v // 3):
+            check(x, u, top_k=k, top_p=0.9)
+
+
 def test_infinities_and_nan():
     inf, nan = float("inf"), float("nan")
     x, u = rows(6, 3001)

@@ -13,13 +13,14 @@
 // depend on their order, whatever order atomics come in.
 //
 // A row belongs to one cluster of 1 to 8 CTAs, which reads it once and keeps
-// it in shared memory.  The border of the first k, and that of the mass top_p,
-// are found without sorting: a histogram (count and mass) of the values over
-// 2048 bins, even over [min, max] of the row, tells which bin the border lies
-// in; the keys (order-preserving integers) of that bin are binned again until
-// one value is left, and equal values go by index.  A few passes over
-// shared memory, each followed by an exchange of 2048 sums through distributed
-// shared memory; HBM is read once.
+// it in shared memory.  The border of the first k, and that of the mass
+// top_p, are found without sorting the row: a histogram (count and mass) of
+// the values over 2048 bins, even over [min, max] of the row, tells which bin
+// a border lies in; that bin's values, few as a rule, are gathered by one CTA,
+// sorted and cut exactly.  A bin with more values than fit there (rows of many
+// equal values) is binned again by key until one value is left.  HBM is read
+// once; what bounds the kernel is the exchanges between the CTAs for few rows
+// and the 64-bit arithmetic of the weights for many.
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 
@@ -37,9 +38,12 @@ constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kBins = 2048;
 constexpr int kMaxCluster = 8;
+constexpr int kList = 2048;  // values of a bin that one CTA sorts
+constexpr int kTable = 128;  // steps of the exponential's table per factor of two
 // 16 vectors a thread hold kSampleMaxVocab values.
 constexpr int kMaxSmem = 16 * (kThreads * 16 + kWarps * 8);
 constexpr double kMassOne = 35184372088832.0;  // 2^45: with up to 2^18 values sums stay below 2^63
+constexpr double kMagic = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to a whole number
 constexpr float kNegInf = -__builtin_huge_valf();
 
 struct SampleArgs {
@@ -56,33 +60,63 @@ struct SampleArgs {
   int64_t* ids;
 };
 
-// Order-preserving key of a float that is not NaN.
+// Order-preserving key of a float that is not NaN, and back.
 WR_DEVINL uint32_t key_of(float x) {
   const uint32_t u = __float_as_uint(x);
   return u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
+}
+WR_DEVINL float value_of(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k); }
+
+// Where the kept part of the order ends: values with key > `key` are kept,
+// those equal to it up to and with index `last`.
+struct Cut {
+  uint32_t key;
+  int last;
+};
+WR_DEVINL bool in_cut(const Cut& c, uint32_t key, int idx) {
+  return key > c.key || (key == c.key && idx <= c.last);
 }
 
 struct Shared {
   uint32_t count[kBins];
   uint64_t mass[kBins];
+  uint64_t list[kList];  // (key, ~index); rank 0's alone is used
+  double table[kTable];
   uint64_t warp64[kWarps];
   uint64_t warp64b[kWarps];
   // written by every rank of the cluster into every rank's copy
-  uint64_t all_a[2][kMaxCluster], all_b[2][kMaxCluster], all_c[2][kMaxCluster];
-  uint64_t found[4];
+  uint64_t all_a[2][kMaxCluster], all_b[2][kMaxCluster];
+  uint64_t found[2][4];
+  uint32_t listed;
 };
 
 struct Row {
   float max;
-  double inv_t;
+  double maxd;
+  double steps;         // table steps per unit of x: kTable * log2(e) / temperature
+  const double* table;  // 2^(i / kTable)
 };
-// Weight and its whole number.  Below e^-60 nothing rounds to 2^-45.
+
+// w = 2^(steps (x - max) / kTable): the whole steps by the table and the
+// exponent, the rest of at most half a step (|u| <= ln 2 / 256) by the
+// exponential's series up to u^4 (the next term is below 2^-49).  Table-driven
+// reduction as in P. T. P. Tang, ACM TOMS 15 (1989).
 WR_DEVINL double weight(const Row& r, float x) {
   if (x == r.max) return 1.0;  // +inf among them
-  const double d = ((double)x - (double)r.max) * r.inv_t;
-  return d < -60.0 ? 0.0 : exp(d);
+  const double t = ((double)x - r.maxd) * r.steps;
+  if (!(t > -60.0 * kTable)) return 0.0;  // far below 2^-46, which rounds to nothing
+  const double m = t + kMagic;
+  const int k = __double2loint(m);
+  const double u = (t - (m - kMagic)) * (0.69314718055994530942 / kTable);
+  const double e = fma(fma(fma(fma(u, 1.0 / 24, 1.0 / 6), u, 0.5), u, 1.0), u, 1.0);
+  const double w = r.table[k & (kTable - 1)] * e;
+  return __hiloint2double(__double2hiint(w) + ((k >> 7) << 20), __double2loint(w));
 }
-WR_DEVINL uint64_t mass_of(double w) { return (uint64_t)__double2ll_rn(w * kMassOne); }
+static_assert(kTable == 128, "the shift above");
+// Rounded to a whole number of 2^-45 (w <= 1).
+WR_DEVINL uint64_t mass_of(double w) {
+  return (uint64_t)__double_as_longlong(fma(w, kMassOne, 4503599627370496.0)) & 0xfffffffffffffull;
+}
 
 // This CTA's part of the row in shared memory: vector l of thread t holds the
 // values 4 * ((rank * levels + l) * kThreads + t) .. + 3 of the row, -inf
@@ -105,211 +139,244 @@ struct Slice {
   }
 };
 
+struct Add { WR_DEVINL uint64_t operator()(uint64_t x, uint64_t y) const { return x + y; } };
+struct Max { WR_DEVINL uint64_t operator()(uint64_t x, uint64_t y) const { return x > y ? x : y; } };
+struct Min { WR_DEVINL uint64_t operator()(uint64_t x, uint64_t y) const { return x < y ? x : y; } };
+
 template <typename F>
 WR_DEVINL uint64_t warp_reduce(uint64_t v, F f) {
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) v = f(v, __shfl_xor_sync(0xffffffffu, v, d));
   return v;
 }
-
-// Two values of the CTA's threads reduced over the cluster (fa, fb
-// associative and commutative); every thread gets both.  `par` alternates
-// between calls, so that one call's exchange never meets the next one's.
-template <typename FA, typename FB>
-WR_DEVINL void cluster_reduce(cg::cluster_group& cl, Shared& s, int& par, uint64_t& a, uint64_t& b,
-                              FA fa, FB fb) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  a = warp_reduce(a, fa);
-  b = warp_reduce(b, fb);
-  if (lane == 0) {
-    s.warp64[warp] = a;
-    s.warp64b[warp] = b;
-  }
-  __syncthreads();
-  const int n = (int)cl.num_blocks(), me = (int)cl.block_rank();
-  if (warp == 0) {
-    a = s.warp64[lane % kWarps];
-    b = s.warp64b[lane % kWarps];
+WR_DEVINL uint64_t warp_inclusive(uint64_t v, int lane) {
 #pragma unroll
-    for (int d = 1; d < kWarps; d <<= 1) {
-      a = fa(a, __shfl_xor_sync(0xffffffffu, a, d));
-      b = fb(b, __shfl_xor_sync(0xffffffffu, b, d));
-    }
-    if (lane < n) {
-      Shared* o = cl.map_shared_rank(&s, lane);
-      o->all_a[par][me] = a;
-      o->all_b[par][me] = b;
-    }
+  for (int d = 1; d < 32; d <<= 1) {
+    const uint64_t u = __shfl_up_sync(0xffffffffu, v, d);
+    if (lane >= d) v += u;
   }
-  cl.sync();
-  a = s.all_a[par][0];
-  b = s.all_b[par][0];
-  for (int i = 1; i < n; ++i) {
-    a = fa(a, s.all_a[par][i]);
-    b = fb(b, s.all_b[par][i]);
-  }
-  par ^= 1;
+  return v;
 }
 
-struct Add { WR_DEVINL uint64_t operator()(uint64_t x, uint64_t y) const { return x + y; } };
-struct Max { WR_DEVINL uint64_t operator()(uint64_t x, uint64_t y) const { return x > y ? x : y; } };
-struct Min { WR_DEVINL uint64_t operator()(uint64_t x, uint64_t y) const { return x < y ? x : y; } };
+// The cluster and what its exchanges go through.  Each exchange writes into
+// the copy of all_* or found that `par` names and flips it: a rank can write
+// into a copy again only after a cluster barrier that every rank reaches after
+// reading it.
+struct Group {
+  cg::cluster_group cl;
+  Shared* s;
+  int n, me, par;
 
-// Where the kept part of the order ends: values with key > `key` are kept,
-// those equal to it up to and with index `last`.
-struct Cut {
-  uint32_t key;
-  int last;
+  // Two values of the CTA's threads reduced over the cluster (fa, fb
+  // associative and commutative); every thread gets both.
+  template <typename FA, typename FB>
+  WR_DEVINL void reduce(uint64_t& a, uint64_t& b, FA fa, FB fb) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    a = warp_reduce(a, fa);
+    b = warp_reduce(b, fb);
+    if (lane == 0) {
+      s->warp64[warp] = a;
+      s->warp64b[warp] = b;
+    }
+    __syncthreads();
+    if (warp == 0) {
+      a = s->warp64[lane % kWarps];
+      b = s->warp64b[lane % kWarps];
+#pragma unroll
+      for (int d = 1; d < kWarps; d <<= 1) {
+        a = fa(a, __shfl_xor_sync(0xffffffffu, a, d));
+        b = fb(b, __shfl_xor_sync(0xffffffffu, b, d));
+      }
+      if (lane < n) {
+        Shared* o = cl.map_shared_rank(s, lane);
+        o->all_a[par][me] = a;
+        o->all_b[par][me] = b;
+      }
+    }
+    cl.sync();
+    a = s->all_a[par][0];
+    b = s->all_b[par][0];
+    for (int i = 1; i < n; ++i) {
+      a = fa(a, s->all_a[par][i]);
+      b = fb(b, s->all_b[par][i]);
+    }
+    par ^= 1;
+  }
+
+  // This rank's share of the bins, kBins / n of them from first_bin(), one to
+  // four a thread, summed over the ranks; and what lies before a thread's
+  // first one in the whole order, and in all of it.
+  struct Bins {
+    uint64_t v[4], before, whole;
+  };
+  WR_DEVINL int share() const { return kBins / n; }
+  WR_DEVINL int per() const { return (share() + kThreads - 1) / kThreads; }
+  WR_DEVINL int first_bin() const { return me * share() + (int)threadIdx.x * per(); }
+
+  // After the histograms are whole (a cluster barrier).  Both sums at once.
+  WR_DEVINL void sum_bins(Bins& c, Bins& m) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    uint64_t sc = 0, sm = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      c.v[e] = m.v[e] = 0;
+      if (e < per() && (int)threadIdx.x * per() + e < share()) {
+        const int b = first_bin() + e;
+#pragma unroll
+        for (int r = 0; r < kMaxCluster; ++r)
+          if (r < n) {
+            const Shared* o = cl.map_shared_rank(s, r);
+            c.v[e] += o->count[b];
+            m.v[e] += o->mass[b];
+          }
+      }
+      sc += c.v[e];
+      sm += m.v[e];
+    }
+    const uint64_t ic = warp_inclusive(sc, lane), im = warp_inclusive(sm, lane);
+    if (lane == 31) {
+      s->warp64[warp] = ic;
+      s->warp64b[warp] = im;
+    }
+    __syncthreads();
+    c.before = ic - sc;
+    m.before = im - sm;
+    uint64_t tc = 0, tm = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < warp) {
+        c.before += s->warp64[w];
+        m.before += s->warp64b[w];
+      }
+      tc += s->warp64[w];
+      tm += s->warp64b[w];
+    }
+    if ((int)threadIdx.x < n) {
+      Shared* o = cl.map_shared_rank(s, threadIdx.x);
+      o->all_a[par][me] = tc;
+      o->all_b[par][me] = tm;
+    }
+    cl.sync();
+    c.whole = m.whole = 0;
+    for (int r = 0; r < n; ++r) {
+      if (r < me) {
+        c.before += s->all_a[par][r];
+        m.before += s->all_b[par][r];
+      }
+      c.whole += s->all_a[par][r];
+      m.whole += s->all_b[par][r];
+    }
+    par ^= 1;
+  }
+
+  // The last bin with something of x in it whose preceding sum is below
+  // target (0 < target <= x.whole); the sums of x and y before it.
+  WR_DEVINL int find_bin(const Bins& x, const Bins& y, uint64_t target, uint64_t& bx, uint64_t& by) {
+    uint64_t before = x.before, other = y.before;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (x.v[e] && before < target && before + x.v[e] >= target)
+        for (int r = 0; r < n; ++r) {
+          Shared* o = cl.map_shared_rank(s, r);
+          o->found[par][0] = (uint64_t)(first_bin() + e);
+          o->found[par][1] = before;
+          o->found[par][2] = other;
+        }
+      before += x.v[e];
+      other += y.v[e];
+    }
+    cl.sync();
+    const int bin = (int)s->found[par][0];
+    bx = s->found[par][1];
+    by = s->found[par][2];
+    par ^= 1;
+    return bin;
+  }
 };
-WR_DEVINL bool in_cut(const Cut& c, uint32_t key, int idx) {
-  return key > c.key || (key == c.key && idx <= c.last);
+
+// Sorts list[0 .. n) descending (n <= kList), all threads of the CTA.
+__device__ __noinline__ void sort_list(uint64_t* list, int n) {
+  int size = 32;
+  while (size < n) size *= 2;
+  for (int i = n + threadIdx.x; i < size; i += kThreads) list[i] = 0;
+  for (int k = 2; k <= size; k *= 2)
+    for (int j = k >> 1; j > 0; j >>= 1) {
+      __syncthreads();
+      for (int i = threadIdx.x; i < size / 2; i += kThreads) {
+        const int lo = ((i & ~(j - 1)) << 1) | (i & (j - 1)), hi = lo | j;
+        const uint64_t a = list[lo], b = list[hi];
+        if ((a < b) == ((lo & k) == 0)) {
+          list[lo] = b;
+          list[hi] = a;
+        }
+      }
+    }
+  __syncthreads();
 }
 
-// The last value of the order (within `within`) whose preceding sum is below
-// `target`: sums of 1 (kMass false) or of mass.  kMass: target is top_p times
-// the whole mass, of which the first histogram gives the whole.
+// top_p (below 1) of a mass, rounded up to a whole number and at least 1: a
+// value is kept if the mass before it is below this.
+WR_DEVINL uint64_t mass_target(float top_p, uint64_t whole) {
+  const uint64_t p = (uint64_t)((double)fmaxf(top_p, 0.f) * 18446744073709551616.0);
+  const uint64_t t = __umul64hi(p, whole) + (p * whole != 0 ? 1 : 0);
+  return t ? t : 1;
+}
+
+// A border inside keys [lo, hi] (all of them within `within`), where `above`
+// lies before them in the order: the last value whose preceding sum is below
+// target, sums of 1 (kMass false) or of mass.  For bins too full to sort:
+// binned by key until one key is left, whose values go by index.
 template <bool kMass>
-__device__ __noinline__ Cut find_cut(cg::cluster_group& cl, Shared& s, int& par, const Slice& x,
-                                     const Row& row, const Cut& within, uint32_t lo, uint32_t hi,
-                                     float low, uint64_t target, float top_p) {
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int n = (int)cl.num_blocks(), me = (int)cl.block_rank();
-  const int seg = kBins / n;  // bins whose sums this rank adds up
-  uint64_t above = 0;
-  // Even bins over the values first (monotone in x, whatever it rounds to).
-  float scale = (float)kBins / (row.max - low);
-  bool by_value = scale < 3e38f && scale > 0.f;  // false: max == low or an infinity between them
-  for (;;) {
-    if (lo == hi) break;
+__device__ __noinline__ Cut find_by_key(Group& g, const Slice& x, const Row& row, const Cut& within,
+                                        uint32_t lo, uint32_t hi, uint64_t above, uint64_t target) {
+  Shared& s = *g.s;
+  while (lo != hi) {
     int shift = 0;
     while (((hi - lo) >> shift) >= (uint32_t)kBins) ++shift;
-    auto bin_of = [&](float v, uint32_t k) {
-      if (by_value) return min(kBins - 1, (int)((row.max - v) * scale));
-      return (int)((hi - k) >> shift);
-    };
-    for (int i = tid; i < kBins; i += kThreads) {
-      if (kMass) s.mass[i] = 0; else s.count[i] = 0;
+    for (int i = threadIdx.x; i < kBins; i += kThreads) {
+      s.mass[i] = 0;
+      s.count[i] = 0;
     }
     __syncthreads();
     x.each([&](float f, int i) {
       const uint32_t k = key_of(f);
       if (k < lo || k > hi || !in_cut(within, k, i)) return;
-      if (kMass) {
-        const uint64_t m = mass_of(weight(row, f));
-        if (m) atomicAdd(reinterpret_cast<unsigned long long*>(&s.mass[bin_of(f, k)]),
-                         (unsigned long long)m);
-      } else {
-        atomicAdd(&s.count[bin_of(f, k)], 1u);
-      }
+      const uint64_t m = kMass ? mass_of(weight(row, f)) : 1;
+      if (m) atomicAdd(reinterpret_cast<unsigned long long*>(&s.mass[(hi - k) >> shift]),
+                       (unsigned long long)m);
     });
-    cl.sync();
-    // This rank's bins, summed over the ranks: thread t has bins t * per ...
-    // of the segment (seg >= 256, kThreads 512: one to four bins a thread).
-    const int per = (seg + kThreads - 1) / kThreads;
-    uint64_t v[4], mine = 0;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      v[e] = 0;
-      const int i = tid * per + e;
-      if (e < per && i < seg)
-        for (int r = 0; r < n; ++r) {
-          const Shared* o = cl.map_shared_rank(&s, r);
-          v[e] += kMass ? o->mass[me * seg + i] : (uint64_t)o->count[me * seg + i];
-        }
-      mine += v[e];
-    }
-    uint64_t incl = mine;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const uint64_t u = __shfl_up_sync(0xffffffffu, incl, d);
-      if (lane >= d) incl += u;
-    }
-    if (lane == 31) s.warp64[warp] = incl;
-    __syncthreads();
-    uint64_t before = incl - mine, total = 0;
-    for (int w = 0; w < kWarps; ++w) {
-      if (w < warp) before += s.warp64[w];
-      total += s.warp64[w];
-    }
-    if (tid < n) cl.map_shared_rank(&s, tid)->all_a[par][me] = total;
-    cl.sync();
-    uint64_t whole = 0, start = above;
-    for (int r = 0; r < n; ++r) {
-      whole += s.all_a[par][r];
-      if (r < me) start += s.all_a[par][r];
-    }
-    par ^= 1;
-    if (kMass && target == 0) {  // the first histogram: top_p of the whole, rounded up
-      const uint64_t p = (uint64_t)((double)top_p * 18446744073709551616.0);
-      target = __umul64hi(p, whole) + (p * whole != 0 ? 1 : 0);
-      if (target == 0) target = 1;  // top_p 0: the first alone
-    }
-    // The last bin with something in it whose preceding sum is below target.
-    before += start;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      if (e < per && v[e] && before < target && before + v[e] >= target) {
-        const int bin = me * seg + tid * per + e;
-        for (int r = 0; r < n; ++r) {
-          Shared* o = cl.map_shared_rank(&s, r);
-          o->found[0] = (uint64_t)bin;
-          o->found[1] = before;
-        }
-      }
-      before += v[e];
-    }
-    cl.sync();
-    const int bin = (int)s.found[0];
-    above = s.found[1];
-    // The keys of that bin.
+    g.cl.sync();
+    Group::Bins c, m;
+    g.sum_bins(c, m);
+    uint64_t before, none;
+    const int bin = g.find_bin(m, c, target - above, before, none);
+    above += before;
     uint64_t a = 0xffffffffull, b = 0;
     x.each([&](float f, int i) {
       const uint32_t k = key_of(f);
-      if (k < lo || k > hi || !in_cut(within, k, i) || bin_of(f, k) != bin) return;
-      if (kMass && mass_of(weight(row, f)) == 0) return;
+      if (k < lo || k > hi || (int)((hi - k) >> shift) != bin || !in_cut(within, k, i)) return;
       a = min(a, (uint64_t)k);
       b = max(b, (uint64_t)k);
     });
-    cluster_reduce(cl, s, par, a, b, Min(), Max());
+    g.reduce(a, b, Min(), Max());
     lo = (uint32_t)a;
     hi = (uint32_t)b;
-    by_value = false;
   }
-  // Equal values: the first r by index.  Each counts one, or its mass.
+  // Equal values: the first r by index.
   Cut c;
   c.key = lo;
-  uint64_t each = 1;
-  if (kMass) {
-    const uint32_t u = lo & 0x80000000u ? lo ^ 0x80000000u : ~lo;
-    each = mass_of(weight(row, __uint_as_float(u)));
-  }
-  if (kMass && target == 0) {  // all values equal: no histogram was made
-    uint64_t cnt = 0, none = 0;
-    x.each([&](float f, int i) { cnt += key_of(f) == lo && in_cut(within, lo, i); });
-    cluster_reduce(cl, s, par, cnt, none, Add(), Add());
-    const uint64_t whole = cnt * each, p = (uint64_t)((double)top_p * 18446744073709551616.0);
-    target = __umul64hi(p, whole) + (p * whole != 0 ? 1 : 0);
-    if (target == 0) target = 1;
-  }
+  const uint64_t each = kMass ? mass_of(weight(row, value_of(lo))) : 1;
   const uint64_t r = each ? (target - above + each - 1) / each : 1;
-  uint64_t cnt = 0, none = 0;
-  x.each([&](float f, int i) { cnt += key_of(f) == lo && in_cut(within, lo, i); });
-  cluster_reduce(cl, s, par, cnt, none, Add(), Add());
-  if (r >= cnt) {
-    c.last = 0x7fffffff;
-    return c;
-  }
-  // Bisection over the index: rare (ties across the border), at most 18 steps.
-  int a = 0, b = 1 << 18;  // ties with index < a: fewer than r; with index < b: at least r
+  const int most = lo == within.key ? within.last : 0x7fffffff;
+  int a = 0, b = 1 << 18;  // fewer than r of them have an index below a; r or more below b, or b is the end
   while (b - a > 1) {
     const int mid = (a + b) >> 1;
-    uint64_t q = 0;
-    none = 0;
-    x.each([&](float f, int i) { q += key_of(f) == lo && i < mid && in_cut(within, lo, i); });
-    cluster_reduce(cl, s, par, q, none, Add(), Add());
+    uint64_t q = 0, none = 0;
+    x.each([&](float f, int i) { q += key_of(f) == lo && i < mid && i <= most; });
+    g.reduce(q, none, Add(), Add());
     if (q >= r) b = mid; else a = mid;
   }
-  c.last = b - 1;
+  c.last = min(b - 1, most);
   return c;
 }
 
@@ -317,13 +384,14 @@ template <typename T>
 __global__ void __launch_bounds__(kThreads) k_sample(const SampleArgs a) {
   extern __shared__ __align__(16) float4 s_values[];
   __shared__ Shared s;
-  cg::cluster_group cl = cg::this_cluster();
-  auto started = cl.barrier_arrive();  // a rank's memory is there once it runs
-  const int n = (int)cl.num_blocks(), me = (int)cl.block_rank();
-  const int64_t r = blockIdx.x / n;
+  Group g{cg::this_cluster(), &s, 0, 0, 0};
+  auto started = g.cl.barrier_arrive();  // a rank's memory is there once it runs
+  g.n = (int)g.cl.num_blocks();
+  g.me = (int)g.cl.block_rank();
+  const int64_t r = blockIdx.x / g.n;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const T* p = static_cast<const T*>(a.logits) + r * a.row_stride;
-  const Slice x{s_values, a.levels, me};
+  const Slice x{s_values, a.levels, g.me};
   uint64_t* s_level = reinterpret_cast<uint64_t*>(s_values + a.levels * kThreads);  // [levels][kWarps]
   // Maximum with its lowest index, and the lowest value above -inf.
   uint64_t best = 0, low = ~0ull;
@@ -356,46 +424,182 @@ __global__ void __launch_bounds__(kThreads) k_sample(const SampleArgs a) {
     }
     s_values[l * kThreads + tid] = make_float4(f[0], f[1], f[2], f[3]);
   }
-
+  if (tid < kTable) s.table[tid] = exp2((double)tid / kTable);
+  if (tid == 0) s.listed = 0;
+  for (int i = tid; i < kBins; i += kThreads) {
+    s.mass[i] = 0;
+    s.count[i] = 0;
+  }
   const float temp = a.temperature ? a.temperature[r] : a.temperature1;
   const float top_p = a.top_p ? a.top_p[r] : a.top_p1;
   const float min_p = a.min_p ? a.min_p[r] : a.min_p1;
   const int top_k = a.top_k ? a.top_k[r] : a.top_k1;
 
-  int par = 0;
-  cl.barrier_wait(std::move(started));
-  cluster_reduce(cl, s, par, best, low, Max(), Min());
-  const uint32_t kmax = (uint32_t)(best >> 32);
+  g.cl.barrier_wait(std::move(started));
+  g.reduce(best, low, Max(), Min());
+  const uint32_t kmax = (uint32_t)(best >> 32), klow = (uint32_t)low;
   const int imax = (int)(0x7fffffffu - (uint32_t)best);
   if (low == ~0ull || !(temp > 0.f)) {  // nothing to sample, or the maximum itself
-    if (me == 0 && tid == 0) a.ids[r] = low == ~0ull ? -1 : imax;
+    if (g.me == 0 && tid == 0) a.ids[r] = low == ~0ull ? -1 : imax;
     return;
   }
   Row row;
-  row.max = __uint_as_float(kmax & 0x80000000u ? kmax ^ 0x80000000u : ~kmax);
-  row.inv_t = 1.0 / (double)temp;
-  const uint32_t klow = (uint32_t)low;
-  const float lowest = __uint_as_float(klow & 0x80000000u ? klow ^ 0x80000000u : ~klow);
+  row.max = value_of(kmax);
+  row.maxd = (double)row.max;
+  row.steps = kTable * 1.4426950408889634074 / (double)temp;
+  row.table = s.table;
 
   Cut cut{0u, 0x7fffffff};  // everything
-  if (top_k >= 1 && top_k < a.vocab) {
-    // fewer finite values than top_k: nothing is cut
-    uint64_t cnt = 0, none = 0;
-    x.each([&](float f, int) { cnt += f > kNegInf; });
-    cluster_reduce(cl, s, par, cnt, none, Add(), Add());
-    if ((uint64_t)top_k < cnt)
-      cut = find_cut<false>(cl, s, par, x, row, cut, klow, kmax, lowest, (uint64_t)top_k, 0.f);
-  }
-  if (top_p < 1.f) {
-    const uint32_t from = max(cut.key, klow);
-    const float fl = __uint_as_float(from & 0x80000000u ? from ^ 0x80000000u : ~from);
-    cut = find_cut<true>(cl, s, par, x, row, cut, from, kmax, fl, 0, fmaxf(top_p, 0.f));
+  bool by_k = top_k >= 1 && top_k < a.vocab;
+  const bool by_p = top_p < 1.f;
+  if (by_k || by_p) {
+    // Even bins over the values (monotone in x, whatever it rounds to).
+    const float scale = (float)kBins / (row.max - value_of(klow));
+    const bool even = scale > 0.f && scale < 3e38f;  // not: one value, or an infinite span
+    auto bin_of = [&](float f) { return min(kBins - 1, (int)((row.max - f) * scale)); };
+    Group::Bins cnt, mass;
+    if (even) {
+      x.each([&](float f, int) {
+        if (!(f > kNegInf)) return;
+        const int b = bin_of(f);
+        if (by_k) atomicAdd(&s.count[b], 1u);
+        if (by_p) {
+          const uint64_t m = mass_of(weight(row, f));
+          if (m) atomicAdd(reinterpret_cast<unsigned long long*>(&s.mass[b]), (unsigned long long)m);
+        }
+      });
+    } else {
+      uint64_t c = 0, m = 0;
+      x.each([&](float f, int) {
+        if (!(f > kNegInf)) return;
+        ++c;
+        m += mass_of(weight(row, f));
+      });
+      g.reduce(c, m, Add(), Add());
+      cnt.whole = c;
+      mass.whole = m;
+    }
+    if (even) {
+      g.cl.sync();
+      g.sum_bins(cnt, mass);
+    }
+    if (by_k && (uint64_t)top_k >= cnt.whole) by_k = false;  // fewer values than that
+    int listed_bin = -1, listed = 0;
+    uint64_t whole = mass.whole;
+    // The values of a bin, sorted, in rank 0's list; how many (on all ranks).
+    auto gather = [&](int bin) {
+      x.each([&](float f, int i) {
+        if (!(f > kNegInf) || bin_of(f) != bin) return;
+        Shared* o = g.cl.map_shared_rank(&s, 0);
+        const uint32_t at = atomicAdd(&o->listed, 1u);
+        if (at < (uint32_t)kList) o->list[at] = ((uint64_t)key_of(f) << 32) | (uint32_t)~i;
+      });
+      g.cl.sync();
+      listed = (int)g.cl.map_shared_rank(&s, 0)->listed;
+      listed_bin = bin;
+      if (g.me == 0 && listed <= kList) sort_list(s.list, listed);
+    };
+    // Keys of a bin, for find_by_key.
+    auto keys = [&](int bin, uint32_t& lo, uint32_t& hi) {
+      uint64_t l = 0xffffffffull, h = 0;
+      x.each([&](float f, int) {
+        if (!(f > kNegInf) || bin_of(f) != bin) return;
+        l = min(l, (uint64_t)key_of(f));
+        h = max(h, (uint64_t)key_of(f));
+      });
+      g.reduce(l, h, Min(), Max());
+      lo = (uint32_t)l;
+      hi = (uint32_t)h;
+    };
+    if (by_k && even) {
+      uint64_t above = 0, above_mass = 0;
+      const int bin = g.find_bin(cnt, mass, (uint64_t)top_k, above, above_mass);
+      gather(bin);
+      if (listed <= kList) {
+        const int need = top_k - (int)above;  // of the bin
+        if (g.me == 0) {
+          uint64_t m = 0;
+          if (by_p)
+            for (int i = tid; i < need; i += kThreads) m += mass_of(weight(row, value_of((uint32_t)(s.list[i] >> 32))));
+          m = warp_reduce(m, Add());
+          if (lane == 0) s.warp64[warp] = m;
+          __syncthreads();
+          if (tid < g.n) {
+            m = above_mass;
+            for (int w = 0; w < kWarps; ++w) m += s.warp64[w];
+            Shared* o = g.cl.map_shared_rank(&s, tid);
+            o->found[g.par][0] = s.list[need - 1];
+            o->found[g.par][1] = m;
+          }
+        }
+        g.cl.sync();
+        cut.key = (uint32_t)(s.found[g.par][0] >> 32);
+        cut.last = (int)~(uint32_t)s.found[g.par][0];
+        whole = s.found[g.par][1];
+        g.par ^= 1;
+      } else {
+        uint32_t lo, hi;
+        keys(bin, lo, hi);
+        cut = find_by_key<false>(g, x, row, cut, lo, hi, above, (uint64_t)top_k);
+      }
+    } else if (by_k) {
+      cut = find_by_key<false>(g, x, row, cut, klow, kmax, 0, (uint64_t)top_k);
+    }
+    if (by_p && (listed > kList || !even)) {  // the bins are gone: by key, among the first k
+      uint64_t m = 0, none = 0;
+      x.each([&](float f, int i) {
+        if (f > kNegInf && in_cut(cut, key_of(f), i)) m += mass_of(weight(row, f));
+      });
+      g.reduce(m, none, Add(), Add());
+      cut = find_by_key<true>(g, x, row, cut, max(cut.key, klow), kmax, 0, mass_target(top_p, m));
+    } else if (by_p) {
+      const uint64_t target = mass_target(top_p, whole);
+      uint64_t above = 0, none = 0;
+      const int bin = g.find_bin(mass, cnt, target, above, none);
+      if (bin != listed_bin) {
+        if (g.me == 0 && tid == 0) s.listed = 0;
+        g.cl.sync();
+        gather(bin);
+      }
+      if (listed <= kList) {
+        // The last of the list whose preceding mass is below target; with a
+        // top_k in this bin target ends within the first k of it.
+        if (g.me == 0) {
+          const int per = (listed + kThreads - 1) / kThreads;
+          uint64_t sum = 0;
+          for (int e = 0; e < per; ++e) {
+            const int i = tid * per + e;
+            if (i < listed) sum += mass_of(weight(row, value_of((uint32_t)(s.list[i] >> 32))));
+          }
+          const uint64_t incl = warp_inclusive(sum, lane);
+          if (lane == 31) s.warp64[warp] = incl;
+          __syncthreads();
+          uint64_t before = above + incl - sum;
+          for (int w = 0; w < warp; ++w) before += s.warp64[w];
+          for (int e = 0; e < per; ++e) {
+            const int i = tid * per + e;
+            if (i >= listed) break;
+            const uint64_t m = mass_of(weight(row, value_of((uint32_t)(s.list[i] >> 32))));
+            if (m && before < target && before + m >= target)
+              for (int o = 0; o < g.n; ++o) g.cl.map_shared_rank(&s, o)->found[g.par][0] = s.list[i];
+            before += m;
+          }
+        }
+        g.cl.sync();
+        cut.key = (uint32_t)(s.found[g.par][0] >> 32);
+        cut.last = (int)~(uint32_t)s.found[g.par][0];
+        g.par ^= 1;
+      } else {
+        uint32_t lo, hi;
+        keys(bin, lo, hi);
+        cut = find_by_key<true>(g, x, row, cut, max(lo, cut.key), hi, above, target);
+      }
+    }
   }
 
   // Running sums by index: (rank, level, warp, lane, element).
-  const Cut keep = cut;
   auto kept_mass = [&](float f, int i) -> uint64_t {
-    if (!(f > kNegInf) || !in_cut(keep, key_of(f), i)) return 0;
+    if (!(f > kNegInf) || !in_cut(cut, key_of(f), i)) return 0;
     const double w = weight(row, f);
     return w >= (double)min_p || i == imax ? mass_of(w) : 0;
   };
@@ -405,53 +609,51 @@ __global__ void __launch_bounds__(kThreads) k_sample(const SampleArgs a) {
     return kept_mass(q.x, i) + kept_mass(q.y, i + 1) + kept_mass(q.z, i + 2) + kept_mass(q.w, i + 3);
   };
   uint64_t sum = 0;
+  __syncthreads();  // s.warp64 is free, s.table there
 #pragma unroll 1
   for (int l = 0; l < a.levels; ++l) {
-    const uint64_t m = level_mass(l), t = warp_reduce(m, Add());
+    const uint64_t m = level_mass(l);
+    const uint64_t t = __any_sync(0xffffffffu, m != 0) ? warp_reduce(m, Add()) : 0;
     if (lane == 0) s_level[l * kWarps + warp] = t;
-    sum += m;
+    sum += t;
   }
-  // every rank's sum, by rank
-  {
-    uint64_t t = warp_reduce(sum, Add());
-    if (lane == 0) s.warp64[warp] = t;
-    __syncthreads();
-    if (tid < n) {
-      t = 0;
-      for (int w = 0; w < kWarps; ++w) t += s.warp64[w];
-      cl.map_shared_rank(&s, tid)->all_c[0][me] = t;
-    }
-    cl.sync();
+  if (lane == 0) s.warp64[warp] = sum;
+  __syncthreads();
+  if (tid < g.n) {
+    uint64_t t = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) t += s.warp64[w];
+    g.cl.map_shared_rank(&s, tid)->all_a[g.par][g.me] = t;
   }
+  g.cl.sync();
   uint64_t whole = 0, start = 0;
-  for (int i = 0; i < n; ++i) {
-    if (i < me) start += s.all_c[0][i];
-    whole += s.all_c[0][i];
+  for (int i = 0; i < g.n; ++i) {
+    if (i < g.me) start += s.all_a[g.par][i];
+    whole += s.all_a[g.par][i];
   }
-  const uint64_t here = s.all_c[0][me];
+  const uint64_t here = s.all_a[g.par][g.me];
   const double u = fmin(fmax((double)a.uniforms[r], 0.0), 1.0 - 1.0 / 16777216.0);
   const uint64_t goal = __umul64hi((uint64_t)(u * 18446744073709551616.0), whole);  // < whole
   if (goal < start || goal >= start + here) return;
   uint64_t at = start;
-  int l = 0, w0 = 0;
-  for (int i = 0; i < a.levels * kWarps; ++i) {  // the (level, warp) that passes the goal
-    const uint64_t t = s_level[i];
-    if (goal < at + t) {
-      l = i / kWarps;
-      w0 = i % kWarps;
+  int l = 0;
+  bool mine = false;
+  for (; l < a.levels; ++l) {  // the level that passes the goal, then the warp
+    uint64_t t = s_level[l * kWarps + (lane % kWarps)];
+    uint64_t incl = warp_inclusive(lane < kWarps ? t : 0, lane);
+    const uint64_t all = __shfl_sync(0xffffffffu, incl, kWarps - 1);
+    if (goal < at + all) {
+      const uint64_t before = at + __shfl_sync(0xffffffffu, incl - t, warp);
+      const uint64_t own = __shfl_sync(0xffffffffu, t, warp);
+      mine = goal >= before && goal < before + own;
+      at = before;
       break;
     }
-    at += t;
+    at += all;
   }
-  if (warp != w0) return;
+  if (!mine) return;
   const uint64_t m = level_mass(l);
-  uint64_t incl = m;
-#pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const uint64_t v = __shfl_up_sync(0xffffffffu, incl, d);
-    if (lane >= d) incl += v;
-  }
-  at += incl - m;
+  at += warp_inclusive(m, lane) - m;
   if (goal < at || goal >= at + m) return;
   const float4 q = s_values[l * kThreads + tid];
   const float f[4] = {q.x, q.y, q.z, q.w};
