@@ -38,10 +38,10 @@ constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kBins = 2048;
 constexpr int kMaxCluster = 8;
-constexpr int kList = 2048;  // values of a bin that one CTA sorts
+constexpr int kList = 1024;  // values that one CTA sorts
 constexpr int kTable = 128;  // steps of the exponential's table per factor of two
 // 16 vectors a thread hold kSampleMaxVocab values.
-constexpr int kMaxSmem = 16 * (kThreads * 16 + kWarps * 8);
+constexpr int kMaxLevels = 16;
 constexpr double kMassOne = 35184372088832.0;  // 2^45: with up to 2^18 values sums stay below 2^63
 constexpr double kMagic = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to a whole number
 constexpr float kNegInf = -__builtin_huge_valf();
@@ -79,7 +79,10 @@ WR_DEVINL bool in_cut(const Cut& c, uint32_t key, int idx) {
 
 struct Shared {
   uint32_t count[kBins];
-  uint64_t mass[kBins];
+  // Masses in three parts of 17, 17 and 12 bits, each added with a native
+  // 32-bit atomic (a 64-bit one is a loop of compare and swap): a CTA has at
+  // most 2^15 values, so no part passes 32 bits.
+  uint32_t mass[3][kBins];
   uint64_t list[kList];  // (key, ~index); rank 0's alone is used
   double table[kTable];
   uint64_t warp64[kWarps];
@@ -89,6 +92,18 @@ struct Shared {
   uint64_t found[2][4];
   uint32_t listed;
 };
+
+WR_DEVINL void add_mass(Shared& s, int bin, uint64_t m) {
+  const uint32_t a = (uint32_t)m & 0x1ffffu, b = (uint32_t)(m >> 17) & 0x1ffffu, c = (uint32_t)(m >> 34);
+  if (a) atomicAdd(&s.mass[0][bin], a);
+  if (b) atomicAdd(&s.mass[1][bin], b);
+  if (c) atomicAdd(&s.mass[2][bin], c);
+}
+WR_DEVINL void clear_bins(Shared& s) {
+  for (int i = threadIdx.x; i < kBins; i += kThreads)
+    s.count[i] = s.mass[0][i] = s.mass[1][i] = s.mass[2][i] = 0;
+}
+static_assert(kMaxLevels * kThreads * 4 <= 1 << 15, "parts of the masses");
 
 struct Row {
   float max;
@@ -121,20 +136,31 @@ WR_DEVINL uint64_t mass_of(double w) {
 // This CTA's part of the row in shared memory: vector l of thread t holds the
 // values 4 * ((rank * levels + l) * kThreads + t) .. + 3 of the row, -inf
 // behind its end.  A thread touches its own vectors only.
+// V: four values as they came, float4 or uint2 (bf16), NaN and -0 replaced.
+WR_DEVINL void widen4(const float4& v, float (&f)[4]) { f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w; }
+WR_DEVINL void widen4(const uint2& v, float (&f)[4]) {
+  f[0] = bf16lo(v.x); f[1] = bf16hi(v.x);
+  f[2] = bf16lo(v.y); f[3] = bf16hi(v.y);
+}
+WR_DEVINL void pack4(const float (&f)[4], float4& v) { v = make_float4(f[0], f[1], f[2], f[3]); }
+WR_DEVINL void pack4(const float (&f)[4], uint2& v) {  // exact: they came from bf16
+  v.x = (__float_as_uint(f[0]) >> 16) | (__float_as_uint(f[1]) & 0xffff0000u);
+  v.y = (__float_as_uint(f[2]) >> 16) | (__float_as_uint(f[3]) & 0xffff0000u);
+}
+template <typename V>
 struct Slice {
-  float4* v;
+  V* v;
   int levels, rank;
   WR_DEVINL int index(int l) const { return ((rank * levels + l) * kThreads + (int)threadIdx.x) * 4; }
   template <typename F>
   WR_DEVINL void each(F f) const {
 #pragma unroll 1
     for (int l = 0; l < levels; ++l) {
-      const float4 q = v[l * kThreads + threadIdx.x];
+      float q[4];
+      widen4(v[l * kThreads + threadIdx.x], q);
       const int i = index(l);
-      f(q.x, i);
-      f(q.y, i + 1);
-      f(q.z, i + 2);
-      f(q.w, i + 3);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) f(q[e], i + e);
     }
   }
 };
@@ -227,7 +253,7 @@ struct Group {
           if (r < n) {
             const Shared* o = cl.map_shared_rank(s, r);
             c.v[e] += o->count[b];
-            m.v[e] += o->mass[b];
+            m.v[e] += o->mass[0][b] + ((uint64_t)o->mass[1][b] << 17) + ((uint64_t)o->mass[2][b] << 34);
           }
       }
       sc += c.v[e];
@@ -270,8 +296,10 @@ struct Group {
   }
 
   // The last bin with something of x in it whose preceding sum is below
-  // target (0 < target <= x.whole); the sums of x and y before it.
-  WR_DEVINL int find_bin(const Bins& x, const Bins& y, uint64_t target, uint64_t& bx, uint64_t& by) {
+  // target (0 < target <= x.whole); the sums of x and y before it, and that of
+  // x up to its end.
+  WR_DEVINL int find_bin(const Bins& x, const Bins& y, uint64_t target, uint64_t& bx, uint64_t& by,
+                         uint64_t& ex) {
     uint64_t before = x.before, other = y.before;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -281,6 +309,7 @@ struct Group {
           o->found[par][0] = (uint64_t)(first_bin() + e);
           o->found[par][1] = before;
           o->found[par][2] = other;
+          o->found[par][3] = before + x.v[e];
         }
       before += x.v[e];
       other += y.v[e];
@@ -289,6 +318,7 @@ struct Group {
     const int bin = (int)s->found[par][0];
     bx = s->found[par][1];
     by = s->found[par][2];
+    ex = s->found[par][3];
     par ^= 1;
     return bin;
   }
@@ -322,34 +352,101 @@ WR_DEVINL uint64_t mass_target(float top_p, uint64_t whole) {
   return t ? t : 1;
 }
 
+// uniform * whole, rounded down (so below whole): the token's running sum
+// exceeds it.
+WR_DEVINL uint64_t goal_of(float uniform, uint64_t whole) {
+  const double u = fmin(fmax((double)uniform, 0.0), 1.0 - 1.0 / 16777216.0);
+  return __umul64hi((uint64_t)(u * 18446744073709551616.0), whole);
+}
+
+// Exclusive running sum over the CTA's threads, and the whole.
+WR_DEVINL uint64_t cta_before(Shared& s, uint64_t v, uint64_t& whole) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const uint64_t incl = warp_inclusive(v, lane);
+  __syncthreads();
+  if (lane == 31) s.warp64[warp] = incl;
+  __syncthreads();
+  uint64_t before = incl - v;
+  whole = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    if (w < warp) before += s.warp64[w];
+    whole += s.warp64[w];
+  }
+  return before;
+}
+
+// The rest of a row whose first top_k all lie in the list (n >= top_k values
+// of it, unsorted): one CTA, two list entries a thread.
+__device__ __noinline__ void finish_list(Shared& s, const Row& row, int n, int top_k, float top_p,
+                                         float min_p, float uniform, int64_t* id) {
+  constexpr int kPer = kList / kThreads;
+  sort_list(s.list, n);
+  uint64_t entry[kPer], m[kPer], sum = 0, whole;
+  bool keep[kPer];
+#pragma unroll
+  for (int e = 0; e < kPer; ++e) {
+    const int i = threadIdx.x * kPer + e;
+    keep[e] = i < top_k && i < n;
+    entry[e] = keep[e] ? s.list[i] : 0;
+    const double w = keep[e] ? weight(row, value_of((uint32_t)(entry[e] >> 32))) : 0.0;
+    m[e] = mass_of(w);
+    sum += m[e];
+    keep[e] = keep[e] && (w >= (double)min_p || i == 0);
+  }
+  uint64_t before = cta_before(s, sum, whole);
+  if (top_p < 1.f) {
+    const uint64_t target = mass_target(top_p, whole);
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) {
+      keep[e] = keep[e] && before < target;
+      before += m[e];
+    }
+  }
+  // By index: the list again, its entries (~index, key), the dropped ones 0.
+#pragma unroll
+  for (int e = 0; e < kPer; ++e) s.list[threadIdx.x * kPer + e] = keep[e] ? (entry[e] << 32) | (entry[e] >> 32) : 0;
+  __syncthreads();
+  sort_list(s.list, n);
+  sum = 0;
+#pragma unroll
+  for (int e = 0; e < kPer; ++e) {
+    entry[e] = s.list[threadIdx.x * kPer + e];
+    m[e] = entry[e] ? mass_of(weight(row, value_of((uint32_t)entry[e]))) : 0;
+    sum += m[e];
+  }
+  before = cta_before(s, sum, whole);
+  const uint64_t goal = goal_of(uniform, whole);
+#pragma unroll
+  for (int e = 0; e < kPer; ++e) {
+    if (goal >= before && goal < before + m[e]) *id = (int64_t)(uint32_t)~(uint32_t)(entry[e] >> 32);
+    before += m[e];
+  }
+}
+
 // A border inside keys [lo, hi] (all of them within `within`), where `above`
 // lies before them in the order: the last value whose preceding sum is below
 // target, sums of 1 (kMass false) or of mass.  For bins too full to sort:
 // binned by key until one key is left, whose values go by index.
-template <bool kMass>
-__device__ __noinline__ Cut find_by_key(Group& g, const Slice& x, const Row& row, const Cut& within,
+template <bool kMass, typename V>
+__device__ __noinline__ Cut find_by_key(Group& g, const Slice<V>& x, const Row& row, const Cut& within,
                                         uint32_t lo, uint32_t hi, uint64_t above, uint64_t target) {
   Shared& s = *g.s;
   while (lo != hi) {
     int shift = 0;
     while (((hi - lo) >> shift) >= (uint32_t)kBins) ++shift;
-    for (int i = threadIdx.x; i < kBins; i += kThreads) {
-      s.mass[i] = 0;
-      s.count[i] = 0;
-    }
+    clear_bins(s);
     __syncthreads();
     x.each([&](float f, int i) {
       const uint32_t k = key_of(f);
       if (k < lo || k > hi || !in_cut(within, k, i)) return;
-      const uint64_t m = kMass ? mass_of(weight(row, f)) : 1;
-      if (m) atomicAdd(reinterpret_cast<unsigned long long*>(&s.mass[(hi - k) >> shift]),
-                       (unsigned long long)m);
+      add_mass(s, (int)((hi - k) >> shift), kMass ? mass_of(weight(row, f)) : 1);
     });
     g.cl.sync();
     Group::Bins c, m;
     g.sum_bins(c, m);
-    uint64_t before, none;
-    const int bin = g.find_bin(m, c, target - above, before, none);
+    uint64_t before, none, end;
+    const int bin = g.find_bin(m, c, target - above, before, none, end);
     above += before;
     uint64_t a = 0xffffffffull, b = 0;
     x.each([&](float f, int i) {
@@ -381,8 +478,17 @@ __device__ __noinline__ Cut find_by_key(Group& g, const Slice& x, const Row& row
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) k_sample(const SampleArgs a) {
-  extern __shared__ __align__(16) float4 s_values[];
+struct Four;
+template <>
+struct Four<float> { using V = float4; };
+template <>
+struct Four<uint16_t> { using V = uint2; };
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 2) k_sample(const SampleArgs a) {
+  using V = typename Four<T>::V;
+  extern __shared__ __align__(16) uint8_t s_dynamic[];
+  V* s_values = reinterpret_cast<V*>(s_dynamic);
   __shared__ Shared s;
   Group g{cg::this_cluster(), &s, 0, 0, 0};
   auto started = g.cl.barrier_arrive();  // a rank's memory is there once it runs
@@ -391,10 +497,11 @@ __global__ void __launch_bounds__(kThreads) k_sample(const SampleArgs a) {
   const int64_t r = blockIdx.x / g.n;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const T* p = static_cast<const T*>(a.logits) + r * a.row_stride;
-  const Slice x{s_values, a.levels, g.me};
+  const Slice<V> x{s_values, a.levels, g.me};
   uint64_t* s_level = reinterpret_cast<uint64_t*>(s_values + a.levels * kThreads);  // [levels][kWarps]
   // Maximum with its lowest index, and the lowest value above -inf.
-  uint64_t best = 0, low = ~0ull;
+  float top = kNegInf, least = __builtin_huge_valf();
+  int at_top = 0x7fffffff;
 #pragma unroll 4
   for (int l = 0; l < a.levels; ++l) {
     const int j = x.index(l);
@@ -418,18 +525,19 @@ __global__ void __launch_bounds__(kThreads) k_sample(const SampleArgs a) {
     for (int e = 0; e < 4; ++e) {
       // NaN counts as -inf; -0 as 0 (equal numbers have equal keys).
       f[e] = f[e] != f[e] ? kNegInf : f[e] + 0.f;
-      const uint32_t k = key_of(f[e]);
-      best = max(best, ((uint64_t)k << 32) | (0x7fffffffu - (uint32_t)(j + e)));
-      if (f[e] > kNegInf) low = min(low, (uint64_t)k);
+      if (f[e] > top) {
+        top = f[e];
+        at_top = j + e;
+      }
+      if (f[e] > kNegInf) least = fminf(least, f[e]);
     }
-    s_values[l * kThreads + tid] = make_float4(f[0], f[1], f[2], f[3]);
+    pack4(f, s_values[l * kThreads + tid]);
   }
+  uint64_t best = ((uint64_t)key_of(top) << 32) | (0x7fffffffu - (uint32_t)at_top);
+  uint64_t low = top > kNegInf ? (uint64_t)key_of(least) : ~0ull;
   if (tid < kTable) s.table[tid] = exp2((double)tid / kTable);
   if (tid == 0) s.listed = 0;
-  for (int i = tid; i < kBins; i += kThreads) {
-    s.mass[i] = 0;
-    s.count[i] = 0;
-  }
+  clear_bins(s);
   const float temp = a.temperature ? a.temperature[r] : a.temperature1;
   const float top_p = a.top_p ? a.top_p[r] : a.top_p1;
   const float min_p = a.min_p ? a.min_p[r] : a.min_p1;
@@ -457,16 +565,16 @@ __global__ void __launch_bounds__(kThreads) k_sample(const SampleArgs a) {
     const float scale = (float)kBins / (row.max - value_of(klow));
     const bool even = scale > 0.f && scale < 3e38f;  // not: one value, or an infinite span
     auto bin_of = [&](float f) { return min(kBins - 1, (int)((row.max - f) * scale)); };
+    // The first top_k as a rule fit one CTA's list, which then needs no masses
+    // of the others.
+    const bool small_k = by_k && top_k <= kList / 2;
     Group::Bins cnt, mass;
     if (even) {
       x.each([&](float f, int) {
         if (!(f > kNegInf)) return;
         const int b = bin_of(f);
         if (by_k) atomicAdd(&s.count[b], 1u);
-        if (by_p) {
-          const uint64_t m = mass_of(weight(row, f));
-          if (m) atomicAdd(reinterpret_cast<unsigned long long*>(&s.mass[b]), (unsigned long long)m);
-        }
+        if (by_p && !small_k) add_mass(s, b, mass_of(weight(row, f)));
       });
     } else {
       uint64_t c = 0, m = 0;
@@ -512,8 +620,29 @@ __global__ void __launch_bounds__(kThreads) k_sample(const SampleArgs a) {
       hi = (uint32_t)h;
     };
     if (by_k && even) {
-      uint64_t above = 0, above_mass = 0;
-      const int bin = g.find_bin(cnt, mass, (uint64_t)top_k, above, above_mass);
+      uint64_t above = 0, above_mass = 0, end = 0;
+      const int bin = g.find_bin(cnt, mass, (uint64_t)top_k, above, above_mass, end);
+      if (end <= kList) {  // everything down to the border goes to one CTA, which ends the row
+        x.each([&](float f, int i) {
+          if (f > kNegInf && bin_of(f) <= bin) {
+            Shared* o = g.cl.map_shared_rank(&s, 0);
+            o->list[atomicAdd(&o->listed, 1u)] = ((uint64_t)key_of(f) << 32) | (uint32_t)~i;
+          }
+        });
+        g.cl.sync();
+        if (g.me == 0) finish_list(s, row, (int)end, top_k, top_p, min_p, a.uniforms[r], a.ids + r);
+        return;
+      }
+      if (by_p && small_k) {  // masses after all
+        x.each([&](float f, int) {
+          if (f > kNegInf) add_mass(s, bin_of(f), mass_of(weight(row, f)));
+        });
+        g.cl.sync();
+        g.sum_bins(cnt, mass);
+        above_mass = 0;
+        uint64_t again;
+        g.find_bin(cnt, mass, (uint64_t)top_k, again, above_mass, end);
+      }
       gather(bin);
       if (listed <= kList) {
         const int need = top_k - (int)above;  // of the bin
@@ -554,8 +683,8 @@ __global__ void __launch_bounds__(kThreads) k_sample(const SampleArgs a) {
       cut = find_by_key<true>(g, x, row, cut, max(cut.key, klow), kmax, 0, mass_target(top_p, m));
     } else if (by_p) {
       const uint64_t target = mass_target(top_p, whole);
-      uint64_t above = 0, none = 0;
-      const int bin = g.find_bin(mass, cnt, target, above, none);
+      uint64_t above = 0, none = 0, end = 0;
+      const int bin = g.find_bin(mass, cnt, target, above, none, end);
       if (bin != listed_bin) {
         if (g.me == 0 && tid == 0) s.listed = 0;
         g.cl.sync();
@@ -604,9 +733,10 @@ __global__ void __launch_bounds__(kThreads) k_sample(const SampleArgs a) {
     return w >= (double)min_p || i == imax ? mass_of(w) : 0;
   };
   auto level_mass = [&](int l) -> uint64_t {
-    const float4 q = s_values[l * kThreads + tid];
+    float q[4];
+    widen4(s_values[l * kThreads + tid], q);
     const int i = x.index(l);
-    return kept_mass(q.x, i) + kept_mass(q.y, i + 1) + kept_mass(q.z, i + 2) + kept_mass(q.w, i + 3);
+    return kept_mass(q[0], i) + kept_mass(q[1], i + 1) + kept_mass(q[2], i + 2) + kept_mass(q[3], i + 3);
   };
   uint64_t sum = 0;
   __syncthreads();  // s.warp64 is free, s.table there
@@ -632,8 +762,7 @@ __global__ void __launch_bounds__(kThreads) k_sample(const SampleArgs a) {
     whole += s.all_a[g.par][i];
   }
   const uint64_t here = s.all_a[g.par][g.me];
-  const double u = fmin(fmax((double)a.uniforms[r], 0.0), 1.0 - 1.0 / 16777216.0);
-  const uint64_t goal = __umul64hi((uint64_t)(u * 18446744073709551616.0), whole);  // < whole
+  const uint64_t goal = goal_of(a.uniforms[r], whole);
   if (goal < start || goal >= start + here) return;
   uint64_t at = start;
   int l = 0;
@@ -655,8 +784,8 @@ __global__ void __launch_bounds__(kThreads) k_sample(const SampleArgs a) {
   const uint64_t m = level_mass(l);
   at += warp_inclusive(m, lane) - m;
   if (goal < at || goal >= at + m) return;
-  const float4 q = s_values[l * kThreads + tid];
-  const float f[4] = {q.x, q.y, q.z, q.w};
+  float f[4];
+  widen4(s_values[l * kThreads + tid], f);
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     const uint64_t t = kept_mass(f[e], x.index(l) + e);
@@ -668,8 +797,9 @@ __global__ void __launch_bounds__(kThreads) k_sample(const SampleArgs a) {
 template <typename T>
 cudaError_t launch_rows(const SampleArgs& a, int64_t rows, int cluster, cudaStream_t stream) {
   const void* k = reinterpret_cast<const void*>(k_sample<T>);
-  const int smem = a.levels * (kThreads * 16 + kWarps * 8);
-  cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem);
+  constexpr int level = kThreads * (int)sizeof(typename Four<T>::V) + kWarps * 8;
+  const int smem = a.levels * level;
+  cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxLevels * level);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(rows * cluster));
@@ -700,11 +830,11 @@ wr_status_t launch_sample(const SampleProblem& p, cudaStream_t stream) {
   a.temperature = p.temperatures; a.top_p = p.top_ps; a.min_p = p.min_ps; a.top_k = p.top_ks;
   a.temperature1 = p.temperature; a.top_p1 = p.top_p; a.min_p1 = p.min_p; a.top_k1 = p.top_k;
   a.ids = p.ids;
-  // The smallest cluster whose CTAs hold the row with 8 vectors a thread (64
-  // KB, so that two share an SM; fewer exchanges than with more CTAs); with
-  // few rows, for their latency, one vector a thread or the largest cluster.
+  // The smallest cluster whose CTAs hold the row in 64 KB each (so that two
+  // share an SM; fewer exchanges than with more CTAs); with few rows, for
+  // their latency, one vector a thread or the largest cluster.
   const int64_t vectors = ((int64_t)p.vocab + 3) / 4;
-  const int64_t per = p.rows * kMaxCluster <= device_sm_count() ? kThreads : 8 * kThreads;
+  const int64_t per = p.rows * kMaxCluster <= device_sm_count() ? kThreads : (elt == 2 ? 16 : 8) * kThreads;
   int cluster = 1;
   while (cluster < kMaxCluster && vectors > cluster * per) cluster *= 2;
   a.levels = (int)((vectors + (int64_t)cluster * kThreads - 1) / ((int64_t)cluster * kThreads));
