@@ -134,8 +134,56 @@ def test_several_tokens_a_sequence(nq, lens, prefix, dtype):
     check(s, out, lse)
 
 
-def test_many_rows_behind_a_prefix():
-    s = make([(i * 37) % 90 for i in range(70)], [1] * 70, 16, 2, 128, 16, 1000, torch.bfloat16)
+@pytest.mark.parametrize("n,hq,hk,d,page,prefix,layout", [
+    (70, 16, 2, 128, 16, 1000, "heads"),      # 560 rows: two tiles and a rest
+    (17, 4, 2, 128, 16, 1, "heads"),          # 34 rows, one key
+    (33, 2, 2, 64, 32, 127, "tokens"),
+    (64, 2, 1, 128, 128, 128, "heads"),       # 128 rows, whole tiles of keys
+    (65, 2, 1, 64, 256, 129, "heads"),        # pages larger than a tile
+    (43, 6, 2, 128, 64, 4000, "tokens"),      # a group that does not divide a tile
+    (256, 8, 8, 64, 16, 511, "heads"),
+    (130, 48, 8, 128, 64, 2500, "heads"),
+    (40, 4, 4, 128, 8, 300, "heads"),         # pages too small for TMA copies of tiles
+    (40, 4, 4, 96, 16, 300, "heads"),
+    (40, 4, 4, 128, 24, 300, "heads"),
+])
+def test_many_rows_behind_a_prefix(n, hq, hk, d, page, prefix, layout):
+    s = make([(i * 37) % 90 for i in range(n)], [1] * n, hq, hk, d, page, prefix, torch.bfloat16, layout=layout)
+    out, lse = call(s, return_lse=True)
+    check(s, out, lse)
+    again, _ = call(s, return_lse=True)
+    assert torch.equal(out, again)
+
+
+def test_scores_that_grow_along_the_prefix():
+    """The running maximum moves by more than the kernels tolerate without
+    rescaling, again and again, for some rows and not for others."""
+    s = make([5] * 80, [1] * 80, 4, 2, 128, 16, 2000, torch.bfloat16)
+    ramp = torch.linspace(0.05, 3.0, 2000, device="cuda")
+    pages = s["prefix_pages"].long()
+    for i, p in enumerate(pages.tolist()):
+        rows = min(16, 2000 - 16 * i)
+        s["k_cache"][p, :, :rows] *= ramp[16 * i:16 * i + rows, None].to(torch.bfloat16)
+    s["q"][::3] *= 4
+    out, lse = call(s, return_lse=True)
+    check(s, out, lse)
+
+
+def test_bad_pages_hide_a_tile_of_the_prefix():
+    s = make([9] * 50, [1] * 50, 4, 2, 128, 16, 500, torch.bfloat16)
+    s["prefix_pages"][3] = -1
+    s["prefix_pages"][8:16] = 2 ** 31 - 1   # a whole tile of 128 keys
+    s["prefix_pages"][-1] = s["k_cache"].shape[0]
+    out, lse = call(s, return_lse=True)
+    check(s, out, lse)
+    s["prefix_pages"][:] = -7               # nothing of the prefix is left
+    out, lse = call(s, return_lse=True)
+    check(s, out, lse)
+
+
+def test_several_tokens_and_many_rows():
+    s = make([(i * 53) % 200 + 9 for i in range(24)], [i % 9 + 1 for i in range(24)], 8, 2, 128, 32, 1111,
+             torch.bfloat16)
     out, lse = call(s, return_lse=True)
     check(s, out, lse)
 

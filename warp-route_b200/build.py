@@ -32,8 +32,10 @@ NVCC_FLAGS = ARCH + ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC",
                      "-Xcompiler", "-fvisibility=hidden", "--expt-relaxed-constexpr",
                      "-I" + INCLUDE, "-I" + CSRC]
 KERNEL_SOURCES = ["wr_api.cu", "wr_fused.cu", "wr_naive.cu", "wr_noalloc.cu", "wr_comm.cu",
-                  "wr_grouped.cu", "wr_pack.cu", "wr_kvcache.cu", "wr_attention.cu", "wr_sample.cu"]
-HEADERS = ["wr_common.cuh", "wr_router.cuh", "wr_internal.h", "wr_attention.cuh"]
+                  "wr_grouped.cu", "wr_pack.cu", "wr_kvcache.cu", "wr_attention.cu",
+                  "wr_attn_prefix.cu", "wr_sample.cu"]
+HEADERS = ["wr_common.cuh", "wr_router.cuh", "wr_internal.h", "wr_attention.cuh",
+           "wr_tcgen05.cuh"]
 
 
 def _sig(paths, flags) -> str:

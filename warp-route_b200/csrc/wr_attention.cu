@@ -697,30 +697,28 @@ __global__ void __launch_bounds__(StreamF32Cfg<DP>::kWarps * 32) k_attn_stream_f
 struct CombineArgs {
   AttnArgs own;       // the launch over the sequences' own keys
   int64_t own_warps;
-  AttnArgs pre;       // the launch over the prefix (pre_kind == 1)
-  int64_t pre_warps;
-  int pre_kind;       // 0: none, 1: k_attn_stream*, 2: splits [splits][rows of all tokens][dim]
-  const float* split;
-  const float2* split_ml;
-  int splits;
-  int64_t split_rows;
+  int has_pre;        // a launch over the prefix: its partial results
+  AttnPartials pre;
+  const float* pre_home;
+  const float2* pre_home_ml;
+  AttnSplit pre_split;
+  int pre_mr, pre_rts, pre_us;  // rows a tile, tiles a key head, units of its keys
 };
 
-// The pieces of a row of one launch: piece i of `n` lies at row(i).
+// A row's pieces of one launch: whole (in home), or n in slots of the warps
+// (or CTAs) from w0 on.
 struct PieceList {
   int64_t w0;
-  int n, rl, mr;
+  int n, rl;
   bool whole;
 };
-template <int MR>
-WR_DEVINL PieceList piece_list(const AttnSplit& sp, int64_t unit0, int us, int r) {
+WR_DEVINL PieceList piece_list(const AttnSplit& sp, int64_t unit0, int us, int row_in_tile) {
   PieceList p;
   const int64_t w0 = range_of(sp, unit0), w1 = range_of(sp, unit0 + us - 1);
   p.whole = w0 == w1;
   p.w0 = w0;
   p.n = (int)(w1 - w0) + 1;
-  p.rl = r % MR;
-  p.mr = MR;
+  p.rl = row_in_tile;
   return p;
 }
 
@@ -748,48 +746,27 @@ __global__ void __launch_bounds__(kWarps == 1 ? 128 : kWarps * 32) k_attn_combin
     sp.units = a.seq_unit[a.B];
     sp.ranges = min(c.own_warps, sp.units);
     const int r = (t - s.q0) * a.group + g;
-    po = piece_list<MR>(sp, a.seq_unit[b] + ((int64_t)h * rts + r / MR) * us, us, r);
+    po = piece_list(sp, a.seq_unit[b] + ((int64_t)h * rts + r / MR) * us, us, r % MR);
     done = po.whole && a.direct;
   }
   if (done) return;  // written by the first kernel
-  if (c.pre_kind == 1 && b >= 0) {
-    const SeqInfo s = seq_info(c.pre, 0);
-    const int us = key_units(c.pre, s), rts = row_tiles<MR>(c.pre, s);
-    AttnSplit sp;
-    sp.units = (int64_t)a.hkv * rts * us;
-    sp.ranges = min(c.pre_warps, sp.units);
-    const int r = t * a.group + g;
-    pp = piece_list<MR>(sp, ((int64_t)h * rts + r / MR) * us, us, r);
-  } else if (c.pre_kind == 2 && b >= 0) {
-    pp.n = c.splits;
+  if (c.has_pre && b >= 0) {
+    const int r = t * a.group + g, rt = r / c.pre_mr;
+    pp = piece_list(c.pre_split, ((int64_t)h * c.pre_rts + rt) * c.pre_us, c.pre_us, r - rt * c.pre_mr);
   }
   const int total = po.n + pp.n;
   float m = WR_NEG_INF, l = 0.f, o[VC];
 #pragma unroll
   for (int i = 0; i < VC; ++i) o[i] = 0.f;
-  const int64_t prow = (int64_t)h * c.split_rows + (int64_t)t * a.group + g;
 #pragma unroll 4
   for (int i = kWarps == 1 ? 0 : wid; i < total; i += kWarps) {
-    const float* src;
-    float2 ml;
-    if (i < po.n || c.pre_kind == 1) {
-      const bool mine = i < po.n;
-      const PieceList& p = mine ? po : pp;
-      const AttnArgs& x = mine ? a : c.pre;
-      const int k = mine ? i : i - po.n;
-      if (p.whole) {
-        src = x.home + row * a.dim;
-        ml = x.home_ml[row];
-      } else {
-        const int64_t at = ((p.w0 + k) * 2 + (k == 0 ? 1 : 0)) * MR + p.rl;
-        src = x.part.piece + at * a.dim;
-        ml = x.part.piece_ml[at];
-      }
-    } else {
-      const int64_t at = (int64_t)(i - po.n) * a.hkv * c.split_rows + prow;
-      src = c.split + at * a.dim;
-      ml = c.split_ml[at];
-    }
+    const bool mine = i < po.n;
+    const PieceList& p = mine ? po : pp;
+    const int k = mine ? i : i - po.n;
+    const AttnPartials& part = mine ? a.part : c.pre;
+    const int64_t at = p.whole ? row : ((p.w0 + k) * 2 + (k == 0 ? 1 : 0)) * (mine ? MR : c.pre_mr) + p.rl;
+    const float* src = (p.whole ? (mine ? a.home : c.pre_home) : part.piece) + at * a.dim;
+    const float2 ml = (p.whole ? (mine ? a.home_ml : c.pre_home_ml) : part.piece_ml)[at];
     const float nm = fmaxf(m, ml.x);
     const float base = nm == WR_NEG_INF ? 0.f : nm;
     const float fo = ex2(m - base), fn = ex2(ml.x - base);
@@ -846,11 +823,17 @@ __global__ void __launch_bounds__(kWarps == 1 ? 128 : kWarps * 32) k_attn_combin
 // ---------------------------------------------------------------------------
 // Host
 // ---------------------------------------------------------------------------
+// From this many rows a key head the prefix goes to the tensor cores; the
+// warps of k_attn_stream take 16 rows each and read the keys again for every 16.
+constexpr int kTileMinRows = 32;
+
 struct Plan {
   int dp, mr, warps_cta, smem;
   int own_grid, pre_grid;
-  int pre_kind;      // see CombineArgs
   int inline_prefix; // each sequence reads the prefix with its own keys
+  int has_pre;       // the prefix has a launch of its own,
+  int tiles;         // on the tensor cores
+  int pre_mr, pre_unit;
   int64_t rows;      // T * hq
   size_t off_piece, off_piece_ml, off_home, off_home_ml, off_seq, off_tok;
   size_t off_ppiece, off_ppiece_ml, off_phome, off_phome_ml;
@@ -868,9 +851,13 @@ Plan make_plan(const AttnProblem& p) {
   const int per_sm = 228 * 1024 / (pl.smem + 4096) < 1 ? 1 : (228 * 1024 / (pl.smem + 4096) > 4 ? 4 : 228 * 1024 / (pl.smem + 4096));
   const int64_t most = (int64_t)device_sm_count() * per_sm;
   const int group = p.hq / p.c.hkv;
-  pl.rows = (int64_t)p.T * p.hq;
+  pl.rows = (int64_t)p.T * p.hq;  // of the output
   pl.inline_prefix = p.prefix_len > 0 && p.B == 1;
-  pl.pre_kind = p.prefix_len > 0 && !pl.inline_prefix ? 1 : 0;
+  pl.has_pre = p.prefix_len > 0 && !pl.inline_prefix;
+  const int64_t group_rows = (int64_t)p.T * group;  // rows that meet the prefix, a key head
+  pl.tiles = pl.has_pre && group_rows > kTileMinRows && prefix_tiles_ok(p);
+  pl.pre_mr = pl.tiles ? (group_rows > 128 ? 256 : 128) : pl.mr;
+  pl.pre_unit = pl.tiles ? kPrefixUnit : kUnitTokens;
   // An upper bound of the units: the lengths are on the device.
   const int64_t keys = (int64_t)p.table_width * p.c.page_size + (pl.inline_prefix ? p.prefix_len : 0);
   const int64_t tiles = ((int64_t)p.T * group + pl.mr - 1) / pl.mr + (p.B > 0 ? p.B : 0);
@@ -886,18 +873,19 @@ Plan make_plan(const AttnProblem& p) {
   const size_t own_rows = (size_t)pl.own_grid * pl.warps_cta * 2 * pl.mr;
   pl.off_piece = take(own_rows * p.c.dim * 4);
   pl.off_piece_ml = take(own_rows * 8);
-  if (pl.pre_kind) {
+  if (pl.has_pre) {
     pl.off_home = take((size_t)pl.rows * p.c.dim * 4);
     pl.off_home_ml = take((size_t)pl.rows * 8);
   }
   pl.off_seq = take((size_t)(p.B + 1) * 8);
   pl.off_tok = take((size_t)(p.q_start ? p.T : 0) * 4);
-  if (pl.pre_kind == 1) {
-    const int64_t pu = (int64_t)p.c.hkv * (((int64_t)p.T * group + pl.mr - 1) / pl.mr) *
-                       ((p.prefix_len + kUnitTokens - 1) / kUnitTokens);
-    const int64_t pc = (pu + pl.warps_cta - 1) / pl.warps_cta;
-    pl.pre_grid = (int)(pc < most ? pc : most);
-    const size_t pre_rows = (size_t)pl.pre_grid * pl.warps_cta * 2 * pl.mr;
+  if (pl.has_pre) {
+    const int64_t pu = (int64_t)p.c.hkv * ((group_rows + pl.pre_mr - 1) / pl.pre_mr) *
+                       ((p.prefix_len + pl.pre_unit - 1) / pl.pre_unit);
+    const int ways = pl.tiles ? 1 : pl.warps_cta;  // ranges a CTA
+    const int64_t pc = (pu + ways - 1) / ways, cap = pl.tiles ? device_sm_count() : most;
+    pl.pre_grid = (int)(pc < cap ? pc : cap);
+    const size_t pre_rows = (size_t)pl.pre_grid * ways * 2 * pl.pre_mr;
     pl.off_ppiece = take(pre_rows * p.c.dim * 4);
     pl.off_ppiece_ml = take(pre_rows * 8);
     pl.off_phome = take((size_t)pl.rows * p.c.dim * 4);
@@ -969,7 +957,7 @@ wr_status_t launch_attn(const AttnProblem& p, void* ws, cudaStream_t stream) {
   a.table_width = p.table_width;
   a.prefix = pl.inline_prefix ? p.prefix_len : 0;
   a.own = 1;
-  a.direct = pl.pre_kind == 0;
+  a.direct = !pl.has_pre;
   a.scale_log2 = p.scale * kLog2e;
   a.part.piece = reinterpret_cast<float*>(base + pl.off_piece);
   a.part.piece_ml = reinterpret_cast<float2*>(base + pl.off_piece_ml);
@@ -981,21 +969,33 @@ wr_status_t launch_attn(const AttnProblem& p, void* ws, cudaStream_t stream) {
   CombineArgs c{};
   c.own = a;
   c.own_warps = (int64_t)pl.own_grid * pl.warps_cta;
-  c.pre_kind = pl.pre_kind;
   cudaError_t e;
-  if (pl.pre_kind == 1) {
+  if (pl.has_pre) {
     AttnArgs x = a;
     x.B = 1; x.own = 0; x.prefix = p.prefix_len; x.direct = 0; x.q_start = nullptr;
     x.part.piece = reinterpret_cast<float*>(base + pl.off_ppiece);
     x.part.piece_ml = reinterpret_cast<float2*>(base + pl.off_ppiece_ml);
     x.home = reinterpret_cast<float*>(base + pl.off_phome);
     x.home_ml = reinterpret_cast<float2*>(base + pl.off_phome_ml);
-    c.pre = x;
-    c.pre_warps = (int64_t)pl.pre_grid * pl.warps_cta;
-    e = launch_stream(pl, f32, x, pl.pre_grid, false, stream);
-    if (e != cudaSuccess) return cuda_fail(e, "shared_prefix_attention (prefix) launch");
+    c.has_pre = 1;
+    c.pre = x.part;
+    c.pre_home = x.home;
+    c.pre_home_ml = x.home_ml;
+    c.pre_mr = pl.pre_mr;
+    c.pre_rts = (int)(((int64_t)p.T * a.group + pl.pre_mr - 1) / pl.pre_mr);
+    c.pre_us = (p.prefix_len + pl.pre_unit - 1) / pl.pre_unit;
+    c.pre_split.units = (int64_t)a.hkv * c.pre_rts * c.pre_us;
+    const int64_t ranges = (int64_t)pl.pre_grid * (pl.tiles ? 1 : pl.warps_cta);
+    c.pre_split.ranges = ranges < c.pre_split.units ? ranges : c.pre_split.units;
+    if (pl.tiles) {
+      const wr_status_t st = launch_attn_prefix(p, x, pl.pre_mr, pl.pre_grid, stream);
+      if (st != WR_OK) return st;
+    } else {
+      e = launch_stream(pl, f32, x, pl.pre_grid, false, stream);
+      if (e != cudaSuccess) return cuda_fail(e, "shared_prefix_attention (prefix) launch");
+    }
   }
-  e = launch_stream(pl, f32, a, pl.own_grid, pl.pre_kind != 0, stream);
+  e = launch_stream(pl, f32, a, pl.own_grid, pl.has_pre, stream);
   if (e != cudaSuccess) return cuda_fail(e, "shared_prefix_attention launch");
   // Few rows: 8 warps a row read its many pieces; many rows: a warp each.
   const bool wide = pl.rows <= (int64_t)device_sm_count() * 8;

@@ -64,6 +64,13 @@ struct AttnArgs {
   float* lse;
 };
 
+// The prefix on the tensor cores (wr_attn_prefix.cu): units of 128 keys, row
+// tiles of 128 or 256 rows, one CTA a range.
+constexpr int kPrefixUnit = 128;
+bool prefix_tiles_ok(const AttnProblem& p);
+wr_status_t launch_attn_prefix(const AttnProblem& p, const AttnArgs& a, int row_tile, int grid,
+                               cudaStream_t stream);
+
 // Keys that a page holds: index and rest.
 WR_DEVINL void split_page(int j, int page_size, int shift, int& page, int& row) {
   page = shift >= 0 ? j >> shift : j / page_size;

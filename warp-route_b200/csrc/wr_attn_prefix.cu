@@ -1,0 +1,488 @@
+// wr_attn_prefix.cu — the shared prefix's part of the attention on the tensor
+// cores: the rows of all sequences' tokens meet the prefix's keys once.
+//
+// A product of [rows, keys] and one of [rows, dim], 4 * rows * keys * dim
+// operations for 4 * keys * dim bytes: from some 200 rows a key head on the
+// tensor cores (and, next to them, the exponentials: rows * keys of them, 16 a
+// cycle and SM, take as long as both products at dim 128) bound it, below that
+// HBM.
+//
+// A CTA has one SM and NT tiles of 128 rows (NT 2 when there are that many:
+// while one tile's softmax runs, the tensor core works on the other).  Per
+// 128 keys: S = Q K^T into TMEM; a thread reads its row of S (lane = row, so
+// no exchange between threads), takes the running maximum and the weights
+// 2^(s - m), which go back over S as bf16, the A operand of O += P V, whose
+// sum stays in TMEM for all of a piece's keys.  m follows the true maximum
+// only when it has grown by more than 8 (a factor of 256, harmless in fp32
+// sums and bf16 weights), so O is rescaled rarely.  Warp 4 * NT brings K and V
+// by TMA, a copy a page and 64 columns, into two rings; the next warp issues
+// the MMAs.  Keys in pages outside the cache, and those behind the prefix's
+// end in its last page, are masked in S and their rows of V set to zero.
+//
+// The (key head, row tiles, 128 keys) units are dealt to the CTAs in ranges of
+// equal length, their pieces joined by k_attn_combine (wr_attention.cu).
+//
+// Every wait is bounded.  One that runs out ends the CTA's work and leaves NaN
+// in the rows of its pieces, in their sums, so that it shows in the output.
+#include "wr_attention.cuh"
+#include "wr_tcgen05.cuh"
+
+namespace wr {
+namespace {
+
+constexpr int kTileKeys = kPrefixUnit;
+constexpr int kTileRows = 128;
+constexpr int kMaskRing = 8;
+constexpr float kRescale = 8.f;
+#define WR_NEG_INF (-__int_as_float(0x7f800000))
+
+template <int D, int NT>
+struct Cfg {
+  static constexpr int kStages = D == 64 ? 4 : (NT == 2 ? 2 : 3);
+  static_assert(kStages <= 4, "mask ring");
+  static constexpr int kPanels = D / 64;
+  static constexpr int kPanelBytes = 128 * 128;  // 128 rows of 64 columns
+  static constexpr int kTileBytes = kPanels * kPanelBytes;
+  static constexpr int kSmem = 1024 + NT * kTileBytes + 2 * kStages * kTileBytes;
+  static constexpr int kThreads = NT * 128 + 64;
+  static constexpr uint32_t kTmemCols = NT == 2 ? 512 : 256;
+};
+
+struct PrefixArgs {
+  AttnArgs a;
+  int pairs;  // row tiles of NT * 128 rows a key head
+  int us;     // units of 128 keys
+  AttnSplit sp;
+  int box;    // keys of one TMA copy
+};
+
+WR_DEVINL float ex2p(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// A CTA's pieces in order: the units of one (key head, row tiles) in its range.
+struct Piece {
+  int h, pair, u, n;
+};
+WR_DEVINL Piece piece_at(const PrefixArgs& p, int64_t unit, int64_t end) {
+  Piece x;
+  const int64_t tile = unit / p.us;
+  x.u = (int)(unit - tile * p.us);
+  x.h = (int)(tile / p.pairs);
+  x.pair = (int)(tile - (int64_t)x.h * p.pairs);
+  x.n = (int)min((int64_t)(p.us - x.u), end - unit);
+  return x;
+}
+
+template <int D, int NT>
+__global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1)
+    k_attn_prefix(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
+                  const PrefixArgs p) {
+  using C = Cfg<D, NT>;
+  constexpr int S = C::kStages, MR = NT * kTileRows;
+  extern __shared__ uint8_t s_raw[];
+  __shared__ uint64_t k_full[S], k_empty[S], v_full[S], v_empty[S], aux;
+  __shared__ uint64_t q_full[NT], s_full[NT], p_full[NT], pv_done[NT];
+  __shared__ uint32_t s_mask[kMaskRing][4], s_special[kMaskRing], s_tmem;
+  __shared__ int s_abort;
+  const AttnArgs& a = p.a;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(s_raw) + 1023) & ~(uintptr_t)1023);
+  uint8_t* qbuf = smem;
+  uint8_t* kbuf = qbuf + NT * C::kTileBytes;
+  uint8_t* vbuf = kbuf + S * C::kTileBytes;
+  volatile int* abort = &s_abort;
+
+  griddep_launch_dependents();
+  if (tid == 0) {
+    for (int i = 0; i < S; ++i) {
+      mbar_init(&k_full[i], 1);
+      mbar_init(&k_empty[i], 1);
+      mbar_init(&v_full[i], 1);
+      mbar_init(&v_empty[i], 1);
+    }
+    for (int t = 0; t < NT; ++t) {
+      mbar_init(&q_full[t], kTileRows);
+      mbar_init(&s_full[t], 1);
+      mbar_init(&p_full[t], kTileRows);
+      mbar_init(&pv_done[t], 1);
+    }
+    mbar_init(&aux, 1);
+    s_abort = 0;
+    fence_mbar_init();
+  }
+  if (warp == NT * 4 + 1) {
+    tmem_alloc(&s_tmem, C::kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = s_tmem;
+  const uint32_t tmem_s = tmem, tmem_o = tmem + NT * kTileKeys;
+  const int64_t u0 = range_start(p.sp, blockIdx.x), u1 = range_start(p.sp, blockIdx.x + 1);
+  const int total = (int)(u1 - u0);
+
+  if (warp == NT * 4) {
+    // ---- K and V, by TMA -------------------------------------------------
+    const uint64_t policy = l2_policy_evict_last();  // other CTAs read the same keys
+    const int per_tile = kTileKeys / p.box;          // copies a tile and panel
+    const int ops = per_tile * C::kPanels;
+    const uint32_t op_bytes = (uint32_t)p.box * 128;
+    int issued_k = 0, issued_v = 0;
+    uint32_t aux_phase = 0;
+    int64_t unit = u0;
+    int it = 0;
+    while (it < total && !*abort) {
+      const Piece pc = piece_at(p, unit, u1);
+      for (int i = 0; i < pc.n && !*abort; ++i, ++it) {
+        const int st = it % S;
+        const uint32_t ph = (it / S) & 1;
+        const int key0 = (pc.u + i) * kTileKeys;
+        const int pi = lane / C::kPanels, panel = lane % C::kPanels;
+        const int k0 = key0 + pi * p.box;
+        int page = -1, row = 0;
+        if (lane < ops && k0 < a.prefix) {
+          int idx;
+          split_page(k0, a.page_size, a.page_shift, idx, row);
+          page = __ldg(a.prefix_pages + idx);
+        }
+        const bool ok = page >= 0 && page < a.num_pages;
+        const uint32_t oks = __ballot_sync(0xffffffffu, ok);
+        const uint32_t bytes = __popc(oks) * op_bytes;
+        const bool special = __popc(oks) != ops || key0 + kTileKeys > a.prefix;
+        // Keys of this tile that count: word w of the mask, by lane w.
+        uint32_t word = 0xffffffffu;
+        if (special) {
+          word = 0;
+          for (int j = 0; j < 32; ++j) {
+            const int key = lane * 32 + j;  // lanes 0..3 alone are used
+            const bool in = lane < 4 && key0 + key < a.prefix && ((oks >> ((key / p.box) * C::kPanels)) & 1);
+            word |= (uint32_t)in << j;
+          }
+        }
+        if (it >= S && !mbar_wait(&k_empty[st], ph ^ 1, abort)) *abort = 1;
+        __syncwarp();
+        if (*abort) break;
+        if (lane < 4) s_mask[it % kMaskRing][lane] = word;
+        if (lane == 0) s_special[it % kMaskRing] = special;
+        __syncwarp();
+        if (lane == 0) {
+          if (bytes) mbar_arrive_expect_tx(&k_full[st], bytes); else mbar_arrive(&k_full[st]);
+        }
+        __syncwarp();
+        uint8_t* dst = kbuf + st * C::kTileBytes + panel * C::kPanelBytes + pi * p.box * 128;
+        if (ok) tma_load_4d(dst, &kmap, panel * 64, row, pc.h, page, &k_full[st], policy);
+        issued_k = it + 1;
+        if (it >= S && !mbar_wait(&v_empty[st], ph ^ 1, abort)) *abort = 1;
+        __syncwarp();
+        if (*abort) break;
+        dst += vbuf - kbuf;
+        uint64_t* bar = special ? &aux : &v_full[st];
+        if (lane == 0) {
+          if (bytes) mbar_arrive_expect_tx(bar, bytes); else mbar_arrive(bar);
+        }
+        __syncwarp();
+        if (ok) tma_load_4d(dst, &vmap, panel * 64, row, pc.h, page, bar, policy);
+        if (special) {
+          // What the copies left behind the prefix, or did not bring, becomes 0.
+          if (!mbar_wait(&aux, aux_phase, nullptr)) *abort = 1;
+          aux_phase ^= 1;
+          for (int key = 0; key < kTileKeys; ++key) {
+            const uint32_t w = __shfl_sync(0xffffffffu, word, key >> 5);
+            if ((w >> (key & 31)) & 1) continue;
+            if (lane < 8 * C::kPanels)
+              *reinterpret_cast<uint4*>(vbuf + st * C::kTileBytes + (lane >> 3) * C::kPanelBytes + key * 128 +
+                                        (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&v_full[st]);
+        }
+        issued_v = it + 1;
+      }
+      unit += pc.n;
+    }
+    // Nothing of this CTA's is in flight when it ends: copies have landed, and
+    // (unless it gave up) the MMAs have released the stages.
+    for (int i = max(0, issued_k - S); i < issued_k; ++i)
+      mbar_wait(*abort ? &k_full[i % S] : &k_empty[i % S], (i / S) & 1, nullptr);
+    for (int i = max(0, issued_v - S); i < issued_v; ++i)
+      mbar_wait(*abort ? &v_full[i % S] : &v_empty[i % S], (i / S) & 1, nullptr);
+  } else if (warp == NT * 4 + 1) {
+    // ---- the MMAs ---------------------------------------------------------
+    if (lane == 0) {
+      const uint32_t id_qk = idesc_bf16(kTileRows, kTileKeys);
+      const uint32_t id_pv = idesc_bf16(kTileRows, D) | kIdescBMajorMn;
+      auto qk = [&](int t, int it) {  // S_t = Q_t K^T
+        const uint32_t qa = smem_u32(qbuf + t * C::kTileBytes), ka = smem_u32(kbuf + (it % S) * C::kTileBytes);
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+          const uint32_t off = (k >> 2) * C::kPanelBytes + (k & 3) * 32;
+          umma_bf16(tmem_s + t * kTileKeys, sw128_desc(qa + off), sw128_desc(ka + off), id_qk, k > 0);
+        }
+        if (t == NT - 1) umma_commit(&k_empty[it % S]);
+        umma_commit(&s_full[t]);
+      };
+      auto pv = [&](int t, int it, bool more) {  // O_t (+)= P_t V
+        const uint32_t va = smem_u32(vbuf + (it % S) * C::kTileBytes);
+#pragma unroll
+        for (int k = 0; k < kTileKeys / 16; ++k)
+          umma_bf16_ta(tmem_o + t * D, tmem_s + t * kTileKeys + k * 8,
+                       sw128_desc_mn(va + k * 2048, C::kPanelBytes), id_pv, more || k > 0);
+        if (t == NT - 1) umma_commit(&v_empty[it % S]);
+        umma_commit(&pv_done[t]);
+      };
+      bool dead = false;
+      auto wait = [&](uint64_t* bar, uint32_t parity) {
+        if (!dead && !mbar_wait(bar, parity, abort)) {
+          *abort = 1;
+          dead = true;
+        }
+        return !dead;
+      };
+      int64_t unit = u0;
+      int it = 0, piece = 0;
+      while (it < total && !dead) {
+        const Piece pc = piece_at(p, unit, u1);
+        for (int t = 0; t < NT; ++t) wait(&q_full[t], piece & 1);
+        wait(&k_full[it % S], (it / S) & 1);
+        for (int t = 0; t < NT && !dead; ++t) {
+          if (it > 0 && !wait(&pv_done[t], (it - 1) & 1)) break;
+          tc_fence_after();
+          qk(t, it);
+        }
+        for (int i = 0; i < pc.n && !dead; ++i, ++it) {
+          for (int t = 0; t < NT && !dead; ++t) {
+            if (!wait(&p_full[t], it & 1) || !wait(&v_full[it % S], (it / S) & 1)) break;
+            tc_fence_after();
+            pv(t, it, i > 0);
+            if (i + 1 < pc.n) {
+              if (!wait(&k_full[(it + 1) % S], ((it + 1) / S) & 1) || !wait(&pv_done[t], it & 1)) break;
+              tc_fence_after();
+              qk(t, it + 1);
+            }
+          }
+        }
+        unit += pc.n;
+        ++piece;
+      }
+      if (dead) {  // let what was issued end
+        umma_commit(&aux);
+        const uint64_t t0 = globaltimer_ns();
+        while (globaltimer_ns() - t0 < 1000000) {
+        }
+      }
+    }
+    __syncwarp();
+  } else {
+    // ---- softmax: thread = row of tile t ----------------------------------
+    const int t = warp >> 2, rl = tid & 127;
+    const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // this warp's 32 TMEM lanes
+    const uint32_t ts = tmem_s + t * kTileKeys + lanes, to = tmem_o + t * D + lanes;
+    const float c = a.scale_log2;
+    int64_t unit = u0;
+    int it = 0;
+    bool dead = false;
+    while (unit < u1) {
+      const Piece pc = piece_at(p, unit, u1);
+      const int r = pc.pair * MR + t * kTileRows + rl;
+      const int tok = r / a.group, g = r - tok * a.group;
+      const bool in = tok < a.T;
+      if (!dead) {  // this row of Q
+        const uint16_t* src = static_cast<const uint16_t*>(a.q) + (int64_t)tok * a.q_ts +
+                              (int64_t)(pc.h * a.group + g) * a.q_hs;
+        uint8_t* dst = qbuf + t * C::kTileBytes + rl * 128;
+#pragma unroll
+        for (int k = 0; k < D / 8; ++k) {
+          const uint4 v = in ? *reinterpret_cast<const uint4*>(src + k * 8) : make_uint4(0, 0, 0, 0);
+          *reinterpret_cast<uint4*>(dst + (k >> 3) * C::kPanelBytes + (((k & 7) ^ (rl & 7)) << 4)) = v;
+        }
+        fence_proxy_async_smem();
+        mbar_arrive(&q_full[t]);
+      }
+      float m = WR_NEG_INF, l = 0.f;
+      for (int i = 0; i < pc.n && !dead; ++i, ++it) {
+        if (!mbar_wait(&s_full[t], it & 1, abort)) {
+          *abort = 1;
+          dead = true;
+          break;
+        }
+        tc_fence_after();
+        // Twice over S, 32 columns at a time: the whole row does not fit into
+        // registers beside the rest, and TMEM reads are cheap.
+        const bool special = s_special[it % kMaskRing];
+        auto mask = [&](uint32_t (&s)[32], int k) {
+          if (!special) return;
+          const uint32_t w = s_mask[it % kMaskRing][k];
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            if (!((w >> j) & 1)) s[j] = 0xff800000u;
+        };
+        uint32_t s[2][32];
+        float mx[4] = {WR_NEG_INF, WR_NEG_INF, WR_NEG_INF, WR_NEG_INF};
+#pragma unroll
+        for (int k = 0; k < 4; k += 2) {
+          tmem_ld32(ts + k * 32, s[0]);
+          tmem_ld32(ts + k * 32 + 32, s[1]);
+          tmem_wait_lds();
+          reg_dep32(s[0]);
+          reg_dep32(s[1]);
+          mask(s[0], k);
+          mask(s[1], k + 1);
+#pragma unroll
+          for (int j = 0; j < 32; j += 2) {
+            mx[j & 2] = fmaxf(mx[j & 2], fmaxf(__uint_as_float(s[0][j]), __uint_as_float(s[0][j + 1])));
+            mx[1 + (j & 2)] = fmaxf(mx[1 + (j & 2)], fmaxf(__uint_as_float(s[1][j]), __uint_as_float(s[1][j + 1])));
+          }
+        }
+        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c;
+        if (i == 0) {
+          m = top;
+        } else {
+          const bool up = top > m + kRescale;
+          if (__any_sync(0xffffffffu, up)) {
+            const float nm = up ? top : m;
+            const float f = up ? ex2p(m - nm) : 1.f;
+            m = nm;
+            l *= f;
+#pragma unroll
+            for (int k = 0; k < D / 32; ++k) {
+              uint32_t o[32];
+              tmem_ld32(to + k * 32, o);
+              tmem_wait_lds();
+              reg_dep32(o);
+#pragma unroll
+              for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
+              tmem_st32(to + k * 32, o);
+            }
+          }
+        }
+        const float base = m == WR_NEG_INF ? 0.f : m;
+        float ls[4] = {0.f, 0.f, 0.f, 0.f};
+        tmem_ld32(ts, s[0]);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          tmem_wait_lds();
+          reg_dep32(s[k & 1]);
+          if (k < 3) tmem_ld32(ts + k * 32 + 32, s[(k + 1) & 1]);
+          mask(s[k & 1], k);
+          uint32_t w[16];
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            const float x = ex2p(fmaf(__uint_as_float(s[k & 1][2 * j]), c, -base));
+            const float y = ex2p(fmaf(__uint_as_float(s[k & 1][2 * j + 1]), c, -base));
+            ls[j & 3] += x + y;
+            __nv_bfloat162 b = __floats2bfloat162_rn(x, y);
+            w[j] = *reinterpret_cast<uint32_t*>(&b);
+          }
+          // columns 16 k .. 16 k + 15, whose scores have been read
+          tmem_st16(ts + k * 16, w);
+        }
+        l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(&p_full[t]);
+      }
+      if (!dead && !mbar_wait(&pv_done[t], (it - 1) & 1, abort)) {
+        *abort = 1;
+        dead = true;
+      }
+      // The piece's result.
+      const bool whole = pc.u == 0 && pc.n == p.us;
+      const int64_t orow = (int64_t)tok * a.hq + pc.h * a.group + g;
+      const int64_t prow = ((int64_t)blockIdx.x * 2 + (pc.u == 0 ? 1 : 0)) * MR + t * kTileRows + rl;
+      float* op = whole ? a.home + orow * D : a.part.piece + prow * D;
+      if (!dead) {
+        tc_fence_after();
+#pragma unroll
+        for (int k = 0; k < D / 32; ++k) {
+          uint32_t o[32];
+          tmem_ld32(to + k * 32, o);
+          tmem_wait_lds();
+          reg_dep32(o);
+          if (in)
+#pragma unroll
+            for (int j = 0; j < 32; j += 4)
+              *reinterpret_cast<uint4*>(op + k * 32 + j) = make_uint4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+        }
+        tc_fence_before();
+      } else {
+        l = __int_as_float(0x7fc00000);
+        m = 0.f;
+      }
+      if (in) (whole ? a.home_ml + orow : a.part.piece_ml + prow)[0] = make_float2(m, l);
+      unit += pc.n;  // once dead, the pieces that are left get NaN too
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == NT * 4 + 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, C::kTmemCols);
+  }
+}
+
+template <int D, int NT>
+cudaError_t launch_tiles(const CUtensorMap& km, const CUtensorMap& vm, const PrefixArgs& p, int grid,
+                         cudaStream_t stream) {
+  using C = Cfg<D, NT>;
+  const void* k = reinterpret_cast<const void*>(k_attn_prefix<D, NT>);
+  const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+  if (e != cudaSuccess) return e;
+  void* args[3] = {const_cast<CUtensorMap*>(&km), const_cast<CUtensorMap*>(&vm), const_cast<PrefixArgs*>(&p)};
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(C::kThreads);
+  cfg.dynamicSmemBytes = C::kSmem;
+  cfg.stream = stream;
+  return cudaLaunchKernelExC(&cfg, k, args);
+}
+
+}  // namespace
+
+// TMA copies want pages that cut a tile of 128 keys evenly (or the reverse),
+// 16 keys at least so that a warp's 32 lanes issue a tile's copies at once,
+// and strides other than 0.
+bool prefix_tiles_ok(const AttnProblem& p) {
+  const PagedKv& c = p.c;
+  const bool strides = (c.num_pages == 1 || c.page_stride > 0) && (c.hkv == 1 || c.head_stride > 0) &&
+                       (c.page_size == 1 || c.slot_stride > 0);
+  const int64_t most = (int64_t)1 << 38;  // elements; tensor maps hold strides below 2^40 bytes
+  return c.dtype == WR_DTYPE_BF16 && (c.dim == 64 || c.dim == 128) && p.scale > 1e-30f && p.scale < 1e30f && c.page_size >= 16 &&
+         (c.page_size & (c.page_size - 1)) == 0 && strides && c.page_stride < most && c.head_stride < most &&
+         c.slot_stride < most;
+}
+
+wr_status_t launch_attn_prefix(const AttnProblem& p, const AttnArgs& a, int row_tile, int grid,
+                               cudaStream_t stream) {
+  const PagedKv& c = p.c;
+  CUtensorMap km, vm;
+  const int box_keys = c.page_size < kTileKeys ? c.page_size : kTileKeys;
+  const cuuint64_t dims[4] = {(cuuint64_t)c.dim, (cuuint64_t)c.page_size, (cuuint64_t)c.hkv, (cuuint64_t)c.num_pages};
+  auto bytes = [&](int64_t stride, int n) { return (cuuint64_t)(n > 1 ? stride * 2 : c.dim * 2); };
+  const cuuint64_t strides[3] = {bytes(c.slot_stride, c.page_size), bytes(c.head_stride, c.hkv),
+                                 bytes(c.page_stride, c.num_pages)};
+  const cuuint32_t box[4] = {64, (cuuint32_t)box_keys, 1, 1};
+  wr_status_t st = encode_map(&km, c.k, 4, dims, strides, box);
+  if (st == WR_OK) st = encode_map(&vm, c.v, 4, dims, strides, box);
+  if (st != WR_OK) return st;
+  PrefixArgs x{};
+  x.a = a;
+  x.pairs = (int)(((int64_t)a.T * a.group + row_tile - 1) / row_tile);
+  x.us = (a.prefix + kTileKeys - 1) / kTileKeys;
+  x.sp.units = (int64_t)a.hkv * x.pairs * x.us;
+  x.sp.ranges = grid < x.sp.units ? grid : x.sp.units;
+  x.box = box_keys;
+  cudaError_t e;
+  const int g = (int)x.sp.ranges;
+  if (c.dim == 64)
+    e = row_tile == 128 ? launch_tiles<64, 1>(km, vm, x, g, stream) : launch_tiles<64, 2>(km, vm, x, g, stream);
+  else
+    e = row_tile == 128 ? launch_tiles<128, 1>(km, vm, x, g, stream) : launch_tiles<128, 2>(km, vm, x, g, stream);
+  return e == cudaSuccess ? WR_OK : cuda_fail(e, "shared_prefix_attention (prefix tiles) launch");
+}
+
+}  // namespace wr

@@ -61,6 +61,7 @@
 #include "wr_common.cuh"
 #include "wr_internal.h"
 #include "wr_router.cuh"
+#include "wr_tcgen05.cuh"
 
 namespace wr {
 namespace {
@@ -157,130 +158,6 @@ __host__ __device__ inline TileCost tile_cost_of(int cnt, int nt, int nmax, int 
   d.wlast = nt > 0 ? chunk_cost<kGU>(np - (nt - 1) * nmax, nmax) : 0;
   d.r = nt > 0 ? (int64_t)kc * ((int64_t)(nt - 1) * d.wfull + d.wlast) : 0;
   return d;
-}
-
-// ---------------------------------------------------------------------------
-// tcgen05 / TMA wrappers
-// ---------------------------------------------------------------------------
-
-// Shared-memory matrix descriptor for a K-major bf16 tile written by TMA with
-// 128-byte swizzling: rows of 128 bytes, 8-row groups 1024 bytes apart (SBO),
-// descriptor version 1, layout type 2 (128-byte swizzle).  The tile base must
-// be 1024-byte aligned; stepping along K inside the 128-byte row adds the
-// byte offset to the start address.
-WR_DEVINL uint64_t sw128_desc(uint32_t saddr) {
-  return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) |
-         ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
-}
-
-// Instruction descriptor of kind::f16: bf16 A and B, fp32 accumulator, both
-// K-major, M = m (64 or 128), N = n (multiple of 16, 16..256).
-WR_DEVINL uint32_t idesc_bf16(int m, int n) {
-  return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) |
-         ((uint32_t)(m >> 4) << 24);
-}
-
-WR_DEVINL void umma_bf16(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
-                         uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-      ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
-      : "memory");
-}
-
-// Arrives once on `bar` when every tcgen05 operation this thread issued so
-// far has completed.
-WR_DEVINL void umma_commit(uint64_t* bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
-                   smem_u32(bar))
-               : "memory");
-}
-
-WR_DEVINL void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-WR_DEVINL void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-
-WR_DEVINL void tmem_alloc(uint32_t* slot, uint32_t cols) {
-  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
-                   smem_u32(slot)),
-               "r"(cols)
-               : "memory");
-}
-WR_DEVINL void tmem_relinquish() {
-  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-}
-WR_DEVINL void tmem_dealloc(uint32_t taddr, uint32_t cols) {
-  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(cols)
-               : "memory");
-}
-
-// 16 consecutive fp32 columns of this warp's 32 TMEM lanes (one per thread).
-WR_DEVINL void tmem_ld16(uint32_t taddr, uint32_t (&v)[16]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]),
-        "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]),
-        "=r"(v[14]), "=r"(v[15])
-      : "r"(taddr)
-      : "memory");
-}
-// Waits for this thread's tcgen05.ld results; the registers are threaded
-// through the asm so no use of them can be scheduled before the wait.
-WR_DEVINL void tmem_wait_ld(uint32_t (&v)[16]) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;"
-               : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]),
-                 "+r"(v[6]), "+r"(v[7]), "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]),
-                 "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15])
-               :
-               : "memory");
-}
-WR_DEVINL void reg_dep16(uint32_t (&v)[16]) {
-  asm volatile(""
-               : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]),
-                 "+r"(v[6]), "+r"(v[7]), "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]),
-                 "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15])
-               :
-               : "memory");
-}
-
-// Tiled TMA loads (no multicast) into this CTA's shared memory, completion
-// counted in bytes on `bar`.  The innermost coordinate is always a multiple
-// of 64 bf16 elements (128 bytes).
-WR_DEVINL void tma_load_2d(void* dst, const CUtensorMap* map, int c0, int c1, uint64_t* bar,
-                           uint64_t policy) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
-      ".L2::cache_hint [%0], [%1, {%2, %3}], [%4], %5;" ::"r"(smem_u32(dst)),
-      "l"(map), "r"(c0), "r"(c1), "r"(smem_u32(bar)), "l"(policy)
-      : "memory");
-}
-WR_DEVINL void tma_load_3d(void* dst, const CUtensorMap* map, int c0, int c1, int c2,
-                           uint64_t* bar, uint64_t policy) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
-      ".L2::cache_hint [%0], [%1, {%2, %3, %4}], [%5], %6;" ::"r"(smem_u32(dst)),
-      "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(smem_u32(bar)), "l"(policy)
-      : "memory");
-}
-// Named barrier `id` over `n` threads that also ORs `v` across them: every
-// participant gets the same answer, so a decision taken on it is uniform.
-WR_DEVINL bool named_bar_or(int id, int n, bool v) {
-  uint32_t r;
-  asm volatile(
-      "{\n\t.reg .pred pi, po;\n\t"
-      "setp.ne.u32 pi, %1, 0;\n\t"
-      "bar.red.or.pred po, %2, %3, pi;\n\t"
-      "selp.u32 %0, 1, 0, po;\n\t}"
-      : "=r"(r)
-      : "r"((uint32_t)v), "r"(id), "r"(n)
-      : "memory");
-  return r != 0;
-}
-
-WR_DEVINL void prefetch_tmap(const CUtensorMap* map) {
-  asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
 }
 
 // ---------------------------------------------------------------------------
@@ -1984,42 +1861,6 @@ __global__ void __launch_bounds__(kGemmThreadsF, 1)
 // ---------------------------------------------------------------------------
 // Host side
 // ---------------------------------------------------------------------------
-
-using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
-                                   const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
-                                   const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                   CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-wr_status_t get_encoder(EncodeTiledFn* out) {
-  static std::once_flag once;
-  static void* fn = nullptr;
-  static cudaError_t err = cudaSuccess;
-  std::call_once(once, [] {
-    cudaDriverEntryPointQueryResult q = cudaDriverEntryPointSymbolNotFound;
-    err = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q);
-    if (err == cudaSuccess && q != cudaDriverEntryPointSuccess) fn = nullptr;
-  });
-  if (err != cudaSuccess) return cuda_fail(err, "cudaGetDriverEntryPoint(cuTensorMapEncodeTiled)");
-  if (!fn) return fail(WR_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
-  *out = reinterpret_cast<EncodeTiledFn>(fn);
-  return WR_OK;
-}
-
-// bf16 tensor map with 128-byte swizzling, zero fill outside the tensor.
-wr_status_t encode_map(CUtensorMap* m, const void* base, int rank, const cuuint64_t* dims,
-                       const cuuint64_t* strides_bytes, const cuuint32_t* box,
-                       CUtensorMapDataType dtype = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16) {
-  EncodeTiledFn enc;
-  wr_status_t st = get_encoder(&enc);
-  if (st != WR_OK) return st;
-  cuuint32_t estr[3] = {1, 1, 1};
-  CUresult r = enc(m, dtype, (cuuint32_t)rank, const_cast<void*>(base),
-                   dims, strides_bytes, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) return fail(WR_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
-  return WR_OK;
-}
 
 // Token maps with boxes of 16, 32, .. rows.  Heights above the largest tile
 // (nmax, and never above the rows a tile can start in) are never used and
