@@ -9,14 +9,18 @@
 //
 // A CTA has one SM and NT tiles of 128 rows (NT 2 when there are that many:
 // while one tile's softmax runs, the tensor core works on the other).  Per
-// 128 keys: S = Q K^T into TMEM; a thread reads its row of S (lane = row, so
+// 64 keys: S = Q K^T into TMEM; a thread reads its row of S (lane = row, so
 // no exchange between threads), takes the running maximum and the weights
 // 2^(s - m), which go back over S as bf16, the A operand of O += P V, whose
-// sum stays in TMEM for all of a piece's keys.  m follows the true maximum
+// sum stays in TMEM for all of a piece's keys.  S has two buffers of 64
+// columns a tile (with O of both tiles TMEM is full), so the next scores are
+// there when a softmax ends; with one of 128 columns, whose P has to be
+// consumed before the next S, softmax and products of a tile took turns
+// (145 us for 1536 rows and 16384 keys of 8 heads).  m follows the true maximum
 // only when it has grown by more than 8 (a factor of 256, harmless in fp32
 // sums and bf16 weights), so O is rescaled rarely.  Warp 4 * NT brings K and V
-// by TMA, a copy a page and 64 columns, into two rings; the next warp issues
-// the MMAs.  Keys in pages outside the cache, and those behind the prefix's
+// by TMA, a copy a page and 64 columns, into two rings; the warps behind it
+// issue the MMAs, one for each tile.  Keys in pages outside the cache, and those behind the prefix's
 // end in its last page, are masked in S and their rows of V set to zero.
 //
 // The (key head, row tiles, 128 keys) units are dealt to the CTAs in ranges of
@@ -32,6 +36,7 @@ namespace {
 
 constexpr int kTileKeys = kPrefixUnit;
 constexpr int kTileRows = 128;
+constexpr int kHalf = 64;  // keys of one S buffer
 constexpr int kMaskRing = 8;
 constexpr float kRescale = 8.f;
 #define WR_NEG_INF (-__int_as_float(0x7f800000))
@@ -44,7 +49,7 @@ struct Cfg {
   static constexpr int kPanelBytes = 128 * 128;  // 128 rows of 64 columns
   static constexpr int kTileBytes = kPanels * kPanelBytes;
   static constexpr int kSmem = 1024 + NT * kTileBytes + 2 * kStages * kTileBytes;
-  static constexpr int kThreads = NT * 128 + 64;
+  static constexpr int kThreads = NT * 128 + 32 + NT * 32;
   static constexpr uint32_t kTmemCols = NT == 2 ? 512 : 256;
 };
 
@@ -60,6 +65,14 @@ WR_DEVINL float ex2p(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
+}
+
+// mbar_wait for waits on the critical path: the clock is read only after many
+// tries, each of which the hardware suspends for a while.
+WR_DEVINL bool wait_quick(uint64_t* bar, uint32_t parity, const volatile int* abort) {
+  for (uint32_t it = 0; it < 64; ++it)
+    if (mbar_try_wait(bar, parity)) return true;
+  return mbar_wait(bar, parity, abort);
 }
 
 // A CTA's pieces in order: the units of one (key head, row tiles) in its range.
@@ -84,7 +97,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1)
   constexpr int S = C::kStages, MR = NT * kTileRows;
   extern __shared__ uint8_t s_raw[];
   __shared__ uint64_t k_full[S], k_empty[S], v_full[S], v_empty[S], aux;
-  __shared__ uint64_t q_full[NT], s_full[NT], p_full[NT], pv_done[NT];
+  __shared__ uint64_t q_full[NT], s_full[NT][2], p_full[NT][2], pv_done[NT][2], drain[NT];
   __shared__ uint32_t s_mask[kMaskRing][4], s_special[kMaskRing], s_tmem;
   __shared__ int s_abort;
   const AttnArgs& a = p.a;
@@ -99,15 +112,18 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1)
   if (tid == 0) {
     for (int i = 0; i < S; ++i) {
       mbar_init(&k_full[i], 1);
-      mbar_init(&k_empty[i], 1);
+      mbar_init(&k_empty[i], NT);
       mbar_init(&v_full[i], 1);
-      mbar_init(&v_empty[i], 1);
+      mbar_init(&v_empty[i], NT);
     }
     for (int t = 0; t < NT; ++t) {
       mbar_init(&q_full[t], kTileRows);
-      mbar_init(&s_full[t], 1);
-      mbar_init(&p_full[t], kTileRows);
-      mbar_init(&pv_done[t], 1);
+      for (int b = 0; b < 2; ++b) {
+        mbar_init(&s_full[t][b], 1);
+        mbar_init(&p_full[t][b], kTileRows);
+        mbar_init(&pv_done[t][b], 1);
+      }
+      mbar_init(&drain[t], 1);
     }
     mbar_init(&aux, 1);
     s_abort = 0;
@@ -211,69 +227,70 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1)
       mbar_wait(*abort ? &k_full[i % S] : &k_empty[i % S], (i / S) & 1, nullptr);
     for (int i = max(0, issued_v - S); i < issued_v; ++i)
       mbar_wait(*abort ? &v_full[i % S] : &v_empty[i % S], (i / S) & 1, nullptr);
-  } else if (warp == NT * 4 + 1) {
-    // ---- the MMAs ---------------------------------------------------------
+  } else if (warp > NT * 4) {
+    // ---- the MMAs of one tile ---------------------------------------------
+    // A warp for each tile: what one tile waits for does not hold up the other.
+    // S(i) needs K and, since P(i - 2) lies in its columns, the end of
+    // PV(i - 2); PV(i) needs P(i) and V.
+    const int t = warp - NT * 4 - 1;
     if (lane == 0) {
-      const uint32_t id_qk = idesc_bf16(kTileRows, kTileKeys);
+      const uint32_t id_qk = idesc_bf16(kTileRows, kHalf);
       const uint32_t id_pv = idesc_bf16(kTileRows, D) | kIdescBMajorMn;
-      auto qk = [&](int t, int it) {  // S_t = Q_t K^T
-        const uint32_t qa = smem_u32(qbuf + t * C::kTileBytes), ka = smem_u32(kbuf + (it % S) * C::kTileBytes);
-#pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-          const uint32_t off = (k >> 2) * C::kPanelBytes + (k & 3) * 32;
-          umma_bf16(tmem_s + t * kTileKeys, sw128_desc(qa + off), sw128_desc(ka + off), id_qk, k > 0);
-        }
-        if (t == NT - 1) umma_commit(&k_empty[it % S]);
-        umma_commit(&s_full[t]);
-      };
-      auto pv = [&](int t, int it, bool more) {  // O_t (+)= P_t V
-        const uint32_t va = smem_u32(vbuf + (it % S) * C::kTileBytes);
-#pragma unroll
-        for (int k = 0; k < kTileKeys / 16; ++k)
-          umma_bf16_ta(tmem_o + t * D, tmem_s + t * kTileKeys + k * 8,
-                       sw128_desc_mn(va + k * 2048, C::kPanelBytes), id_pv, more || k > 0);
-        if (t == NT - 1) umma_commit(&v_empty[it % S]);
-        umma_commit(&pv_done[t]);
-      };
+      const uint64_t qd = sw128_desc(smem_u32(qbuf + t * C::kTileBytes));
+      const uint64_t kd = sw128_desc(smem_u32(kbuf)), vd = sw128_desc_mn(smem_u32(vbuf), C::kPanelBytes);
+      const uint32_t st = tmem_s + t * 2 * kHalf, ot = tmem_o + t * D;
       bool dead = false;
       auto wait = [&](uint64_t* bar, uint32_t parity) {
-        if (!dead && !mbar_wait(bar, parity, abort)) {
+        if (!dead && !wait_quick(bar, parity, abort)) {
           *abort = 1;
           dead = true;
         }
         return !dead;
       };
+      // i: half tiles of this CTA, both halves of 128 keys in one stage.
+      auto qk = [&](int i) {  // S = Q K^T
+        const int it = i >> 1, stage = it % S, b = i & 1;
+        if (!wait(&k_full[stage], (it / S) & 1) || (i >= 2 && !wait(&pv_done[t][b], ((i >> 1) - 1) & 1))) return;
+        tc_fence_after();
+        const uint64_t kk = kd + ((uint64_t)(stage * C::kTileBytes + b * kHalf * 128) >> 4);
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+          const uint64_t ko = ((k >> 2) * C::kPanelBytes + (k & 3) * 32) >> 4;
+          umma_bf16(st + b * kHalf, qd + ko, kk + ko, id_qk, k > 0);
+        }
+        umma_commit(&s_full[t][b]);
+        if (b == 1) umma_commit(&k_empty[stage]);
+      };
+      auto pv = [&](int i, bool more) {  // O (+)= P V
+        const int it = i >> 1, stage = it % S, b = i & 1;
+        if (!wait(&v_full[stage], (it / S) & 1) || !wait(&p_full[t][b], (i >> 1) & 1)) return;
+        tc_fence_after();
+        const uint64_t vv = vd + ((uint64_t)(stage * C::kTileBytes + b * kHalf * 128) >> 4);
+#pragma unroll
+        for (int k = 0; k < kHalf / 16; ++k)
+          umma_bf16_ta(ot, st + b * kHalf + k * 8, vv + (k * 2048 >> 4), id_pv, more || k > 0);
+        umma_commit(&pv_done[t][b]);
+        if (b == 1) umma_commit(&v_empty[stage]);
+      };
       int64_t unit = u0;
-      int it = 0, piece = 0;
-      while (it < total && !dead) {
+      int first = 0, piece = 0;
+      while (first < 2 * total && !dead) {
         const Piece pc = piece_at(p, unit, u1);
-        for (int t = 0; t < NT; ++t) wait(&q_full[t], piece & 1);
-        wait(&k_full[it % S], (it / S) & 1);
-        for (int t = 0; t < NT && !dead; ++t) {
-          if (it > 0 && !wait(&pv_done[t], (it - 1) & 1)) break;
-          tc_fence_after();
-          qk(t, it);
+        const int end = first + 2 * pc.n;
+        if (!wait(&q_full[t], piece & 1)) break;
+        qk(first);
+        qk(first + 1);
+        for (int i = first; i < end && !dead; ++i) {
+          pv(i, i > first);
+          if (i + 2 < end && !dead) qk(i + 2);
         }
-        for (int i = 0; i < pc.n && !dead; ++i, ++it) {
-          for (int t = 0; t < NT && !dead; ++t) {
-            if (!wait(&p_full[t], it & 1) || !wait(&v_full[it % S], (it / S) & 1)) break;
-            tc_fence_after();
-            pv(t, it, i > 0);
-            if (i + 1 < pc.n) {
-              if (!wait(&k_full[(it + 1) % S], ((it + 1) / S) & 1) || !wait(&pv_done[t], it & 1)) break;
-              tc_fence_after();
-              qk(t, it + 1);
-            }
-          }
-        }
+        first = end;
         unit += pc.n;
         ++piece;
       }
       if (dead) {  // let what was issued end
-        umma_commit(&aux);
-        const uint64_t t0 = globaltimer_ns();
-        while (globaltimer_ns() - t0 < 1000000) {
-        }
+        umma_commit(&drain[t]);
+        mbar_wait(&drain[t], 0, nullptr);
       }
     }
     __syncwarp();
@@ -281,7 +298,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1)
     // ---- softmax: thread = row of tile t ----------------------------------
     const int t = warp >> 2, rl = tid & 127;
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // this warp's 32 TMEM lanes
-    const uint32_t ts = tmem_s + t * kTileKeys + lanes, to = tmem_o + t * D + lanes;
+    const uint32_t ts = tmem_s + t * 2 * kHalf + lanes, to = tmem_o + t * D + lanes;
     const float c = a.scale_log2;
     int64_t unit = u0;
     int it = 0;
@@ -304,39 +321,36 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1)
         mbar_arrive(&q_full[t]);
       }
       float m = WR_NEG_INF, l = 0.f;
-      for (int i = 0; i < pc.n && !dead; ++i, ++it) {
-        if (!mbar_wait(&s_full[t], it & 1, abort)) {
+      for (int i = 0; i < 2 * pc.n && !dead; ++i, ++it) {  // it: half tiles of this CTA
+        const int b = it & 1;
+        const uint32_t sb = ts + b * kHalf;
+        if (!wait_quick(&s_full[t][b], (it >> 1) & 1, abort)) {
           *abort = 1;
           dead = true;
           break;
         }
         tc_fence_after();
-        // Twice over S, 32 columns at a time: the whole row does not fit into
-        // registers beside the rest, and TMEM reads are cheap.
-        const bool special = s_special[it % kMaskRing];
-        auto mask = [&](uint32_t (&s)[32], int k) {
-          if (!special) return;
-          const uint32_t w = s_mask[it % kMaskRing][k];
-#pragma unroll
-          for (int j = 0; j < 32; ++j)
-            if (!((w >> j) & 1)) s[j] = 0xff800000u;
-        };
         uint32_t s[2][32];
+        tmem_ld32(sb, s[0]);
+        tmem_ld32(sb + 32, s[1]);
+        tmem_wait_lds();
+        reg_dep32(s[0]);
+        reg_dep32(s[1]);
+        const int slot = (it >> 1) % kMaskRing;
+        if (s_special[slot]) {
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const uint32_t w = s_mask[slot][2 * b + k];
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (!((w >> j) & 1)) s[k][j] = 0xff800000u;
+          }
+        }
         float mx[4] = {WR_NEG_INF, WR_NEG_INF, WR_NEG_INF, WR_NEG_INF};
 #pragma unroll
-        for (int k = 0; k < 4; k += 2) {
-          tmem_ld32(ts + k * 32, s[0]);
-          tmem_ld32(ts + k * 32 + 32, s[1]);
-          tmem_wait_lds();
-          reg_dep32(s[0]);
-          reg_dep32(s[1]);
-          mask(s[0], k);
-          mask(s[1], k + 1);
-#pragma unroll
-          for (int j = 0; j < 32; j += 2) {
-            mx[j & 2] = fmaxf(mx[j & 2], fmaxf(__uint_as_float(s[0][j]), __uint_as_float(s[0][j + 1])));
-            mx[1 + (j & 2)] = fmaxf(mx[1 + (j & 2)], fmaxf(__uint_as_float(s[1][j]), __uint_as_float(s[1][j + 1])));
-          }
+        for (int j = 0; j < 32; j += 2) {
+          mx[j & 2] = fmaxf(mx[j & 2], fmaxf(__uint_as_float(s[0][j]), __uint_as_float(s[0][j + 1])));
+          mx[1 + (j & 2)] = fmaxf(mx[1 + (j & 2)], fmaxf(__uint_as_float(s[1][j]), __uint_as_float(s[1][j + 1])));
         }
         const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c;
         if (i == 0) {
@@ -344,49 +358,49 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1)
         } else {
           const bool up = top > m + kRescale;
           if (__any_sync(0xffffffffu, up)) {
+            // O stands still once the last PV issued has ended.
+            if (!wait_quick(&pv_done[t][b ^ 1], ((it - 1) >> 1) & 1, abort)) {
+              *abort = 1;
+              dead = true;
+              break;
+            }
+            tc_fence_after();
             const float nm = up ? top : m;
             const float f = up ? ex2p(m - nm) : 1.f;
             m = nm;
             l *= f;
+#pragma unroll 1
+            for (int k = 0; k < D / 16; ++k) {
+              uint32_t o[16];
+              tmem_ld16(to + k * 16, o);
+              tmem_wait_ld(o);
 #pragma unroll
-            for (int k = 0; k < D / 32; ++k) {
-              uint32_t o[32];
-              tmem_ld32(to + k * 32, o);
-              tmem_wait_lds();
-              reg_dep32(o);
-#pragma unroll
-              for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
-              tmem_st32(to + k * 32, o);
+              for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
+              tmem_st16(to + k * 16, o);
             }
           }
         }
         const float base = m == WR_NEG_INF ? 0.f : m;
         float ls[4] = {0.f, 0.f, 0.f, 0.f};
-        tmem_ld32(ts, s[0]);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          tmem_wait_lds();
-          reg_dep32(s[k & 1]);
-          if (k < 3) tmem_ld32(ts + k * 32 + 32, s[(k + 1) & 1]);
-          mask(s[k & 1], k);
+        for (int k = 0; k < 2; ++k) {
           uint32_t w[16];
 #pragma unroll
           for (int j = 0; j < 16; ++j) {
-            const float x = ex2p(fmaf(__uint_as_float(s[k & 1][2 * j]), c, -base));
-            const float y = ex2p(fmaf(__uint_as_float(s[k & 1][2 * j + 1]), c, -base));
+            const float x = ex2p(fmaf(__uint_as_float(s[k][2 * j]), c, -base));
+            const float y = ex2p(fmaf(__uint_as_float(s[k][2 * j + 1]), c, -base));
             ls[j & 3] += x + y;
-            __nv_bfloat162 b = __floats2bfloat162_rn(x, y);
-            w[j] = *reinterpret_cast<uint32_t*>(&b);
+            __nv_bfloat162 v = __floats2bfloat162_rn(x, y);
+            w[j] = *reinterpret_cast<uint32_t*>(&v);
           }
-          // columns 16 k .. 16 k + 15, whose scores have been read
-          tmem_st16(ts + k * 16, w);
+          tmem_st16(sb + k * 16, w);  // over the scores, all of which are in registers
         }
         l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
         tmem_wait_st();
         tc_fence_before();
-        mbar_arrive(&p_full[t]);
+        mbar_arrive(&p_full[t][b]);
       }
-      if (!dead && !mbar_wait(&pv_done[t], (it - 1) & 1, abort)) {
+      if (!dead && !wait_quick(&pv_done[t][(it - 1) & 1], ((it - 1) >> 1) & 1, abort)) {
         *abort = 1;
         dead = true;
       }
@@ -397,7 +411,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1)
       float* op = whole ? a.home + orow * D : a.part.piece + prow * D;
       if (!dead) {
         tc_fence_after();
-#pragma unroll
+#pragma unroll 1
         for (int k = 0; k < D / 32; ++k) {
           uint32_t o[32];
           tmem_ld32(to + k * 32, o);
