@@ -67,12 +67,27 @@ WR_DEVINL float ex2p(float x) {
   return r;
 }
 
-// mbar_wait for waits on the critical path: the clock is read only after many
-// tries, each of which the hardware suspends for a while.
-WR_DEVINL bool wait_quick(uint64_t* bar, uint32_t parity, const volatile int* abort) {
-  for (uint32_t it = 0; it < 64; ++it)
-    if (mbar_try_wait(bar, parity)) return true;
-  return mbar_wait(bar, parity, abort);
+// A wait on the critical path, of a converged warp: few instructions (the MMA
+// warps spend their time on them), each try suspended by the hardware for up
+// to 10 ms and 200 of them at most, which is the bound of 2 s.  False: it gave
+// up.
+WR_DEVINL bool wait_lean(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred P;\n\t.reg .u32 n;\n\t"
+      "mov.u32 n, 200;\n\t"
+      "WAIT_%=:\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 P, [%1], %2, 10000000;\n\t"
+      "@P bra DONE_%=;\n\t"
+      "sub.u32 n, n, 1;\n\t"
+      "setp.ne.u32 P, n, 0;\n\t"
+      "@P bra WAIT_%=;\n\t"
+      "DONE_%=:\n\t"
+      "min.u32 %0, n, 1;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
 }
 
 // A CTA's pieces in order: the units of one (key head, row tiles) in its range.
@@ -97,7 +112,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1)
   constexpr int S = C::kStages, MR = NT * kTileRows;
   extern __shared__ uint8_t s_raw[];
   __shared__ uint64_t k_full[S], k_empty[S], v_full[S], v_empty[S], aux;
-  __shared__ uint64_t q_full[NT], s_full[NT][2], p_full[NT][2], pv_done[NT][2], drain[NT];
+  __shared__ uint64_t q_full[NT], s_full[NT][2], p_full[NT][2], pv_done[NT][2], turn[NT], drain[NT];
   __shared__ uint32_t s_mask[kMaskRing][4], s_special[kMaskRing], s_tmem;
   __shared__ int s_abort;
   const AttnArgs& a = p.a;
@@ -124,6 +139,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1)
         mbar_init(&pv_done[t][b], 1);
       }
       mbar_init(&drain[t], 1);
+      mbar_init(&turn[t], 4);
     }
     mbar_init(&aux, 1);
     s_abort = 0;
@@ -232,68 +248,71 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1)
     // A warp for each tile: what one tile waits for does not hold up the other.
     // S(i) needs K and, since P(i - 2) lies in its columns, the end of
     // PV(i - 2); PV(i) needs P(i) and V.
-    const int t = warp - NT * 4 - 1;
-    if (lane == 0) {
-      const uint32_t id_qk = idesc_bf16(kTileRows, kHalf);
-      const uint32_t id_pv = idesc_bf16(kTileRows, D) | kIdescBMajorMn;
-      const uint64_t qd = sw128_desc(smem_u32(qbuf + t * C::kTileBytes));
-      const uint64_t kd = sw128_desc(smem_u32(kbuf)), vd = sw128_desc_mn(smem_u32(vbuf), C::kPanelBytes);
-      const uint32_t st = tmem_s + t * 2 * kHalf, ot = tmem_o + t * D;
-      bool dead = false;
-      auto wait = [&](uint64_t* bar, uint32_t parity) {
-        if (!dead && !wait_quick(bar, parity, abort)) {
-          *abort = 1;
-          dead = true;
-        }
-        return !dead;
-      };
-      // i: half tiles of this CTA, both halves of 128 keys in one stage.
-      auto qk = [&](int i) {  // S = Q K^T
-        const int it = i >> 1, stage = it % S, b = i & 1;
-        if (!wait(&k_full[stage], (it / S) & 1) || (i >= 2 && !wait(&pv_done[t][b], ((i >> 1) - 1) & 1))) return;
-        tc_fence_after();
-        const uint64_t kk = kd + ((uint64_t)(stage * C::kTileBytes + b * kHalf * 128) >> 4);
+    // The whole warp walks through the loop and one elected lane issues: the
+    // descriptors then stay in uniform registers, where the MMAs want them
+    // (in a branch of one lane each takes a detour of some 70 cycles).
+    const int t = __shfl_sync(0xffffffffu, warp, 0) - NT * 4 - 1;
+    const uint32_t id_qk = idesc_bf16(kTileRows, kHalf);
+    const uint32_t id_pv = idesc_bf16(kTileRows, D) | kIdescBMajorMn;
+    const uint64_t qd = sw128_desc(smem_u32(qbuf + t * C::kTileBytes));
+    const uint64_t kd = sw128_desc(smem_u32(kbuf)), vd = sw128_desc_mn(smem_u32(vbuf), C::kPanelBytes);
+    const uint32_t st = tmem_s + t * 2 * kHalf, ot = tmem_o + t * D;
+    bool dead = false;
+    auto wait = [&](uint64_t* bar, uint32_t parity) { dead |= !wait_lean(bar, parity); };
+    int64_t unit = u0;
+    int first = 0, piece = 0;
+    while (first < 2 * total && !dead) {
+      const Piece pc = piece_at(p, unit, u1);
+      const int end = first + 2 * pc.n;
+      wait(&q_full[t], piece & 1);
+      // Half tiles of this CTA, two in a stage: PV(j - 2), then S(j).
+      for (int j = first; j < end + 2 && !dead; ++j) {
+        const int b = j & 1;
+        if (j >= first + 2) {  // O (+)= P V
+          const int i = j - 2, it = i >> 1, stage = it % S;
+          if (b == 0) wait(&v_full[stage], (it / S) & 1);
+          wait(&p_full[t][b], it & 1);
+          if (dead) break;
+          tc_fence_after();
+          const uint64_t vv = vd + ((uint64_t)(stage * C::kTileBytes + b * kHalf * 128) >> 4);
+          if (elect_one()) {
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-          const uint64_t ko = ((k >> 2) * C::kPanelBytes + (k & 3) * 32) >> 4;
-          umma_bf16(st + b * kHalf, qd + ko, kk + ko, id_qk, k > 0);
+            for (int k = 0; k < kHalf / 16; ++k)
+              umma_bf16_ta(ot, st + b * kHalf + k * 8, vv + (k * 2048 >> 4), id_pv, i > first || k > 0);
+            umma_commit(&pv_done[t][b]);
+            if (b == 1) umma_commit(&v_empty[stage]);
+          }
+          __syncwarp();
         }
-        umma_commit(&s_full[t][b]);
-        if (b == 1) umma_commit(&k_empty[stage]);
-      };
-      auto pv = [&](int i, bool more) {  // O (+)= P V
-        const int it = i >> 1, stage = it % S, b = i & 1;
-        if (!wait(&v_full[stage], (it / S) & 1) || !wait(&p_full[t][b], (i >> 1) & 1)) return;
-        tc_fence_after();
-        const uint64_t vv = vd + ((uint64_t)(stage * C::kTileBytes + b * kHalf * 128) >> 4);
+        if (j < end) {  // S = Q K^T
+          const int it = j >> 1, stage = it % S;
+          if (b == 0) wait(&k_full[stage], (it / S) & 1);
+          if (j >= 2) wait(&pv_done[t][b], (it - 1) & 1);
+          if (dead) break;
+          tc_fence_after();
+          const uint64_t kk = kd + ((uint64_t)(stage * C::kTileBytes + b * kHalf * 128) >> 4);
+          if (elect_one()) {
 #pragma unroll
-        for (int k = 0; k < kHalf / 16; ++k)
-          umma_bf16_ta(ot, st + b * kHalf + k * 8, vv + (k * 2048 >> 4), id_pv, more || k > 0);
-        umma_commit(&pv_done[t][b]);
-        if (b == 1) umma_commit(&v_empty[stage]);
-      };
-      int64_t unit = u0;
-      int first = 0, piece = 0;
-      while (first < 2 * total && !dead) {
-        const Piece pc = piece_at(p, unit, u1);
-        const int end = first + 2 * pc.n;
-        if (!wait(&q_full[t], piece & 1)) break;
-        qk(first);
-        qk(first + 1);
-        for (int i = first; i < end && !dead; ++i) {
-          pv(i, i > first);
-          if (i + 2 < end && !dead) qk(i + 2);
+            for (int k = 0; k < D / 16; ++k) {
+              const uint64_t ko = ((k >> 2) * C::kPanelBytes + (k & 3) * 32) >> 4;
+              umma_bf16(st + b * kHalf, qd + ko, kk + ko, id_qk, k > 0);
+            }
+            umma_commit(&s_full[t][b]);
+            if (b == 1) umma_commit(&k_empty[stage]);
+          }
+          __syncwarp();
         }
-        first = end;
-        unit += pc.n;
-        ++piece;
       }
-      if (dead) {  // let what was issued end
-        umma_commit(&drain[t]);
-        mbar_wait(&drain[t], 0, nullptr);
-      }
+      first = end;
+      unit += pc.n;
+      ++piece;
     }
-    __syncwarp();
+    if (dead) {  // let what was issued end
+      *abort = 1;
+      if (elect_one()) umma_commit(&drain[t]);
+      __syncwarp();
+      mbar_wait(&drain[t], 0, nullptr);
+    }
   } else {
     // ---- softmax: thread = row of tile t ----------------------------------
     const int t = warp >> 2, rl = tid & 127;
@@ -324,7 +343,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1)
       for (int i = 0; i < 2 * pc.n && !dead; ++i, ++it) {  // it: half tiles of this CTA
         const int b = it & 1;
         const uint32_t sb = ts + b * kHalf;
-        if (!wait_quick(&s_full[t][b], (it >> 1) & 1, abort)) {
+        if (!wait_lean(&s_full[t][b], (it >> 1) & 1)) {
           *abort = 1;
           dead = true;
           break;
@@ -359,7 +378,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1)
           const bool up = top > m + kRescale;
           if (__any_sync(0xffffffffu, up)) {
             // O stands still once the last PV issued has ended.
-            if (!wait_quick(&pv_done[t][b ^ 1], ((it - 1) >> 1) & 1, abort)) {
+            if (!wait_lean(&pv_done[t][b ^ 1], ((it - 1) >> 1) & 1)) {
               *abort = 1;
               dead = true;
               break;
@@ -382,6 +401,13 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1)
         }
         const float base = m == WR_NEG_INF ? 0.f : m;
         float ls[4] = {0.f, 0.f, 0.f, 0.f};
+        // The tiles' exponentials take turns: side by side both tiles wait for
+        // the SFUs, then both for the rest, and the SFUs for them.
+        if (NT == 2 && (t == 1 || it > 0) && !wait_lean(&turn[t], (t == 1 ? it : it - 1) & 1)) {
+          *abort = 1;
+          dead = true;
+          break;
+        }
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           uint32_t w[16];
@@ -394,13 +420,14 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1)
             w[j] = *reinterpret_cast<uint32_t*>(&v);
           }
           tmem_st16(sb + k * 16, w);  // over the scores, all of which are in registers
+          if (NT == 2 && k == 0 && lane == 0) mbar_arrive(&turn[t ^ 1]);
         }
         l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
         tmem_wait_st();
         tc_fence_before();
         mbar_arrive(&p_full[t][b]);
       }
-      if (!dead && !wait_quick(&pv_done[t][(it - 1) & 1], ((it - 1) >> 1) & 1, abort)) {
+      if (!dead && !wait_lean(&pv_done[t][(it - 1) & 1], ((it - 1) >> 1) & 1)) {
         *abort = 1;
         dead = true;
       }

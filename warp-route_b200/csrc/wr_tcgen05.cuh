@@ -66,6 +66,17 @@ WR_DEVINL uint64_t sw128_desc_mn(uint32_t saddr, uint32_t panel) {
 }
 constexpr uint32_t kIdescBMajorMn = 1u << 16;  // B is MN-major
 
+// True in one lane of a converged warp.
+WR_DEVINL bool elect_one() {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(r));
+  return r != 0;
+}
+
 // Arrives once on `bar` when every tcgen05 operation this thread issued so
 // far has completed.
 WR_DEVINL void umma_commit(uint64_t* bar) {
