@@ -49,7 +49,7 @@ struct Cfg {
   static constexpr int kPanelBytes = 128 * 128;  // 128 rows of 64 columns
   static constexpr int kTileBytes = kPanels * kPanelBytes;
   static constexpr int kSmem = 1024 + NT * kTileBytes + 2 * kStages * kTileBytes;
-  static constexpr int kThreads = NT * 128 + 32 + NT * 32;
+  static constexpr int kThreads = NT * 128 + 32 + NT * 64;
   static constexpr uint32_t kTmemCols = NT == 2 ? 512 : 256;
 };
 
@@ -112,7 +112,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1)
   constexpr int S = C::kStages, MR = NT * kTileRows;
   extern __shared__ uint8_t s_raw[];
   __shared__ uint64_t k_full[S], k_empty[S], v_full[S], v_empty[S], aux;
-  __shared__ uint64_t q_full[NT], s_full[NT][2], p_full[NT][2], pv_done[NT][2], turn[NT], drain[NT];
+  __shared__ uint64_t q_full[NT], s_full[NT][2], p_full[NT][2], pv_done[NT][2], turn[NT], drain[2 * NT];
   __shared__ uint32_t s_mask[kMaskRing][4], s_special[kMaskRing], s_tmem;
   __shared__ int s_abort;
   const AttnArgs& a = p.a;
@@ -139,6 +139,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1)
         mbar_init(&pv_done[t][b], 1);
       }
       mbar_init(&drain[t], 1);
+      mbar_init(&drain[NT + t], 1);
       mbar_init(&turn[t], 4);
     }
     mbar_init(&aux, 1);
@@ -244,74 +245,76 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1)
     for (int i = max(0, issued_v - S); i < issued_v; ++i)
       mbar_wait(*abort ? &v_full[i % S] : &v_empty[i % S], (i / S) & 1, nullptr);
   } else if (warp > NT * 4) {
-    // ---- the MMAs of one tile ---------------------------------------------
-    // A warp for each tile: what one tile waits for does not hold up the other.
-    // S(i) needs K and, since P(i - 2) lies in its columns, the end of
-    // PV(i - 2); PV(i) needs P(i) and V.
-    // The whole warp walks through the loop and one elected lane issues: the
-    // descriptors then stay in uniform registers, where the MMAs want them
-    // (in a branch of one lane each takes a detour of some 70 cycles).
-    const int t = __shfl_sync(0xffffffffu, warp, 0) - NT * 4 - 1;
-    const uint32_t id_qk = idesc_bf16(kTileRows, kHalf);
-    const uint32_t id_pv = idesc_bf16(kTileRows, D) | kIdescBMajorMn;
-    const uint64_t qd = sw128_desc(smem_u32(qbuf + t * C::kTileBytes));
-    const uint64_t kd = sw128_desc(smem_u32(kbuf)), vd = sw128_desc_mn(smem_u32(vbuf), C::kPanelBytes);
-    const uint32_t st = tmem_s + t * 2 * kHalf, ot = tmem_o + t * D;
+    // ---- the MMAs ---------------------------------------------------------
+    // A warp for each tile's scores and one for its sums: what one waits for
+    // does not hold up the other.  S(j) needs K and, since P(j - 2) lies in its
+    // columns, the end of PV(j - 2); PV(j) needs P(j) and V.  (j: half tiles of
+    // this CTA, two in a stage.)  The whole warp walks through the loop and one
+    // elected lane issues: the descriptors then stay in uniform registers,
+    // where the MMAs want them (in a branch of one lane each takes a detour of
+    // some 70 cycles).
+    const int which = __shfl_sync(0xffffffffu, warp, 0) - NT * 4 - 1;
+    const int t = which % NT;
+    const uint32_t st = tmem_s + t * 2 * kHalf;
     bool dead = false;
     auto wait = [&](uint64_t* bar, uint32_t parity) { dead |= !wait_lean(bar, parity); };
     int64_t unit = u0;
-    int first = 0, piece = 0;
-    while (first < 2 * total && !dead) {
-      const Piece pc = piece_at(p, unit, u1);
-      const int end = first + 2 * pc.n;
-      wait(&q_full[t], piece & 1);
-      // Half tiles of this CTA, two in a stage: PV(j - 2), then S(j).
-      for (int j = first; j < end + 2 && !dead; ++j) {
-        const int b = j & 1;
-        if (j >= first + 2) {  // O (+)= P V
-          const int i = j - 2, it = i >> 1, stage = it % S;
-          if (b == 0) wait(&v_full[stage], (it / S) & 1);
-          wait(&p_full[t][b], it & 1);
-          if (dead) break;
-          tc_fence_after();
-          const uint64_t vv = vd + ((uint64_t)(stage * C::kTileBytes + b * kHalf * 128) >> 4);
-          if (elect_one()) {
-#pragma unroll
-            for (int k = 0; k < kHalf / 16; ++k)
-              umma_bf16_ta(ot, st + b * kHalf + k * 8, vv + (k * 2048 >> 4), id_pv, i > first || k > 0);
-            umma_commit(&pv_done[t][b]);
-            if (b == 1) umma_commit(&v_empty[stage]);
-          }
-          __syncwarp();
-        }
-        if (j < end) {  // S = Q K^T
-          const int it = j >> 1, stage = it % S;
+    int j = 0, piece = 0;
+    if (which < NT) {  // S = Q K^T
+      const uint32_t idesc = idesc_bf16(kTileRows, kHalf);
+      const uint64_t qd = sw128_desc(smem_u32(qbuf + t * C::kTileBytes)), kd = sw128_desc(smem_u32(kbuf));
+      while (j < 2 * total && !dead) {
+        const Piece pc = piece_at(p, unit, u1);
+        wait(&q_full[t], piece & 1);
+        for (const int end = j + 2 * pc.n; j < end && !dead; ++j) {
+          const int b = j & 1, it = j >> 1, stage = it % S;
           if (b == 0) wait(&k_full[stage], (it / S) & 1);
           if (j >= 2) wait(&pv_done[t][b], (it - 1) & 1);
-          if (dead) break;
           tc_fence_after();
           const uint64_t kk = kd + ((uint64_t)(stage * C::kTileBytes + b * kHalf * 128) >> 4);
-          if (elect_one()) {
+          if (elect_one() && !dead) {
 #pragma unroll
             for (int k = 0; k < D / 16; ++k) {
               const uint64_t ko = ((k >> 2) * C::kPanelBytes + (k & 3) * 32) >> 4;
-              umma_bf16(st + b * kHalf, qd + ko, kk + ko, id_qk, k > 0);
+              umma_bf16(st + b * kHalf, qd + ko, kk + ko, idesc, k > 0);
             }
             umma_commit(&s_full[t][b]);
             if (b == 1) umma_commit(&k_empty[stage]);
           }
           __syncwarp();
         }
+        unit += pc.n;
+        ++piece;
       }
-      first = end;
-      unit += pc.n;
-      ++piece;
+    } else {  // O (+)= P V
+      const uint32_t idesc = idesc_bf16(kTileRows, D) | kIdescBMajorMn, ot = tmem_o + t * D;
+      const uint64_t vd = sw128_desc_mn(smem_u32(vbuf), C::kPanelBytes);
+      while (j < 2 * total && !dead) {
+        const Piece pc = piece_at(p, unit, u1);
+        const int first = j;
+        for (const int end = j + 2 * pc.n; j < end && !dead; ++j) {
+          const int b = j & 1, it = j >> 1, stage = it % S;
+          if (b == 0) wait(&v_full[stage], (it / S) & 1);
+          wait(&p_full[t][b], it & 1);
+          tc_fence_after();
+          const uint64_t vv = vd + ((uint64_t)(stage * C::kTileBytes + b * kHalf * 128) >> 4);
+          if (elect_one() && !dead) {
+#pragma unroll
+            for (int k = 0; k < kHalf / 16; ++k)
+              umma_bf16_ta(ot, st + b * kHalf + k * 8, vv + (k * 2048 >> 4), idesc, j > first || k > 0);
+            umma_commit(&pv_done[t][b]);
+            if (b == 1) umma_commit(&v_empty[stage]);
+          }
+          __syncwarp();
+        }
+        unit += pc.n;
+      }
     }
     if (dead) {  // let what was issued end
       *abort = 1;
-      if (elect_one()) umma_commit(&drain[t]);
+      if (elect_one()) umma_commit(&drain[which]);
       __syncwarp();
-      mbar_wait(&drain[t], 0, nullptr);
+      mbar_wait(&drain[which], 0, nullptr);
     }
   } else {
     // ---- softmax: thread = row of tile t ----------------------------------
