@@ -30,7 +30,10 @@
 namespace wr {
 namespace {
 
-constexpr int kStreamWarps = 4;
+// A CTA is one warp: its ring is small enough to fit beside a CTA of the
+// prefix's kernel, so that the own keys stream while the prefix computes, and
+// the hardware brings further CTAs as room appears.
+constexpr int kStreamWarps = 1;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 #define WR_NEG_INF (-__int_as_float(0x7f800000))
@@ -75,13 +78,13 @@ WR_DEVINL uint32_t pack_bf16(float lo, float hi) {
 // ---------------------------------------------------------------------------
 // The split, computed by each CTA from the lengths
 // ---------------------------------------------------------------------------
-constexpr int kScanThreads = kStreamWarps * 32;
+constexpr int kScanThreads = 32;
 
 struct ScanSmem {
   int64_t chunk[kScanThreads + 1];  // units before each thread's run of sequences
 };
 
-// All threads of the CTA (NT of them).  Fills sm.chunk; CTA 0 of an own
+// All threads of the CTA (one warp).  Fills sm.chunk; CTA 0 of an own
 // launch also writes seq_unit, all CTAs together token_seq.
 template <int MR, int NT>
 WR_DEVINL int64_t scan_units(const AttnArgs& a, ScanSmem& sm) {
@@ -92,20 +95,16 @@ WR_DEVINL int64_t scan_units(const AttnArgs& a, ScanSmem& sm) {
     const SeqInfo s = seq_info(a, b);
     sum += (int64_t)a.hkv * row_tiles<MR>(a, s) * key_units(a, s);
   }
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x;
   int64_t incl = sum;
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
     const int64_t u = __shfl_up_sync(0xffffffffu, incl, d);
     if (lane >= d) incl += u;
   }
-  __shared__ int64_t warp_sum[NT / 32];
-  if (lane == 31) warp_sum[warp] = incl;
-  __syncthreads();
-  for (int w = 0; w < warp; ++w) incl += warp_sum[w];
-  sm.chunk[threadIdx.x + 1] = incl;
-  if (threadIdx.x == 0) sm.chunk[0] = 0;
-  __syncthreads();
+  sm.chunk[lane + 1] = incl;
+  if (lane == 0) sm.chunk[0] = 0;
+  __syncwarp();
   if (a.own) {
     if (blockIdx.x == 0) {
       int64_t at = sm.chunk[threadIdx.x];
@@ -464,7 +463,7 @@ __global__ void __launch_bounds__(kStreamWarps * 32) k_attn_stream(const AttnArg
 template <int DP>
 struct StreamF32Cfg {
   static constexpr int kMR = 8;
-  static constexpr int kWarps = DP > 128 ? 2 : 4;
+  static constexpr int kWarps = 1;
   static constexpr int kRowBytes = DP * 4;
   static constexpr int kTile = kUnitTokens * kRowBytes;
   static constexpr int kQBytes = kMR * kRowBytes;
@@ -722,6 +721,10 @@ WR_DEVINL PieceList piece_list(const AttnSplit& sp, int64_t unit0, int us, int r
   return p;
 }
 
+// A row's pieces, 32 at a time: lane i looks up piece i and its weight, then
+// all lanes add up the pieces' columns, whose loads do not wait for one
+// another.  kWarps 1: a warp a row; 8: a CTA a row, each warp an eighth of its
+// pieces (few rows with many pieces).
 template <typename T, int MR, int DP, int kWarps>
 __global__ void __launch_bounds__(kWarps == 1 ? 128 : kWarps * 32) k_attn_combine(const CombineArgs c) {
   constexpr int VC = DP / 32;
@@ -734,11 +737,10 @@ __global__ void __launch_bounds__(kWarps == 1 ? 128 : kWarps * 32) k_attn_combin
   const int64_t row = (int64_t)blockIdx.x * kRowsCta + (kWarps == 1 ? wid : 0);
   griddep_wait();
   if (row >= (int64_t)a.T * a.hq) return;  // uniform over a row's warps
-  const int t = (int)(row / a.hq), hq = (int)(row - (int64_t)t * a.hq);
+  const int t = (int)row / a.hq, hq = (int)row - t * a.hq;
   const int h = hq / a.group, g = hq - h * a.group;
   const int b = a.q_start ? a.token_seq[t] : t;
   PieceList po{}, pp{};
-  bool done = false;
   if (b >= 0) {
     const SeqInfo s = seq_info(a, b);
     const int us = key_units(a, s), rts = row_tiles<MR>(a, s);
@@ -747,36 +749,59 @@ __global__ void __launch_bounds__(kWarps == 1 ? 128 : kWarps * 32) k_attn_combin
     sp.ranges = min(c.own_warps, sp.units);
     const int r = (t - s.q0) * a.group + g;
     po = piece_list(sp, a.seq_unit[b] + ((int64_t)h * rts + r / MR) * us, us, r % MR);
-    done = po.whole && a.direct;
-  }
-  if (done) return;  // written by the first kernel
-  if (c.has_pre && b >= 0) {
-    const int r = t * a.group + g, rt = r / c.pre_mr;
-    pp = piece_list(c.pre_split, ((int64_t)h * c.pre_rts + rt) * c.pre_us, c.pre_us, r - rt * c.pre_mr);
+    if (po.whole && a.direct) return;  // written by the first kernel
+    if (c.has_pre) {
+      const int rp = t * a.group + g, rt = rp / c.pre_mr;
+      pp = piece_list(c.pre_split, ((int64_t)h * c.pre_rts + rt) * c.pre_us, c.pre_us, rp - rt * c.pre_mr);
+    }
   }
   const int total = po.n + pp.n;
+  const int lo = kWarps == 1 ? 0 : total * wid / kWarps, hi = kWarps == 1 ? total : total * (wid + 1) / kWarps;
   float m = WR_NEG_INF, l = 0.f, o[VC];
 #pragma unroll
   for (int i = 0; i < VC; ++i) o[i] = 0.f;
-#pragma unroll 4
-  for (int i = kWarps == 1 ? 0 : wid; i < total; i += kWarps) {
-    const bool mine = i < po.n;
-    const PieceList& p = mine ? po : pp;
-    const int k = mine ? i : i - po.n;
-    const AttnPartials& part = mine ? a.part : c.pre;
-    const int64_t at = p.whole ? row : ((p.w0 + k) * 2 + (k == 0 ? 1 : 0)) * (mine ? MR : c.pre_mr) + p.rl;
-    const float* src = (p.whole ? (mine ? a.home : c.pre_home) : part.piece) + at * a.dim;
-    const float2 ml = (p.whole ? (mine ? a.home_ml : c.pre_home_ml) : part.piece_ml)[at];
-    const float nm = fmaxf(m, ml.x);
+  for (int c0 = lo; c0 < hi; c0 += 32) {
+    const int i = c0 + lane;
+    const float* src = nullptr;
+    float2 ml = make_float2(WR_NEG_INF, 0.f);
+    if (i < hi) {
+      const bool mine = i < po.n;
+      const PieceList& p = mine ? po : pp;
+      const int k = mine ? i : i - po.n;
+      const int64_t at = p.whole ? row : ((p.w0 + k) * 2 + (k == 0 ? 1 : 0)) * (mine ? MR : c.pre_mr) + p.rl;
+      src = (p.whole ? (mine ? a.home : c.pre_home) : (mine ? a.part.piece : c.pre.piece)) + at * a.dim;
+      ml = (p.whole ? (mine ? a.home_ml : c.pre_home_ml) : (mine ? a.part.piece_ml : c.pre.piece_ml))[at];
+    }
+    float nm = fmaxf(m, ml.x);
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) nm = fmaxf(nm, __shfl_xor_sync(0xffffffffu, nm, d));
     const float base = nm == WR_NEG_INF ? 0.f : nm;
-    const float fo = ex2(m - base), fn = ex2(ml.x - base);
+    const float fo = ex2(m - base), w = ex2(ml.x - base);
+    float add = ml.y * w;
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) add += __shfl_xor_sync(0xffffffffu, add, d);
     m = nm;
-    l = l * fo + ml.y * fn;
+    l = l * fo + add;
 #pragma unroll
-    for (int q = 0; q < VC; q += VW) {
-      const int d = q * 32 + lane * VW;
+    for (int q = 0; q < VC; ++q) o[q] *= fo;
+    const int n = min(32, hi - c0);
+#pragma unroll 4
+    for (int k = 0; k < n; ++k) {
+      const float* p = reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(src), k));
+      const float f = __shfl_sync(0xffffffffu, w, k);
 #pragma unroll
-      for (int e = 0; e < VW; ++e) o[q + e] = o[q + e] * fo + (d < a.dim ? src[d + e] : 0.f) * fn;
+      for (int q = 0; q < VC; q += VW) {
+        const int d = q * 32 + lane * VW;
+        if (d < a.dim) {
+          if constexpr (VW == 4) {
+            const float4 v = *reinterpret_cast<const float4*>(p + d);
+            o[q] += f * v.x; o[q + 1] += f * v.y; o[q + 2] += f * v.z; o[q + 3] += f * v.w;
+          } else {
+            const float2 v = *reinterpret_cast<const float2*>(p + d);
+            o[q] += f * v.x; o[q + 1] += f * v.y;
+          }
+        }
+      }
     }
   }
   if constexpr (kWarps > 1) {
@@ -845,10 +870,11 @@ Plan make_plan(const AttnProblem& p) {
   const bool f32 = p.c.dtype == WR_DTYPE_F32;
   pl.dp = p.c.dim <= 64 ? 64 : (p.c.dim <= 128 ? 128 : 256);
   pl.mr = f32 ? 8 : 16;
-  pl.warps_cta = f32 && pl.dp > 128 ? 2 : kStreamWarps;
+  pl.warps_cta = kStreamWarps;
   pl.smem = f32 ? (pl.dp == 64 ? StreamF32Cfg<64>::kSmem : pl.dp == 128 ? StreamF32Cfg<128>::kSmem : StreamF32Cfg<256>::kSmem)
                 : (pl.dp == 64 ? StreamCfg<64>::kSmem : pl.dp == 128 ? StreamCfg<128>::kSmem : StreamCfg<256>::kSmem);
-  const int per_sm = 228 * 1024 / (pl.smem + 4096) < 1 ? 1 : (228 * 1024 / (pl.smem + 4096) > 4 ? 4 : 228 * 1024 / (pl.smem + 4096));
+  const int fit = 227 * 1024 / (pl.smem + 2048);
+  const int per_sm = fit < 1 ? 1 : (fit > 16 ? 16 : fit);
   const int64_t most = (int64_t)device_sm_count() * per_sm;
   const int group = p.hq / p.c.hkv;
   pl.rows = (int64_t)p.T * p.hq;  // of the output

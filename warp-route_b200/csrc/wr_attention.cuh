@@ -25,12 +25,17 @@ struct AttnSplit {
   int64_t units;   // of the launch
   int64_t ranges;  // warps with a range: min(warps, units)
 };
+// Quotients of 32 bits where they do (a 64-bit division is some hundred
+// instructions).
+__host__ __device__ inline int64_t quotient(int64_t a, int64_t b) {
+  return ((uint64_t)a | (uint64_t)b) >> 32 ? a / b : (int64_t)((uint32_t)a / (uint32_t)b);
+}
 __host__ __device__ inline int64_t range_start(const AttnSplit& s, int64_t w) {
-  return w * s.units / s.ranges;
+  return quotient(w * s.units, s.ranges);
 }
 // The warp whose range holds unit u.
 __host__ __device__ inline int64_t range_of(const AttnSplit& s, int64_t u) {
-  return ((u + 1) * s.ranges - 1) / s.units;
+  return quotient((u + 1) * s.ranges - 1, s.units);
 }
 
 // Partial results: unnormalised sums O [dim] in fp32 with (m, l): m the
