@@ -76,57 +76,56 @@ WR_DEVINL uint32_t pack_bf16(float lo, float hi) {
 }
 
 // ---------------------------------------------------------------------------
-// The split, computed by each CTA from the lengths
+// The split, computed by each warp from the lengths
 // ---------------------------------------------------------------------------
-constexpr int kScanThreads = 32;
+template <int MR>
+WR_DEVINL int64_t seq_units(const AttnArgs& a, int b) {
+  if (b >= a.B) return 0;
+  const SeqInfo s = seq_info(a, b);
+  return (int64_t)a.hkv * row_tiles<MR>(a, s) * key_units(a, s);
+}
 
-struct ScanSmem {
-  int64_t chunk[kScanThreads + 1];  // units before each thread's run of sequences
-};
-
-// All threads of the CTA (one warp).  Fills sm.chunk; CTA 0 of an own
-// launch also writes seq_unit, all CTAs together token_seq.
-template <int MR, int NT>
-WR_DEVINL int64_t scan_units(const AttnArgs& a, ScanSmem& sm) {
-  const int per = (a.B + NT - 1) / NT;
-  const int b0 = min(a.B, (int)threadIdx.x * per), b1 = min(a.B, b0 + per);
+// Units of the launch: a warp adds them up, 32 sequences at a time.
+template <int MR>
+WR_DEVINL int64_t all_units(const AttnArgs& a, int lane) {
   int64_t sum = 0;
-  for (int b = b0; b < b1; ++b) {
-    const SeqInfo s = seq_info(a, b);
-    sum += (int64_t)a.hkv * row_tiles<MR>(a, s) * key_units(a, s);
-  }
-  const int lane = threadIdx.x;
-  int64_t incl = sum;
+#pragma unroll 4
+  for (int b = lane; b < a.B; b += 32) sum += seq_units<MR>(a, b);
 #pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const int64_t u = __shfl_up_sync(0xffffffffu, incl, d);
-    if (lane >= d) incl += u;
-  }
-  sm.chunk[lane + 1] = incl;
-  if (lane == 0) sm.chunk[0] = 0;
-  __syncwarp();
-  if (a.own) {
-    if (blockIdx.x == 0) {
-      int64_t at = sm.chunk[threadIdx.x];
-      for (int b = b0; b < b1; ++b) {
-        const SeqInfo s = seq_info(a, b);
-        a.seq_unit[b] = at;
-        at += (int64_t)a.hkv * row_tiles<MR>(a, s) * key_units(a, s);
+  for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+  return sum;
+}
+
+// What the joining kernel needs: the first unit of each sequence, by warp 0 of
+// an own launch, and the sequence of each token, by all of them.
+template <int MR>
+WR_DEVINL void write_index(const AttnArgs& a, int lane) {
+  if (!a.own) return;
+  if (blockIdx.x == 0) {
+    int64_t base = 0;
+    for (int b0 = 0; b0 < a.B; b0 += 32) {
+      const int64_t v = seq_units<MR>(a, b0 + lane);
+      int64_t incl = v;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int64_t u = __shfl_up_sync(0xffffffffu, incl, d);
+        if (lane >= d) incl += u;
       }
-      if (threadIdx.x == 0) a.seq_unit[a.B] = sm.chunk[NT];
+      if (b0 + lane < a.B) a.seq_unit[b0 + lane] = base + incl - v;
+      base += __shfl_sync(0xffffffffu, incl, 31);
     }
-    if (a.q_start)
-      for (int t = blockIdx.x * NT + threadIdx.x; t < a.T; t += gridDim.x * NT) {
-        int lo = 0, hi = a.B;  // last b with q_start[b] <= t
-        while (hi - lo > 1) {
-          const int mid = (lo + hi) >> 1;
-          if (__ldg(a.q_start + mid) <= t) lo = mid; else hi = mid;
-        }
-        const SeqInfo s = seq_info(a, lo);
-        a.token_seq[t] = t >= s.q0 && t < s.q0 + s.nq ? lo : -1;
-      }
+    if (lane == 0) a.seq_unit[a.B] = base;
   }
-  return sm.chunk[NT];
+  if (a.q_start)
+    for (int t = blockIdx.x * 32 + lane; t < a.T; t += gridDim.x * 32) {
+      int lo = 0, hi = a.B;  // last b with q_start[b] <= t
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (__ldg(a.q_start + mid) <= t) lo = mid; else hi = mid;
+      }
+      const SeqInfo s = seq_info(a, lo);
+      a.token_seq[t] = t >= s.q0 && t < s.q0 + s.nq ? lo : -1;
+    }
 }
 
 // A position in the order of the units.
@@ -142,25 +141,28 @@ struct Cursor {
     us = key_units(a, s);
   }
   // To unit `at` (< units of the launch).
-  template <int NT>
-  WR_DEVINL void seek(const AttnArgs& a, const ScanSmem& sm, int64_t at) {
-    int lo = 0, hi = NT;  // last run that starts at or before `at`
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (sm.chunk[mid] <= at) lo = mid; else hi = mid;
+  WR_DEVINL void seek(const AttnArgs& a, int lane, int64_t at) {
+    for (int b0 = 0;; b0 += 32) {
+      const int64_t v = seq_units<MR>(a, b0 + lane);
+      int64_t incl = v;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int64_t u = __shfl_up_sync(0xffffffffu, incl, d);
+        if (lane >= d) incl += u;
+      }
+      const uint32_t past = __ballot_sync(0xffffffffu, incl > at);
+      if (past) {
+        const int first = __ffs(past) - 1;
+        b = b0 + first;
+        at -= __shfl_sync(0xffffffffu, incl - v, first);
+        break;
+      }
+      at -= __shfl_sync(0xffffffffu, incl, 31);
     }
-    int64_t left = at - sm.chunk[lo];
-    b = lo * ((a.B + NT - 1) / NT);
-    for (;;) {
-      load(a);
-      const int64_t n = (int64_t)a.hkv * rts * us;
-      if (left < n) break;
-      left -= n;
-      ++b;
-    }
-    const int64_t tile = left / us;
-    u = (int)(left - tile * us);
-    h = (int)(tile / rts);
+    load(a);
+    const int64_t tile = quotient(at, us);
+    u = (int)(at - tile * us);
+    h = (int)quotient(tile, rts);
     rt = (int)(tile - (int64_t)h * rts);
   }
   // Never called past the launch's last unit.
@@ -236,12 +238,11 @@ __global__ void __launch_bounds__(kStreamWarps * 32) k_attn_stream(const AttnArg
   using C = StreamCfg<DP>;
   constexpr int MR = 16, CPR = DP / 8, RPP = 32 / CPR;  // chunks a row, rows a pass of the warp
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ ScanSmem sm;
   __shared__ uint32_t s_bits[kStreamWarps][kStages];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   griddep_launch_dependents();
   AttnSplit sp;
-  sp.units = scan_units<MR, kStreamWarps * 32>(a, sm);
+  sp.units = all_units<MR>(a, lane);
   sp.ranges = min((int64_t)gridDim.x * kStreamWarps, sp.units);
   const int64_t w = (int64_t)warp * gridDim.x + blockIdx.x;
   if (w < sp.ranges) {
@@ -250,7 +251,7 @@ __global__ void __launch_bounds__(kStreamWarps * 32) k_attn_stream(const AttnArg
     const uint32_t ring_s = smem_u32(ring);
     const uint32_t q_s = ring_s + kStages * 2 * C::kTile;
     Cursor<MR> cl, cc;  // the copies' and the products' position
-    cl.seek<kStreamWarps * 32>(a, sm, u0);
+    cl.seek(a, lane, u0);
     cc = cl;
     const int n = (int)(u1 - u0);
     int page = lane_page(a, cl, lane);
@@ -284,6 +285,7 @@ __global__ void __launch_bounds__(kStreamWarps * 32) k_attn_stream(const AttnArg
     };
 #pragma unroll
     for (int s = 0; s < kStages - 1; ++s) load();
+    write_index<MR>(a, lane);
 
     uint32_t qf[C::kQSmem ? 1 : DP / 16][4];
     float o[DP / 8][4];
@@ -453,6 +455,8 @@ __global__ void __launch_bounds__(kStreamWarps * 32) k_attn_stream(const AttnArg
       if (it + 1 < n) cc.next(a);
     }
     cp_async_wait<0>();
+  } else {
+    write_index<MR>(a, lane);
   }
   griddep_wait();  // this launch counts as complete only after the one before it
 }
@@ -479,16 +483,15 @@ struct StreamF32Cfg {
 template <int DP>
 __global__ void __launch_bounds__(StreamF32Cfg<DP>::kWarps * 32) k_attn_stream_f32(const AttnArgs a) {
   using C = StreamF32Cfg<DP>;
-  constexpr int MR = C::kMR, CPR = DP / 4, NT = C::kWarps * 32;
+  constexpr int MR = C::kMR, CPR = DP / 4;
   constexpr int VC = DP / 32;  // columns of O a lane has
   constexpr int VW = VC < 4 ? VC : 4;  // ... in runs of VW
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ ScanSmem sm;
   __shared__ uint32_t s_bits[C::kWarps][kStages];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   griddep_launch_dependents();
   AttnSplit sp;
-  sp.units = scan_units<MR, NT>(a, sm);
+  sp.units = all_units<MR>(a, lane);
   sp.ranges = min((int64_t)gridDim.x * C::kWarps, sp.units);
   const int64_t w = (int64_t)warp * gridDim.x + blockIdx.x;
   if (w < sp.ranges) {
@@ -498,7 +501,7 @@ __global__ void __launch_bounds__(StreamF32Cfg<DP>::kWarps * 32) k_attn_stream_f
     float* qs = reinterpret_cast<float*>(ring + kStages * 2 * C::kTile);
     float* ps = qs + MR * DP;
     Cursor<MR> cl, cc;
-    cl.template seek<NT>(a, sm, u0);
+    cl.seek(a, lane, u0);
     cc = cl;
     const int n = (int)(u1 - u0);
     int page = lane_page(a, cl, lane);
@@ -531,6 +534,7 @@ __global__ void __launch_bounds__(StreamF32Cfg<DP>::kWarps * 32) k_attn_stream_f
     };
 #pragma unroll
     for (int s = 0; s < kStages - 1; ++s) load();
+    write_index<MR>(a, lane);
 
     const int t = lane & 15, hf = lane >> 4;
     float o[MR][VC], m[4], l[4];  // m, l: rows hf * 4 + 0..3
@@ -686,6 +690,8 @@ __global__ void __launch_bounds__(StreamF32Cfg<DP>::kWarps * 32) k_attn_stream_f
       if (it + 1 < n) cc.next(a);
     }
     cp_async_wait<0>();
+  } else {
+    write_index<MR>(a, lane);
   }
   griddep_wait();
 }
