@@ -18,7 +18,7 @@
 // rate).  The units of all sequences are dealt to the warps evenly (see
 // wr_attention.cuh), so one long sequence and hundreds of short ones fill the
 // GPU alike.  k_attn_stream_f32: the same ring and split with fp32 products
-// on the CUDA cores, 8 rows a warp.
+// on the CUDA cores, 4 or 8 rows a warp.
 //
 // Prefix: its rows are the tokens of all sequences.  With one sequence, or a
 // prefix short enough, each sequence reads it with its own keys; else it is a
@@ -79,85 +79,87 @@ WR_DEVINL uint32_t pack_bf16(float lo, float hi) {
 // The split, computed by each warp from the lengths
 // ---------------------------------------------------------------------------
 template <int MR>
-WR_DEVINL int64_t seq_units(const AttnArgs& a, int b) {
-  if (b >= a.B) return 0;
-  const SeqInfo s = seq_info(a, b);
-  return (int64_t)a.hkv * row_tiles<MR>(a, s) * key_units(a, s);
+WR_DEVINL int64_t seg_units(const AttnArgs& a, int i) {
+  if (i >= segments(a)) return 0;
+  const Segment s = segment(a, i);
+  return (int64_t)a.hkv * row_tiles<MR>(a, s) * key_units(s);
 }
 
-// Units of the launch: a warp adds them up, 32 sequences at a time.
+// Units of the launch: a warp adds them up, 32 segments at a time.
 template <int MR>
 WR_DEVINL int64_t all_units(const AttnArgs& a, int lane) {
   int64_t sum = 0;
 #pragma unroll 4
-  for (int b = lane; b < a.B; b += 32) sum += seq_units<MR>(a, b);
+  for (int i = lane; i < segments(a); i += 32) sum += seg_units<MR>(a, i);
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
   return sum;
 }
 
-// What the joining kernel needs: the first unit of each sequence, by warp 0 of
-// an own launch, and the sequence of each token, by all of them.
+WR_DEVINL int64_t warp_before(int64_t v, int lane, int64_t& all) {
+  int64_t incl = v;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int64_t u = __shfl_up_sync(0xffffffffu, incl, d);
+    if (lane >= d) incl += u;
+  }
+  all = __shfl_sync(0xffffffffu, incl, 31);
+  return incl - v;
+}
+
+// The sequence that token t belongs to, -1: none.
+WR_DEVINL int seq_of(const AttnArgs& a, int t) {
+  int lo = 0, hi = a.B;  // last b with q_start[b] <= t
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (__ldg(a.q_start + mid) <= t) lo = mid; else hi = mid;
+  }
+  const Segment s = segment(a, lo + (a.lead > 0));
+  return t >= s.q0 && t < s.q0 + s.nq ? lo : -1;
+}
+
+// What the joining kernel reads: the first unit of each segment, by warp 0,
+// and the sequence of each token, by all.
 template <int MR>
 WR_DEVINL void write_index(const AttnArgs& a, int lane) {
-  if (!a.own) return;
   if (blockIdx.x == 0) {
-    int64_t base = 0;
-    for (int b0 = 0; b0 < a.B; b0 += 32) {
-      const int64_t v = seq_units<MR>(a, b0 + lane);
-      int64_t incl = v;
-#pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const int64_t u = __shfl_up_sync(0xffffffffu, incl, d);
-        if (lane >= d) incl += u;
-      }
-      if (b0 + lane < a.B) a.seq_unit[b0 + lane] = base + incl - v;
-      base += __shfl_sync(0xffffffffu, incl, 31);
+    int64_t base = 0, all;
+    for (int i0 = 0; i0 < segments(a); i0 += 32) {
+      const int64_t at = base + warp_before(seg_units<MR>(a, i0 + lane), lane, all);
+      if (i0 + lane < segments(a)) a.seg_unit[i0 + lane] = at;
+      base += all;
     }
-    if (lane == 0) a.seq_unit[a.B] = base;
+    if (lane == 0) a.seg_unit[segments(a)] = base;
   }
   if (a.q_start)
-    for (int t = blockIdx.x * 32 + lane; t < a.T; t += gridDim.x * 32) {
-      int lo = 0, hi = a.B;  // last b with q_start[b] <= t
-      while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (__ldg(a.q_start + mid) <= t) lo = mid; else hi = mid;
-      }
-      const SeqInfo s = seq_info(a, lo);
-      a.token_seq[t] = t >= s.q0 && t < s.q0 + s.nq ? lo : -1;
-    }
+    for (int t = blockIdx.x * 32 + lane; t < a.T; t += gridDim.x * 32) a.token_seq[t] = seq_of(a, t);
 }
 
 // A position in the order of the units.
 template <int MR>
 struct Cursor {
-  int b, h, rt, u;   // sequence, key head, row tile, unit
-  int rts, us;       // row tiles and units of the sequence
-  SeqInfo s;
+  int b, h, rt, u;   // segment, key head, row tile, unit
+  int rts, us;       // row tiles and units of the segment
+  Segment s;
 
   WR_DEVINL void load(const AttnArgs& a) {
-    s = seq_info(a, b);
+    s = segment(a, b);
     rts = row_tiles<MR>(a, s);
-    us = key_units(a, s);
+    us = key_units(s);
   }
   // To unit `at` (< units of the launch).
   WR_DEVINL void seek(const AttnArgs& a, int lane, int64_t at) {
-    for (int b0 = 0;; b0 += 32) {
-      const int64_t v = seq_units<MR>(a, b0 + lane);
-      int64_t incl = v;
-#pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const int64_t u = __shfl_up_sync(0xffffffffu, incl, d);
-        if (lane >= d) incl += u;
-      }
-      const uint32_t past = __ballot_sync(0xffffffffu, incl > at);
+    for (int i0 = 0;; i0 += 32) {
+      int64_t all;
+      const int64_t v = seg_units<MR>(a, i0 + lane), before = warp_before(v, lane, all);
+      const uint32_t past = __ballot_sync(0xffffffffu, before + v > at);
       if (past) {
         const int first = __ffs(past) - 1;
-        b = b0 + first;
-        at -= __shfl_sync(0xffffffffu, incl - v, first);
+        b = i0 + first;
+        at -= __shfl_sync(0xffffffffu, before, first);
         break;
       }
-      at -= __shfl_sync(0xffffffffu, incl, 31);
+      at -= all;
     }
     load(a);
     const int64_t tile = quotient(at, us);
@@ -176,7 +178,7 @@ struct Cursor {
     do {
       ++b;
       load(a);
-    } while (rts == 0 && b + 1 < a.B);
+    } while (rts == 0 && b + 1 < segments(a));
   }
 };
 
@@ -185,14 +187,14 @@ template <int MR>
 WR_DEVINL int lane_page(const AttnArgs& a, const Cursor<MR>& c, int lane) {
   const int j = c.u * kUnitTokens + (lane & 15);
   int page, row;
-  if (j < a.prefix) {
+  if (j < c.s.prefix) {
     split_page(j, a.page_size, a.page_shift, page, row);
     return __ldg(a.prefix_pages + page);
   }
-  const int jj = j - a.prefix;
+  const int jj = j - c.s.prefix;
   if (jj >= c.s.len) return -1;
   split_page(jj, a.page_size, a.page_shift, page, row);
-  return __ldg(a.tables + c.b * a.table_stride + page);
+  return __ldg(a.tables + (c.b - (a.lead > 0)) * a.table_stride + page);
 }
 
 // Offset (elements) of this lane's key in the cache; its valid bit.  A page
@@ -201,7 +203,7 @@ template <int MR>
 WR_DEVINL int64_t lane_offset(const AttnArgs& a, const Cursor<MR>& c, int page, int lane, bool& ok) {
   const int j = c.u * kUnitTokens + (lane & 15);
   int p, row;
-  split_page(j < a.prefix ? j : j - a.prefix, a.page_size, a.page_shift, p, row);
+  split_page(j < c.s.prefix ? j : j - c.s.prefix, a.page_size, a.page_shift, p, row);
   ok = page >= 0 && page < a.num_pages;
   return ok ? page * a.page_stride + c.h * a.head_stride + row * a.slot_stride : 0;
 }
@@ -209,16 +211,8 @@ WR_DEVINL int64_t lane_offset(const AttnArgs& a, const Cursor<MR>& c, int page, 
 // Number of keys that row (token i of the sequence) sees of the segment.
 template <int MR>
 WR_DEVINL int row_limit(const AttnArgs& a, const Cursor<MR>& c, int i) {
-  return a.prefix + max(0, c.s.len - c.s.nq + i + 1);
+  return c.s.prefix + max(0, c.s.len - c.s.nq + i + 1);
 }
-
-// Where a finished piece goes: out (whole and final), home or a warp's slot.
-struct PieceDst {
-  float* o;
-  float2* ml;
-  int64_t row0;  // row r of the tile is row0 + r of (o, ml), home and out rows excepted
-  bool home, final;
-};
 
 // ---------------------------------------------------------------------------
 // bf16
@@ -423,7 +417,7 @@ __global__ void __launch_bounds__(kStreamWarps * 32) k_attn_stream(const AttnArg
           t0 += __shfl_xor_sync(0xffffffffu, t0, d);
           t1 += __shfl_xor_sync(0xffffffffu, t1, d);
         }
-        const bool whole = tile_end && first == 0;
+        const bool whole = tile_end && first == 0, lead = a.lead > 0 && cc.b == 0;
         const int rows = cc.s.nq * a.group;
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
@@ -443,12 +437,13 @@ __global__ void __launch_bounds__(kStreamWarps * 32) k_attn_stream(const AttnArg
             if (a.lse && (lane & 3) == 0) a.lse[orow] = ll == 0.f ? WR_NEG_INF : (mm + log2f(ll)) * kLn2;
           } else {
             const int64_t prow = (w * 2 + (first == 0 ? 1 : 0)) * MR + rl;
-            float* op = whole ? a.home + orow * a.dim : a.part.piece + prow * a.dim;
+            float* op = !whole ? a.part.piece + prow * a.dim : (lead ? a.lead_home : a.home) + orow * a.dim;
 #pragma unroll
             for (int d = 0; d < DP / 8; ++d)
               if (d * 8 + c2 < a.dim)
                 *reinterpret_cast<float2*>(op + d * 8 + c2) = make_float2(o[d][2 * half], o[d][2 * half + 1]);
-            if ((lane & 3) == 0) (whole ? a.home_ml + orow : a.part.piece_ml + prow)[0] = make_float2(mm, ll);
+            if ((lane & 3) == 0)
+              *(!whole ? a.part.piece_ml + prow : (lead ? a.lead_home_ml : a.home_ml) + orow) = make_float2(mm, ll);
           }
         }
       }
@@ -464,9 +459,9 @@ __global__ void __launch_bounds__(kStreamWarps * 32) k_attn_stream(const AttnArg
 // ---------------------------------------------------------------------------
 // fp32
 // ---------------------------------------------------------------------------
-template <int DP>
+template <int DP, int MR>
 struct StreamF32Cfg {
-  static constexpr int kMR = 8;
+  static constexpr int kMR = MR;
   static constexpr int kWarps = 1;
   static constexpr int kRowBytes = DP * 4;
   static constexpr int kTile = kUnitTokens * kRowBytes;
@@ -480,10 +475,10 @@ struct StreamF32Cfg {
 // of the second: DP / 32 columns, all keys.  K chunks are swizzled by key, so
 // that the 8 lanes of a 16-byte read phase meet 8 different banks; Q and the
 // weights are read by all lanes at once.
-template <int DP>
-__global__ void __launch_bounds__(StreamF32Cfg<DP>::kWarps * 32) k_attn_stream_f32(const AttnArgs a) {
-  using C = StreamF32Cfg<DP>;
-  constexpr int MR = C::kMR, CPR = DP / 4;
+template <int DP, int MR>
+__global__ void __launch_bounds__(32) k_attn_stream_f32(const AttnArgs a) {
+  using C = StreamF32Cfg<DP, MR>;
+  constexpr int CPR = DP / 4, HR = MR / 2;  // rows whose statistics a half of the lanes keeps
   constexpr int VC = DP / 32;  // columns of O a lane has
   constexpr int VW = VC < 4 ? VC : 4;  // ... in runs of VW
   extern __shared__ __align__(128) uint8_t smem[];
@@ -537,8 +532,8 @@ __global__ void __launch_bounds__(StreamF32Cfg<DP>::kWarps * 32) k_attn_stream_f
     write_index<MR>(a, lane);
 
     const int t = lane & 15, hf = lane >> 4;
-    float o[MR][VC], m[4], l[4];  // m, l: rows hf * 4 + 0..3
-    int lim[4], first = 0;
+    float o[MR][VC], m[HR], l[HR];  // m, l: rows hf * HR + 0 .. HR - 1
+    int lim[HR], first = 0;
     for (int it = 0; it < n; ++it) {
       __syncwarp();
       load();
@@ -550,10 +545,10 @@ __global__ void __launch_bounds__(StreamF32Cfg<DP>::kWarps * 32) k_attn_stream_f
 #pragma unroll
           for (int c = 0; c < VC; ++c) o[r][c] = 0.f;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
+        for (int e = 0; e < HR; ++e) {
           m[e] = WR_NEG_INF;
           l[e] = 0.f;
-          lim[e] = row_limit(a, cc, (cc.rt * MR + hf * 4 + e) / a.group);
+          lim[e] = row_limit(a, cc, (cc.rt * MR + hf * HR + e) / a.group);
         }
         for (int x = lane; x < MR * CPR; x += 32) {
           const int r = x / CPR, c = x % CPR, rr = cc.rt * MR + r, ii = rr / a.group;
@@ -589,14 +584,14 @@ __global__ void __launch_bounds__(StreamF32Cfg<DP>::kWarps * 32) k_attn_stream_f
           }
         }
       }
-      // each half keeps its four rows
+      // each half keeps its rows
       const int j = cc.u * kUnitTokens + t;
       const bool vis = (bits >> t) & 1;
-      float x[4], mx[4];
+      float x[HR], mx[HR];
       bool up = false;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float give = hf ? s[e] : s[e + 4], keep = hf ? s[e + 4] : s[e];
+      for (int e = 0; e < HR; ++e) {
+        const float give = hf ? s[e] : s[e + HR], keep = hf ? s[e + HR] : s[e];
         const float sum = keep + __shfl_xor_sync(0xffffffffu, give, 16);
         x[e] = vis && j < lim[e] ? sum * a.scale_log2 : WR_NEG_INF;
         mx[e] = x[e];
@@ -605,9 +600,9 @@ __global__ void __launch_bounds__(StreamF32Cfg<DP>::kWarps * 32) k_attn_stream_f
         up |= mx[e] > m[e];
       }
       if (__any_sync(0xffffffffu, up)) {
-        float f[4];
+        float f[HR];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
+        for (int e = 0; e < HR; ++e) {
           const float nm = fmaxf(m[e], mx[e]);
           f[e] = nm == m[e] ? 1.f : ex2(m[e] - nm);
           m[e] = nm;
@@ -615,25 +610,24 @@ __global__ void __launch_bounds__(StreamF32Cfg<DP>::kWarps * 32) k_attn_stream_f
         }
 #pragma unroll
         for (int r = 0; r < MR; ++r) {
-          const float fr = __shfl_sync(0xffffffffu, f[r & 3], (r >> 2) << 4);
+          const float fr = __shfl_sync(0xffffffffu, f[r % HR], (r / HR) << 4);
 #pragma unroll
           for (int c = 0; c < VC; ++c) o[r][c] *= fr;
         }
       }
-      float4 pw;
-      float* pv = &pw.x;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        pv[e] = ex2(x[e] - (m[e] == WR_NEG_INF ? 0.f : m[e]));
-        l[e] += pv[e];
+      for (int e = 0; e < HR; ++e) {
+        const float w = ex2(x[e] - (m[e] == WR_NEG_INF ? 0.f : m[e]));
+        l[e] += w;
+        ps[t * MR + hf * HR + e] = w;
       }
-      *reinterpret_cast<float4*>(ps + t * MR + hf * 4) = pw;
       __syncwarp();
 #pragma unroll 4
       for (int k = 0; k < kUnitTokens; ++k) {
-        const float4 pa = *reinterpret_cast<const float4*>(ps + k * MR);
-        const float4 pb = *reinterpret_cast<const float4*>(ps + k * MR + 4);
-        const float p[8] = {pa.x, pa.y, pa.z, pa.w, pb.x, pb.y, pb.z, pb.w};
+        float p[MR];
+#pragma unroll
+        for (int r = 0; r < MR; r += 4)
+          *reinterpret_cast<float4*>(p + r) = *reinterpret_cast<const float4*>(ps + k * MR + r);
         float v[VC];
 #pragma unroll
         for (int g = 0; g < VC; g += VW) {
@@ -653,18 +647,18 @@ __global__ void __launch_bounds__(StreamF32Cfg<DP>::kWarps * 32) k_attn_stream_f
       }
       const bool tile_end = cc.u == cc.us - 1;
       if (tile_end || it == n - 1) {
-        float ls[4];
+        float ls[HR];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
+        for (int e = 0; e < HR; ++e) {
           ls[e] = l[e];
 #pragma unroll
           for (int d = 1; d < 16; d <<= 1) ls[e] += __shfl_xor_sync(0xffffffffu, ls[e], d);
         }
-        const bool whole = tile_end && first == 0;
+        const bool whole = tile_end && first == 0, lead = a.lead > 0 && cc.b == 0;
 #pragma unroll
         for (int r = 0; r < MR; ++r) {
-          const float mm = __shfl_sync(0xffffffffu, m[r & 3], (r >> 2) << 4);
-          const float ll = __shfl_sync(0xffffffffu, ls[r & 3], (r >> 2) << 4);
+          const float mm = __shfl_sync(0xffffffffu, m[r % HR], (r / HR) << 4);
+          const float ll = __shfl_sync(0xffffffffu, ls[r % HR], (r / HR) << 4);
           const int rr = cc.rt * MR + r;
           if (rr >= rows) continue;
           const int i = rr / a.group;
@@ -673,7 +667,7 @@ __global__ void __launch_bounds__(StreamF32Cfg<DP>::kWarps * 32) k_attn_stream_f
           const bool fin = whole && a.direct;
           const float inv = !fin ? 1.f : (ll > 0.f ? 1.f / ll : (ll == 0.f ? 0.f : ll));
           float* op = fin ? static_cast<float*>(a.out) + orow * a.dim
-                          : (whole ? a.home + orow * a.dim : a.part.piece + prow * a.dim);
+                          : (!whole ? a.part.piece + prow * a.dim : (lead ? a.lead_home : a.home) + orow * a.dim);
 #pragma unroll
           for (int g = 0; g < VC; g += VW) {
             const int d = g * 32 + lane * VW;
@@ -682,7 +676,7 @@ __global__ void __launch_bounds__(StreamF32Cfg<DP>::kWarps * 32) k_attn_stream_f
               for (int c = 0; c < VW; ++c) op[d + c] = o[r][g + c] * inv;
           }
           if (lane == 0) {
-            if (!fin) (whole ? a.home_ml + orow : a.part.piece_ml + prow)[0] = make_float2(mm, ll);
+            if (!fin) *(!whole ? a.part.piece_ml + prow : (lead ? a.lead_home_ml : a.home_ml) + orow) = make_float2(mm, ll);
             else if (a.lse) a.lse[orow] = ll == 0.f ? WR_NEG_INF : (mm + log2f(ll)) * kLn2;
           }
         }
@@ -700,14 +694,16 @@ __global__ void __launch_bounds__(StreamF32Cfg<DP>::kWarps * 32) k_attn_stream_f
 // Joining the pieces
 // ---------------------------------------------------------------------------
 struct CombineArgs {
-  AttnArgs own;       // the launch over the sequences' own keys
+  AttnArgs own;       // the launch of k_attn_stream*
   int64_t own_warps;
-  int has_pre;        // a launch over the prefix: its partial results
-  AttnPartials pre;
+  int has_pre;        // the prefix's partial results: of that launch's segment 0,
+                      // or of the tensor cores' launch,
+  int tiles;          // then with this split and these rows a tile, tiles a key
+  AttnPartials pre;   // head and units of its keys
   const float* pre_home;
   const float2* pre_home_ml;
   AttnSplit pre_split;
-  int pre_mr, pre_rts, pre_us;  // rows a tile, tiles a key head, units of its keys
+  int pre_mr, pre_rts, pre_us;
 };
 
 // A row's pieces of one launch: whole (in home), or n in slots of the warps
@@ -736,29 +732,53 @@ __global__ void __launch_bounds__(kWarps == 1 ? 128 : kWarps * 32) k_attn_combin
   constexpr int VC = DP / 32;
   constexpr int VW = VC < 4 ? VC : 4;
   constexpr int kRowsCta = kWarps == 1 ? 4 : 1;
+  constexpr int kFlight = DP > 128 ? 4 : 8;
   __shared__ float s_o[kWarps > 1 ? kWarps : 1][DP];
   __shared__ float2 s_ml[kWarps > 1 ? kWarps : 1];
   const AttnArgs& a = c.own;
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
   const int64_t row = (int64_t)blockIdx.x * kRowsCta + (kWarps == 1 ? wid : 0);
-  griddep_wait();
   if (row >= (int64_t)a.T * a.hq) return;  // uniform over a row's warps
   const int t = (int)row / a.hq, hq = (int)row - t * a.hq;
   const int h = hq / a.group, g = hq - h * a.group;
-  const int b = a.q_start ? a.token_seq[t] : t;
+  // Where the pieces are: few rows work it out from the lengths while the
+  // kernels before are still at it; many rows read what those wrote.
+  int b;
+  int64_t unit0 = 0, units = 0;
+  if (kWarps > 1) {
+    b = a.q_start ? seq_of(a, t) : t;
+    const int seg = b + (a.lead > 0);
+    for (int i0 = 0; i0 < segments(a); i0 += 32) {
+      const int64_t v = seg_units<MR>(a, i0 + lane);
+      units += v;
+      if (i0 + lane < seg) unit0 += v;
+    }
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) {
+      unit0 += __shfl_xor_sync(0xffffffffu, unit0, d);
+      units += __shfl_xor_sync(0xffffffffu, units, d);
+    }
+    griddep_wait();
+  } else {
+    griddep_wait();
+    b = a.q_start ? a.token_seq[t] : t;
+    if (b >= 0) unit0 = a.seg_unit[b + (a.lead > 0)];
+    units = a.seg_unit[segments(a)];
+  }
   PieceList po{}, pp{};
   if (b >= 0) {
-    const SeqInfo s = seq_info(a, b);
-    const int us = key_units(a, s), rts = row_tiles<MR>(a, s);
+    const Segment s = segment(a, b + (a.lead > 0));
+    const int us = key_units(s), rts = row_tiles<MR>(a, s);
     AttnSplit sp;
-    sp.units = a.seq_unit[a.B];
+    sp.units = units;
     sp.ranges = min(c.own_warps, sp.units);
     const int r = (t - s.q0) * a.group + g;
-    po = piece_list(sp, a.seq_unit[b] + ((int64_t)h * rts + r / MR) * us, us, r % MR);
+    po = piece_list(sp, unit0 + ((int64_t)h * rts + r / MR) * us, us, r % MR);
     if (po.whole && a.direct) return;  // written by the first kernel
     if (c.has_pre) {
       const int rp = t * a.group + g, rt = rp / c.pre_mr;
-      pp = piece_list(c.pre_split, ((int64_t)h * c.pre_rts + rt) * c.pre_us, c.pre_us, rp - rt * c.pre_mr);
+      pp = piece_list(c.tiles ? c.pre_split : sp, ((int64_t)h * c.pre_rts + rt) * c.pre_us, c.pre_us,
+                      rp - rt * c.pre_mr);
     }
   }
   const int total = po.n + pp.n;
@@ -791,22 +811,30 @@ __global__ void __launch_bounds__(kWarps == 1 ? 128 : kWarps * 32) k_attn_combin
 #pragma unroll
     for (int q = 0; q < VC; ++q) o[q] *= fo;
     const int n = min(32, hi - c0);
-#pragma unroll 4
-    for (int k = 0; k < n; ++k) {
-      const float* p = reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(src), k));
-      const float f = __shfl_sync(0xffffffffu, w, k);
+    for (int k0 = 0; k0 < n; k0 += kFlight) {  // kFlight pieces' loads at once
+      float v[kFlight][VC];
 #pragma unroll
-      for (int q = 0; q < VC; q += VW) {
-        const int d = q * 32 + lane * VW;
-        if (d < a.dim) {
+      for (int k = 0; k < kFlight; ++k) {
+        const float* p = reinterpret_cast<const float*>(
+            __shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(src), min(k0 + k, n - 1)));
+#pragma unroll
+        for (int q = 0; q < VC; q += VW) {
+          const int d = q * 32 + lane * VW;
           if constexpr (VW == 4) {
-            const float4 v = *reinterpret_cast<const float4*>(p + d);
-            o[q] += f * v.x; o[q + 1] += f * v.y; o[q + 2] += f * v.z; o[q + 3] += f * v.w;
+            const float4 x = d < a.dim ? *reinterpret_cast<const float4*>(p + d) : make_float4(0.f, 0.f, 0.f, 0.f);
+            v[k][q] = x.x; v[k][q + 1] = x.y; v[k][q + 2] = x.z; v[k][q + 3] = x.w;
           } else {
-            const float2 v = *reinterpret_cast<const float2*>(p + d);
-            o[q] += f * v.x; o[q + 1] += f * v.y;
+            const float2 x = d < a.dim ? *reinterpret_cast<const float2*>(p + d) : make_float2(0.f, 0.f);
+            v[k][q] = x.x; v[k][q + 1] = x.y;
           }
         }
+      }
+#pragma unroll
+      for (int k = 0; k < kFlight; ++k) {
+        const float f = __shfl_sync(0xffffffffu, w, min(k0 + k, n - 1));
+        if (k0 + k < n)
+#pragma unroll
+          for (int q = 0; q < VC; ++q) o[q] += f * v[k][q];
       }
     }
   }
@@ -859,69 +887,80 @@ __global__ void __launch_bounds__(kWarps == 1 ? 128 : kWarps * 32) k_attn_combin
 constexpr int kTileMinRows = 32;
 
 struct Plan {
-  int dp, mr, warps_cta, smem;
-  int own_grid, pre_grid;
+  int dp, mr, smem;
+  int own_grid, tile_grid;
   int inline_prefix; // each sequence reads the prefix with its own keys
-  int has_pre;       // the prefix has a launch of its own,
+  int has_pre;       // the prefix is a segment of its own,
   int tiles;         // on the tensor cores
-  int pre_mr, pre_unit;
-  int64_t rows;      // T * hq
-  size_t off_piece, off_piece_ml, off_home, off_home_ml, off_seq, off_tok;
-  size_t off_ppiece, off_ppiece_ml, off_phome, off_phome_ml;
+  int tile_mr;
+  int64_t rows;      // T * hq: of the output
+  size_t off_piece, off_piece_ml, off_home, off_home_ml, off_seg, off_tok;
+  size_t off_tpiece, off_tpiece_ml, off_phome, off_phome_ml;
   size_t bytes;
 };
 
+// Shared memory and rows a warp of the kernel that takes this problem.
+void kernel_shape(const AttnProblem& p, Plan* pl) {
+  pl->dp = p.c.dim <= 64 ? 64 : (p.c.dim <= 128 ? 128 : 256);
+  if (p.c.dtype != WR_DTYPE_F32) {
+    pl->mr = 16;
+    pl->smem = pl->dp == 64 ? StreamCfg<64>::kSmem : pl->dp == 128 ? StreamCfg<128>::kSmem : StreamCfg<256>::kSmem;
+    return;
+  }
+  // 8 rows a warp where the sequences have more than 4 (twice the products
+  // for a key read); a sequence with 1 row wastes 3 of 4 rather than 7 of 8.
+  pl->mr = (int64_t)p.T * (p.hq / p.c.hkv) > 4 * (int64_t)p.B ? 8 : 4;
+  if (pl->mr == 8)
+    pl->smem = pl->dp == 64 ? StreamF32Cfg<64, 8>::kSmem : pl->dp == 128 ? StreamF32Cfg<128, 8>::kSmem
+                                                                          : StreamF32Cfg<256, 8>::kSmem;
+  else
+    pl->smem = pl->dp == 64 ? StreamF32Cfg<64, 4>::kSmem : pl->dp == 128 ? StreamF32Cfg<128, 4>::kSmem
+                                                                          : StreamF32Cfg<256, 4>::kSmem;
+}
+
 Plan make_plan(const AttnProblem& p) {
   Plan pl{};
-  const bool f32 = p.c.dtype == WR_DTYPE_F32;
-  pl.dp = p.c.dim <= 64 ? 64 : (p.c.dim <= 128 ? 128 : 256);
-  pl.mr = f32 ? 8 : 16;
-  pl.warps_cta = kStreamWarps;
-  pl.smem = f32 ? (pl.dp == 64 ? StreamF32Cfg<64>::kSmem : pl.dp == 128 ? StreamF32Cfg<128>::kSmem : StreamF32Cfg<256>::kSmem)
-                : (pl.dp == 64 ? StreamCfg<64>::kSmem : pl.dp == 128 ? StreamCfg<128>::kSmem : StreamCfg<256>::kSmem);
+  kernel_shape(p, &pl);
   const int fit = 227 * 1024 / (pl.smem + 2048);
   const int per_sm = fit < 1 ? 1 : (fit > 16 ? 16 : fit);
   const int64_t most = (int64_t)device_sm_count() * per_sm;
   const int group = p.hq / p.c.hkv;
-  pl.rows = (int64_t)p.T * p.hq;  // of the output
+  pl.rows = (int64_t)p.T * p.hq;
   pl.inline_prefix = p.prefix_len > 0 && p.B == 1;
   pl.has_pre = p.prefix_len > 0 && !pl.inline_prefix;
   const int64_t group_rows = (int64_t)p.T * group;  // rows that meet the prefix, a key head
   pl.tiles = pl.has_pre && group_rows > kTileMinRows && prefix_tiles_ok(p);
-  pl.pre_mr = pl.tiles ? (group_rows > 128 ? 256 : 128) : pl.mr;
-  pl.pre_unit = pl.tiles ? kPrefixUnit : kUnitTokens;
   // An upper bound of the units: the lengths are on the device.
   const int64_t keys = (int64_t)p.table_width * p.c.page_size + (pl.inline_prefix ? p.prefix_len : 0);
-  const int64_t tiles = ((int64_t)p.T * group + pl.mr - 1) / pl.mr + (p.B > 0 ? p.B : 0);
-  const int64_t units = (tiles * p.c.hkv) * ((keys + kUnitTokens - 1) / kUnitTokens + 1);
-  const int64_t ctas = (units + pl.warps_cta - 1) / pl.warps_cta;
-  pl.own_grid = (int)(ctas < most ? (ctas < 1 ? 1 : ctas) : most);
+  const int64_t tiles = (group_rows + pl.mr - 1) / pl.mr + (p.B > 0 ? p.B : 0);
+  int64_t units = (tiles * p.c.hkv) * ((keys + kUnitTokens - 1) / kUnitTokens + 1);
+  if (pl.has_pre && !pl.tiles) units += tiles * p.c.hkv * ((p.prefix_len + kUnitTokens - 1) / kUnitTokens);
+  pl.own_grid = (int)(units < most ? (units < 1 ? 1 : units) : most);
   size_t at = 0;
   auto take = [&](size_t n) {
     const size_t o = at;
     at += (n + 255) & ~(size_t)255;
     return o;
   };
-  const size_t own_rows = (size_t)pl.own_grid * pl.warps_cta * 2 * pl.mr;
+  const size_t own_rows = (size_t)pl.own_grid * 2 * pl.mr;
   pl.off_piece = take(own_rows * p.c.dim * 4);
   pl.off_piece_ml = take(own_rows * 8);
+  pl.off_seg = take((size_t)(p.B + 2) * 8);
+  pl.off_tok = take((size_t)(p.q_start ? p.T : 0) * 4);
   if (pl.has_pre) {
     pl.off_home = take((size_t)pl.rows * p.c.dim * 4);
     pl.off_home_ml = take((size_t)pl.rows * 8);
-  }
-  pl.off_seq = take((size_t)(p.B + 1) * 8);
-  pl.off_tok = take((size_t)(p.q_start ? p.T : 0) * 4);
-  if (pl.has_pre) {
-    const int64_t pu = (int64_t)p.c.hkv * ((group_rows + pl.pre_mr - 1) / pl.pre_mr) *
-                       ((p.prefix_len + pl.pre_unit - 1) / pl.pre_unit);
-    const int ways = pl.tiles ? 1 : pl.warps_cta;  // ranges a CTA
-    const int64_t pc = (pu + ways - 1) / ways, cap = pl.tiles ? device_sm_count() : most;
-    pl.pre_grid = (int)(pc < cap ? pc : cap);
-    const size_t pre_rows = (size_t)pl.pre_grid * ways * 2 * pl.pre_mr;
-    pl.off_ppiece = take(pre_rows * p.c.dim * 4);
-    pl.off_ppiece_ml = take(pre_rows * 8);
     pl.off_phome = take((size_t)pl.rows * p.c.dim * 4);
     pl.off_phome_ml = take((size_t)pl.rows * 8);
+  }
+  if (pl.tiles) {
+    pl.tile_mr = group_rows > 128 ? 256 : 128;
+    const int64_t tu = (int64_t)p.c.hkv * ((group_rows + pl.tile_mr - 1) / pl.tile_mr) *
+                       ((p.prefix_len + kPrefixUnit - 1) / kPrefixUnit);
+    pl.tile_grid = (int)(tu < device_sm_count() ? tu : device_sm_count());
+    const size_t tile_rows = (size_t)pl.tile_grid * 2 * pl.tile_mr;
+    pl.off_tpiece = take(tile_rows * p.c.dim * 4);
+    pl.off_tpiece_ml = take(tile_rows * 8);
   }
   pl.bytes = at;
   return pl;
@@ -941,7 +980,7 @@ cudaError_t launch_one(K kernel, int64_t grid, int threads, int smem, bool pdl, 
   cfg.attrs = at;
   cfg.numAttrs = pdl ? 1 : 0;
   void* ptrs[1] = {const_cast<void*>(args)};
-  if (smem > 0) {
+  if (smem > 48 * 1024) {
     const cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel),
                                                cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
@@ -949,16 +988,15 @@ cudaError_t launch_one(K kernel, int64_t grid, int threads, int smem, bool pdl, 
   return cudaLaunchKernelExC(&cfg, reinterpret_cast<const void*>(kernel), ptrs);
 }
 
-cudaError_t launch_stream(const Plan& pl, bool f32, const AttnArgs& a, int grid, bool pdl, cudaStream_t s) {
-  const int th = pl.warps_cta * 32;
-  if (f32) {
-    if (pl.dp == 64) return launch_one(k_attn_stream_f32<64>, grid, th, pl.smem, pdl, s, &a);
-    if (pl.dp == 128) return launch_one(k_attn_stream_f32<128>, grid, th, pl.smem, pdl, s, &a);
-    return launch_one(k_attn_stream_f32<256>, grid, th, pl.smem, pdl, s, &a);
-  }
-  if (pl.dp == 64) return launch_one(k_attn_stream<64>, grid, th, pl.smem, pdl, s, &a);
-  if (pl.dp == 128) return launch_one(k_attn_stream<128>, grid, th, pl.smem, pdl, s, &a);
-  return launch_one(k_attn_stream<256>, grid, th, pl.smem, pdl, s, &a);
+cudaError_t launch_stream(const Plan& pl, bool f32, const AttnArgs& a, bool pdl, cudaStream_t s) {
+  auto go = [&](auto kernel) { return launch_one(kernel, pl.own_grid, 32, pl.smem, pdl, s, &a); };
+  if (f32 && pl.mr == 8)
+    return pl.dp == 64 ? go(k_attn_stream_f32<64, 8>) : pl.dp == 128 ? go(k_attn_stream_f32<128, 8>)
+                                                                     : go(k_attn_stream_f32<256, 8>);
+  if (f32)
+    return pl.dp == 64 ? go(k_attn_stream_f32<64, 4>) : pl.dp == 128 ? go(k_attn_stream_f32<128, 4>)
+                                                                     : go(k_attn_stream_f32<256, 4>);
+  return pl.dp == 64 ? go(k_attn_stream<64>) : pl.dp == 128 ? go(k_attn_stream<128>) : go(k_attn_stream<256>);
 }
 
 template <typename T, int MR, int W>
@@ -988,56 +1026,60 @@ wr_status_t launch_attn(const AttnProblem& p, void* ws, cudaStream_t stream) {
   a.T = p.T; a.B = p.B; a.hq = p.hq; a.hkv = p.c.hkv; a.group = p.hq / p.c.hkv; a.dim = p.c.dim;
   a.table_width = p.table_width;
   a.prefix = pl.inline_prefix ? p.prefix_len : 0;
-  a.own = 1;
+  a.lead = pl.has_pre && !pl.tiles ? p.prefix_len : 0;
   a.direct = !pl.has_pre;
   a.scale_log2 = p.scale * kLog2e;
   a.part.piece = reinterpret_cast<float*>(base + pl.off_piece);
   a.part.piece_ml = reinterpret_cast<float2*>(base + pl.off_piece_ml);
   a.home = reinterpret_cast<float*>(base + pl.off_home);
   a.home_ml = reinterpret_cast<float2*>(base + pl.off_home_ml);
-  a.seq_unit = reinterpret_cast<int64_t*>(base + pl.off_seq);
+  a.lead_home = reinterpret_cast<float*>(base + pl.off_phome);
+  a.lead_home_ml = reinterpret_cast<float2*>(base + pl.off_phome_ml);
+  a.seg_unit = reinterpret_cast<int64_t*>(base + pl.off_seg);
   a.token_seq = reinterpret_cast<int32_t*>(base + pl.off_tok);
   a.out = p.out; a.lse = p.lse;
   CombineArgs c{};
   c.own = a;
-  c.own_warps = (int64_t)pl.own_grid * pl.warps_cta;
-  cudaError_t e;
+  c.own_warps = pl.own_grid;
   if (pl.has_pre) {
-    AttnArgs x = a;
-    x.B = 1; x.own = 0; x.prefix = p.prefix_len; x.direct = 0; x.q_start = nullptr;
-    x.part.piece = reinterpret_cast<float*>(base + pl.off_ppiece);
-    x.part.piece_ml = reinterpret_cast<float2*>(base + pl.off_ppiece_ml);
-    x.home = reinterpret_cast<float*>(base + pl.off_phome);
-    x.home_ml = reinterpret_cast<float2*>(base + pl.off_phome_ml);
     c.has_pre = 1;
-    c.pre = x.part;
-    c.pre_home = x.home;
-    c.pre_home_ml = x.home_ml;
-    c.pre_mr = pl.pre_mr;
-    c.pre_rts = (int)(((int64_t)p.T * a.group + pl.pre_mr - 1) / pl.pre_mr);
-    c.pre_us = (p.prefix_len + pl.pre_unit - 1) / pl.pre_unit;
-    c.pre_split.units = (int64_t)a.hkv * c.pre_rts * c.pre_us;
-    const int64_t ranges = (int64_t)pl.pre_grid * (pl.tiles ? 1 : pl.warps_cta);
-    c.pre_split.ranges = ranges < c.pre_split.units ? ranges : c.pre_split.units;
-    if (pl.tiles) {
-      const wr_status_t st = launch_attn_prefix(p, x, pl.pre_mr, pl.pre_grid, stream);
-      if (st != WR_OK) return st;
-    } else {
-      e = launch_stream(pl, f32, x, pl.pre_grid, false, stream);
-      if (e != cudaSuccess) return cuda_fail(e, "shared_prefix_attention (prefix) launch");
-    }
+    c.tiles = pl.tiles;
+    c.pre = a.part;
+    c.pre_home = a.lead_home;
+    c.pre_home_ml = a.lead_home_ml;
+    c.pre_mr = pl.tiles ? pl.tile_mr : pl.mr;
+    const int unit = pl.tiles ? kPrefixUnit : kUnitTokens;
+    c.pre_rts = (int)(((int64_t)p.T * a.group + c.pre_mr - 1) / c.pre_mr);
+    c.pre_us = (p.prefix_len + unit - 1) / unit;
   }
-  e = launch_stream(pl, f32, a, pl.own_grid, pl.has_pre, stream);
+  cudaError_t e;
+  if (pl.tiles) {
+    AttnArgs x = a;
+    x.prefix = p.prefix_len;
+    x.part.piece = reinterpret_cast<float*>(base + pl.off_tpiece);
+    x.part.piece_ml = reinterpret_cast<float2*>(base + pl.off_tpiece_ml);
+    x.home = a.lead_home;
+    x.home_ml = a.lead_home_ml;
+    c.pre = x.part;
+    c.pre_split.units = (int64_t)a.hkv * c.pre_rts * c.pre_us;
+    c.pre_split.ranges = pl.tile_grid < c.pre_split.units ? pl.tile_grid : c.pre_split.units;
+    const wr_status_t st = launch_attn_prefix(p, x, pl.tile_mr, pl.tile_grid, stream);
+    if (st != WR_OK) return st;
+  }
+  e = launch_stream(pl, f32, a, pl.tiles, stream);
   if (e != cudaSuccess) return cuda_fail(e, "shared_prefix_attention launch");
   // Few rows: 8 warps a row read its many pieces; many rows: a warp each.
   const bool wide = pl.rows <= (int64_t)device_sm_count() * 8;
   const int64_t grid = wide ? pl.rows : (pl.rows + 3) / 4;
-  if (f32)
+  if (!f32)
+    e = wide ? launch_combine_dp<uint16_t, 16, 8>(pl.dp, c, grid, stream)
+             : launch_combine_dp<uint16_t, 16, 1>(pl.dp, c, grid, stream);
+  else if (pl.mr == 8)
     e = wide ? launch_combine_dp<float, 8, 8>(pl.dp, c, grid, stream)
              : launch_combine_dp<float, 8, 1>(pl.dp, c, grid, stream);
   else
-    e = wide ? launch_combine_dp<uint16_t, 16, 8>(pl.dp, c, grid, stream)
-             : launch_combine_dp<uint16_t, 16, 1>(pl.dp, c, grid, stream);
+    e = wide ? launch_combine_dp<float, 4, 8>(pl.dp, c, grid, stream)
+             : launch_combine_dp<float, 4, 1>(pl.dp, c, grid, stream);
   return e == cudaSuccess ? WR_OK : cuda_fail(e, "shared_prefix_attention (join) launch");
 }
 

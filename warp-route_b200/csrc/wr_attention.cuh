@@ -56,14 +56,17 @@ struct AttnArgs {
   const int32_t* prefix_pages;
   int num_pages, page_size, page_shift;  // page_shift < 0: not a power of two
   int T, B, hq, hkv, group, dim, table_width;
-  int prefix;        // tokens of the shared prefix that these segments read
-  int own;           // 0: the segment is the prefix with all T tokens' rows
-  int direct;        // no other segment adds to these rows: whole tiles are final
+  int prefix;        // keys of the shared prefix that each sequence reads with its own
+  int lead;          // > 0: segment 0 is the prefix of that many keys with all T tokens'
+                     // rows, and the sequences come behind it
+  int direct;        // nothing else adds to the sequences' rows: whole tiles are final
   float scale_log2;
   AttnPartials part;
   float* home;       // [T * hq][dim]
   float2* home_ml;   // [T * hq]
-  int64_t* seq_unit; // [B + 1] first unit of each sequence, [B]: units
+  float* lead_home;  // the same of segment 0
+  float2* lead_home_ml;
+  int64_t* seg_unit; // [segments + 1] first unit of each segment, and all of them
   int32_t* token_seq;  // [T] sequence of each token, -1: none
   void* out;
   float* lse;
@@ -82,32 +85,34 @@ WR_DEVINL void split_page(int j, int page_size, int shift, int& page, int& row) 
   row = j - (shift >= 0 ? page << shift : page * page_size);
 }
 
-struct SeqInfo {
-  int q0, nq, len;  // first token, tokens asked, own keys in the cache
+struct Segment {
+  int q0, nq;  // first token, tokens asked
+  int len;     // own keys in the cache
+  int prefix;  // keys of the prefix before them
 };
+__host__ __device__ inline int segments(const AttnArgs& a) { return a.B + (a.lead > 0); }
 // q_start and lens come from device memory: whatever they hold, the values
 // used lie inside q and the table.
-WR_DEVINL SeqInfo seq_info(const AttnArgs& a, int b) {
-  SeqInfo s;
-  if (!a.own) {
-    s.q0 = 0; s.nq = a.T; s.len = 0;
+WR_DEVINL Segment segment(const AttnArgs& a, int i) {
+  Segment s;
+  if (a.lead > 0 && i-- == 0) {
+    s.q0 = 0; s.nq = a.T; s.len = 0; s.prefix = a.lead;
     return s;
   }
   if (a.q_start) {
-    const int lo = min(max(__ldg(a.q_start + b), 0), a.T);
-    const int hi = min(max(__ldg(a.q_start + b + 1), lo), a.T);
+    const int lo = min(max(__ldg(a.q_start + i), 0), a.T);
+    const int hi = min(max(__ldg(a.q_start + i + 1), lo), a.T);
     s.q0 = lo; s.nq = hi - lo;
   } else {
-    s.q0 = b; s.nq = 1;
+    s.q0 = i; s.nq = 1;
   }
-  s.len = (int)min((int64_t)max(__ldg(a.lens + b), 0), (int64_t)a.table_width * a.page_size);
+  s.len = (int)min((int64_t)max(__ldg(a.lens + i), 0), (int64_t)a.table_width * a.page_size);
+  s.prefix = a.prefix;
   return s;
 }
 template <int MR>
-WR_DEVINL int row_tiles(const AttnArgs& a, const SeqInfo& s) { return (s.nq * a.group + MR - 1) / MR; }
+WR_DEVINL int row_tiles(const AttnArgs& a, const Segment& s) { return (s.nq * a.group + MR - 1) / MR; }
 // A segment without keys still has one unit, so that its rows are written.
-WR_DEVINL int key_units(const AttnArgs& a, const SeqInfo& s) {
-  return max(1, (a.prefix + s.len + kUnitTokens - 1) / kUnitTokens);
-}
+WR_DEVINL int key_units(const Segment& s) { return max(1, (s.prefix + s.len + kUnitTokens - 1) / kUnitTokens); }
 
 }  // namespace wr
