@@ -133,7 +133,7 @@ size_t attn_workspace_bytes(const AttnProblem& p);
 wr_status_t launch_attn(const AttnProblem& p, void* ws, cudaStream_t stream);
 
 // ---- sampling (wr_sample.cu) ----
-constexpr int kSampleMaxVocab = 8 * 512 * 64;  // what a cluster of 8 CTAs of 512 threads keeps, 64 values a thread
+constexpr int kSampleMaxVocab = 1 << 18;  // sums of 2^45 stay below 2^63
 struct SampleProblem {
   int64_t rows;
   int vocab, dtype;

@@ -12,19 +12,24 @@
 // bits and held as a whole number of 2^-45: sums of whole numbers do not
 // depend on their order, whatever order atomics come in.
 //
-// A row belongs to one cluster of 1 to 8 CTAs, which reads it once and keeps
-// it in shared memory.  The border of the first k, and that of the mass
-// top_p, are found without sorting the row: a histogram (count and mass) of
-// the values over 2048 bins, even over [min, max] of the row, tells which bin
-// a border lies in; that bin's values, few as a rule, are gathered by one CTA,
-// sorted and cut exactly.  A bin with more values than fit there (rows of many
-// equal values) is binned again by key until one value is left.  HBM is read
-// once; what bounds the kernel is the exchanges between the CTAs for few rows
-// and the 64-bit arithmetic of the weights for many.
+// A row belongs to one cluster of 1 to 8 CTAs: as many as run at once for all
+// rows (two an SM), and enough to keep the row in shared memory with two CTAs
+// an SM (256 rows of 131072: 8 CTAs a row 240 us, one that reads the row again
+// for each pass 345 us); only what 8 CTAs do not hold is read again for each
+// pass, from L2 as a rule.  The border of the first k, and that of the mass
+// top_p, are found without sorting the row: a histogram of the values over
+// 1024 bins, even over [min, max] of the row, tells which bin a border lies
+// in, for the first k exactly, for the mass by count times weight of the mean of
+// a bin, after which one pass over the exact weights says which of the three
+// bins around it it is (no atomics on masses: they took longer than the
+// weights).  That bin's values, few as a rule, are gathered by one CTA, sorted
+// and cut exactly; with a short top_k everything down to its border goes there,
+// and that CTA ends the row.  A bin with more values than fit there (rows of
+// many equal values) is binned again by key until one value is left.  What
+// bounds the kernel is the chain of passes and exchanges for few rows and the
+// 64-bit arithmetic of the weights for many.
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
-
-#include <utility>
 
 #include "wr_common.cuh"
 #include "wr_internal.h"
@@ -36,12 +41,13 @@ namespace {
 
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
-constexpr int kBins = 2048;
+constexpr int kBins = 1024;
 constexpr int kMaxCluster = 8;
 constexpr int kList = 1024;  // values that one CTA sorts
 constexpr int kTable = 128;  // steps of the exponential's table per factor of two
 // 16 vectors a thread hold kSampleMaxVocab values.
-constexpr int kMaxLevels = 16;
+constexpr int kKeepBytes = 76 * 1024;  // of a row's part in shared memory, at most
+constexpr int kFlight = 4;             // vectors a thread has in flight
 constexpr double kMassOne = 35184372088832.0;  // 2^45: with up to 2^18 values sums stay below 2^63
 constexpr double kMagic = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to a whole number
 constexpr float kNegInf = -__builtin_huge_valf();
@@ -79,31 +85,41 @@ WR_DEVINL bool in_cut(const Cut& c, uint32_t key, int idx) {
 
 struct Shared {
   uint32_t count[kBins];
-  // Masses in three parts of 17, 17 and 12 bits, each added with a native
-  // 32-bit atomic (a 64-bit one is a loop of compare and swap): a CTA has at
-  // most 2^15 values, so no part passes 32 bits.
-  uint32_t mass[3][kBins];
+  // Masses in parts of 14 bits, each added with a native 32-bit atomic (a
+  // 64-bit one is a loop of compare and swap): at most 2^18 values, so no part
+  // passes 32 bits.
+  uint32_t mass[4][kBins];
   uint64_t list[kList];  // (key, ~index); rank 0's alone is used
   double table[kTable];
   uint64_t warp64[kWarps];
   uint64_t warp64b[kWarps];
   // written by every rank of the cluster into every rank's copy
   uint64_t all_a[2][kMaxCluster], all_b[2][kMaxCluster];
+  uint64_t all_w[kMaxCluster][5];
+  uint64_t warp_w[kWarps][2];
+  uint64_t window[3];
+  uint32_t rank[256];
   uint64_t found[2][4];
   uint32_t listed;
 };
 
 WR_DEVINL void add_mass(Shared& s, int bin, uint64_t m) {
-  const uint32_t a = (uint32_t)m & 0x1ffffu, b = (uint32_t)(m >> 17) & 0x1ffffu, c = (uint32_t)(m >> 34);
-  if (a) atomicAdd(&s.mass[0][bin], a);
-  if (b) atomicAdd(&s.mass[1][bin], b);
-  if (c) atomicAdd(&s.mass[2][bin], c);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t part = (uint32_t)(m >> (14 * i)) & 0x3fffu;
+    if (part) atomicAdd(&s.mass[i][bin], part);
+  }
 }
+static_assert(kSampleMaxVocab <= 1 << 18, "parts of the masses");
 WR_DEVINL void clear_bins(Shared& s) {
-  for (int i = threadIdx.x; i < kBins; i += kThreads)
-    s.count[i] = s.mass[0][i] = s.mass[1][i] = s.mass[2][i] = 0;
+  for (int i = threadIdx.x; i < kBins; i += kThreads) {
+    s.count[i] = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) s.mass[j][i] = 0;
+  }
 }
-static_assert(kMaxLevels * kThreads * 4 <= 1 << 15, "parts of the masses");
+
+static_assert(sizeof(Shared) % 16 == 0 && sizeof(Shared) + kKeepBytes < 113 * 1024, "two CTAs an SM");
 
 struct Row {
   float max;
@@ -133,10 +149,17 @@ WR_DEVINL uint64_t mass_of(double w) {
   return (uint64_t)__double_as_longlong(fma(w, kMassOne, 4503599627370496.0)) & 0xfffffffffffffull;
 }
 
-// This CTA's part of the row in shared memory: vector l of thread t holds the
-// values 4 * ((rank * levels + l) * kThreads + t) .. + 3 of the row, -inf
-// behind its end.  A thread touches its own vectors only.
-// V: four values as they came, float4 or uint2 (bf16), NaN and -0 replaced.
+// This CTA's part of the row: vector l of thread t is the four values from
+// 4 * ((rank * levels + l) * kThreads + t) on, -inf behind the row's end, NaN
+// as -inf and -0 as 0 (equal numbers have equal keys).  kKeep: in shared
+// memory, as they came (float4 or uint2), where a thread touches its own
+// vectors only; else they are read from the row each time.
+template <typename T>
+struct Four;
+template <>
+struct Four<float> { using V = float4; };
+template <>
+struct Four<uint16_t> { using V = uint2; };
 WR_DEVINL void widen4(const float4& v, float (&f)[4]) { f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w; }
 WR_DEVINL void widen4(const uint2& v, float (&f)[4]) {
   f[0] = bf16lo(v.x); f[1] = bf16hi(v.x);
@@ -147,20 +170,54 @@ WR_DEVINL void pack4(const float (&f)[4], uint2& v) {  // exact: they came from 
   v.x = (__float_as_uint(f[0]) >> 16) | (__float_as_uint(f[1]) & 0xffff0000u);
   v.y = (__float_as_uint(f[2]) >> 16) | (__float_as_uint(f[3]) & 0xffff0000u);
 }
-template <typename V>
+template <typename T, bool kKeep>
 struct Slice {
-  V* v;
-  int levels, rank;
+  using V = typename Four<T>::V;
+  V* kept;
+  const T* row;
+  int levels, rank, vocab;
+  bool vec;
   WR_DEVINL int index(int l) const { return ((rank * levels + l) * kThreads + (int)threadIdx.x) * 4; }
-  template <typename F>
-  WR_DEVINL void each(F f) const {
-#pragma unroll 1
-    for (int l = 0; l < levels; ++l) {
-      float q[4];
-      widen4(v[l * kThreads + threadIdx.x], q);
-      const int i = index(l);
+  WR_DEVINL V fetch(int l) const {  // from the row
+    const int j = index(l);
+    if (vec && j + 3 < vocab) return __ldg(reinterpret_cast<const V*>(row + j));
+    float f[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) f(q[e], i + e);
+    for (int e = 0; e < 4; ++e) f[e] = j + e < vocab ? load_scalar<T>(row, j + e) : kNegInf;
+    V v;
+    pack4(f, v);
+    return v;
+  }
+  static WR_DEVINL void clean(float (&f)[4]) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) f[e] = f[e] != f[e] ? kNegInf : f[e] + 0.f;
+  }
+  WR_DEVINL void four(int l, float (&f)[4]) const {
+    widen4(kKeep ? kept[l * kThreads + threadIdx.x] : fetch(l), f);
+    if (!kKeep) clean(f);
+  }
+  // f(value, index) for each value; kStore: reads the row and keeps it.
+  template <bool kStore = false, typename F>
+  WR_DEVINL void each(F f) const {
+    constexpr bool kRead = !kKeep || kStore;
+    constexpr int U = kRead ? kFlight : 1;
+#pragma unroll 1
+    for (int l0 = 0; l0 < levels; l0 += U) {
+      V v[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (l0 + u < levels) v[u] = kRead ? fetch(l0 + u) : kept[(l0 + u) * kThreads + threadIdx.x];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (l0 + u >= levels) continue;
+        float q[4];
+        widen4(v[u], q);
+        if (kRead) clean(q);
+        if (kKeep && kStore) pack4(q, kept[(l0 + u) * kThreads + threadIdx.x]);
+        const int i = index(l0 + u);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) f(q[e], i + e);
+      }
     }
   }
 };
@@ -184,6 +241,9 @@ WR_DEVINL uint64_t warp_inclusive(uint64_t v, int lane) {
   return v;
 }
 
+WR_DEVINL void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+WR_DEVINL void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+
 // The cluster and what its exchanges go through.  Each exchange writes into
 // the copy of all_* or found that `par` names and flips it: a rank can write
 // into a copy again only after a cluster barrier that every rank reaches after
@@ -192,6 +252,11 @@ struct Group {
   cg::cluster_group cl;
   Shared* s;
   int n, me, par;
+
+  WR_DEVINL void sync() {
+    if (n == 1) __syncthreads(); else cl.sync();
+  }
+  WR_DEVINL Shared* of(int rank) { return n == 1 ? s : cl.map_shared_rank(s, rank); }
 
   // Two values of the CTA's threads reduced over the cluster (fa, fb
   // associative and commutative); every thread gets both.
@@ -214,12 +279,12 @@ struct Group {
         b = fb(b, __shfl_xor_sync(0xffffffffu, b, d));
       }
       if (lane < n) {
-        Shared* o = cl.map_shared_rank(s, lane);
+        Shared* o = of(lane);
         o->all_a[par][me] = a;
         o->all_b[par][me] = b;
       }
     }
-    cl.sync();
+    sync();
     a = s->all_a[par][0];
     b = s->all_b[par][0];
     for (int i = 1; i < n; ++i) {
@@ -227,6 +292,34 @@ struct Group {
       b = fb(b, s->all_b[par][i]);
     }
     par ^= 1;
+  }
+
+  // Over the cluster: the sums of two values of the threads, and of the
+  // window's three (complete at the call's barrier).
+  WR_DEVINL void reduce_window(uint64_t (&v)[5]) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      v[i] = warp_reduce(v[i], Add());
+      if (lane == 0) s->warp_w[warp][i] = v[i];
+    }
+    __syncthreads();
+    if (threadIdx.x < 5 * n) {
+      const int i = threadIdx.x % 5;
+      uint64_t t = 0;
+      if (i < 2) {
+        for (int w = 0; w < kWarps; ++w) t += s->warp_w[w][i];
+      } else {
+        t = s->window[i - 2];
+      }
+      of(threadIdx.x / 5)->all_w[me][i] = t;
+    }
+    sync();
+#pragma unroll
+    for (int i = 0; i < 5; ++i) {
+      v[i] = 0;
+      for (int r = 0; r < n; ++r) v[i] += s->all_w[r][i];
+    }
   }
 
   // This rank's share of the bins, kBins / n of them from first_bin(), one to
@@ -239,8 +332,11 @@ struct Group {
   WR_DEVINL int per() const { return (share() + kThreads - 1) / kThreads; }
   WR_DEVINL int first_bin() const { return me * share() + (int)threadIdx.x * per(); }
 
-  // After the histograms are whole (a cluster barrier).  Both sums at once.
-  WR_DEVINL void sum_bins(Bins& c, Bins& m) {
+  // After the histograms are whole (a cluster barrier).  Both sums at once:
+  // counts and masses (kMass), or counts and what of_bin makes of a bin, its
+  // count and its values' summed places inside it (kept in mass[0]).
+  template <bool kMass, typename F>
+  WR_DEVINL void sum_bins(Bins& c, Bins& m, F of_bin) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     uint64_t sc = 0, sm = 0;
 #pragma unroll
@@ -248,13 +344,32 @@ struct Group {
       c.v[e] = m.v[e] = 0;
       if (e < per() && (int)threadIdx.x * per() + e < share()) {
         const int b = first_bin() + e;
-#pragma unroll
-        for (int r = 0; r < kMaxCluster; ++r)
-          if (r < n) {
-            const Shared* o = cl.map_shared_rank(s, r);
-            c.v[e] += o->count[b];
-            m.v[e] += o->mass[0][b] + ((uint64_t)o->mass[1][b] << 17) + ((uint64_t)o->mass[2][b] << 34);
+        if constexpr (kMass) {
+          for (int r = 0; r < n; ++r) {
+            const Shared* o = of(r);
+            for (int i = 0; i < 4; ++i) m.v[e] += (uint64_t)o->mass[i][b] << (14 * i);
           }
+        } else {
+          uint32_t offsets = 0;
+          if (n == 1) {
+            c.v[e] = s->count[b];
+            offsets = s->mass[0][b];
+          } else {
+            uint32_t x[kMaxCluster], y[kMaxCluster];  // all at once: each takes some thousand cycles
+#pragma unroll
+            for (int r = 0; r < kMaxCluster; ++r) {
+              const Shared* o = of(r < n ? r : 0);
+              x[r] = o->count[b];
+              y[r] = o->mass[0][b];
+            }
+#pragma unroll
+            for (int r = 0; r < kMaxCluster; ++r) {
+              c.v[e] += r < n ? x[r] : 0;
+              offsets += r < n ? y[r] : 0;
+            }
+          }
+          m.v[e] = c.v[e] ? of_bin(b, (float)c.v[e], (float)offsets) : 0;
+        }
       }
       sc += c.v[e];
       sm += m.v[e];
@@ -278,11 +393,11 @@ struct Group {
       tm += s->warp64b[w];
     }
     if ((int)threadIdx.x < n) {
-      Shared* o = cl.map_shared_rank(s, threadIdx.x);
+      Shared* o = of(threadIdx.x);
       o->all_a[par][me] = tc;
       o->all_b[par][me] = tm;
     }
-    cl.sync();
+    sync();
     c.whole = m.whole = 0;
     for (int r = 0; r < n; ++r) {
       if (r < me) {
@@ -305,7 +420,7 @@ struct Group {
     for (int e = 0; e < 4; ++e) {
       if (x.v[e] && before < target && before + x.v[e] >= target)
         for (int r = 0; r < n; ++r) {
-          Shared* o = cl.map_shared_rank(s, r);
+          Shared* o = of(r);
           o->found[par][0] = (uint64_t)(first_bin() + e);
           o->found[par][1] = before;
           o->found[par][2] = other;
@@ -314,7 +429,7 @@ struct Group {
       before += x.v[e];
       other += y.v[e];
     }
-    cl.sync();
+    sync();
     const int bin = (int)s->found[par][0];
     bx = s->found[par][1];
     by = s->found[par][2];
@@ -324,8 +439,26 @@ struct Group {
   }
 };
 
-// Sorts list[0 .. n) descending (n <= kList), all threads of the CTA.
-__device__ __noinline__ void sort_list(uint64_t* list, int n) {
+// Sorts list[0 .. n) descending (n <= kList), all threads of the CTA.  Up to
+// 256 entries by counting the larger ones (entries differ), a few barriers;
+// more by a bitonic network.  Entries up to the next power of two become 0 in
+// the latter.
+__device__ __noinline__ void sort_list(uint64_t* list, uint32_t* rank, int n) {
+  if (n <= 256) {
+    int size = 32;
+    while (size < n) size *= 2;
+    const int e = threadIdx.x & (size - 1), part = threadIdx.x / size, parts = kThreads / size;
+    if (threadIdx.x < 256) rank[threadIdx.x] = 0;
+    __syncthreads();
+    const uint64_t mine = e < n ? list[e] : 0;
+    uint32_t larger = 0;
+    for (int j = part; j < n; j += parts) larger += list[j] > mine;
+    if (e < n && larger) atomicAdd(&rank[e], larger);
+    __syncthreads();
+    if (part == 0 && e < n) list[rank[e]] = mine;
+    __syncthreads();
+    return;
+  }
   int size = 32;
   while (size < n) size *= 2;
   for (int i = n + threadIdx.x; i < size; i += kThreads) list[i] = 0;
@@ -378,10 +511,10 @@ WR_DEVINL uint64_t cta_before(Shared& s, uint64_t v, uint64_t& whole) {
 
 // The rest of a row whose first top_k all lie in the list (n >= top_k values
 // of it, unsorted): one CTA, two list entries a thread.
-__device__ __noinline__ void finish_list(Shared& s, const Row& row, int n, int top_k, float top_p,
+__device__ __noinline__ void finish_list(Shared& s, const Row row, int n, int top_k, float top_p,
                                          float min_p, float uniform, int64_t* id) {
   constexpr int kPer = kList / kThreads;
-  sort_list(s.list, n);
+  sort_list(s.list, s.rank, n);
   uint64_t entry[kPer], m[kPer], sum = 0, whole;
   bool keep[kPer];
 #pragma unroll
@@ -403,15 +536,21 @@ __device__ __noinline__ void finish_list(Shared& s, const Row& row, int n, int t
       before += m[e];
     }
   }
-  // By index: the list again, its entries (~index, key), the dropped ones 0.
+  // By index: the kept entries again, as (~index, key).
+  uint64_t kept = 0, all;
 #pragma unroll
-  for (int e = 0; e < kPer; ++e) s.list[threadIdx.x * kPer + e] = keep[e] ? (entry[e] << 32) | (entry[e] >> 32) : 0;
+  for (int e = 0; e < kPer; ++e) kept += keep[e];
+  int at = (int)cta_before(s, kept, all);
+#pragma unroll
+  for (int e = 0; e < kPer; ++e)
+    if (keep[e]) s.list[at++] = (entry[e] << 32) | (entry[e] >> 32);
   __syncthreads();
-  sort_list(s.list, n);
+  sort_list(s.list, s.rank, (int)all);
   sum = 0;
 #pragma unroll
   for (int e = 0; e < kPer; ++e) {
-    entry[e] = s.list[threadIdx.x * kPer + e];
+    const int i = threadIdx.x * kPer + e;
+    entry[e] = i < (int)all ? s.list[i] : 0;
     m[e] = entry[e] ? mass_of(weight(row, value_of((uint32_t)entry[e]))) : 0;
     sum += m[e];
   }
@@ -428,8 +567,14 @@ __device__ __noinline__ void finish_list(Shared& s, const Row& row, int n, int t
 // lies before them in the order: the last value whose preceding sum is below
 // target, sums of 1 (kMass false) or of mass.  For bins too full to sort:
 // binned by key until one key is left, whose values go by index.
-template <bool kMass, typename V>
-__device__ __noinline__ Cut find_by_key(Group& g, const Slice<V>& x, const Row& row, const Cut& within,
+// (By value, and `par` back by value: nothing of the kernel's hot loops may
+// have its address taken, or they would read it from memory each time.)
+struct CutPar {
+  Cut cut;
+  int par;
+};
+template <bool kMass, typename X>
+__device__ __noinline__ CutPar find_by_key(Group g, const X x, const Row row, const Cut within,
                                         uint32_t lo, uint32_t hi, uint64_t above, uint64_t target) {
   Shared& s = *g.s;
   while (lo != hi) {
@@ -442,9 +587,9 @@ __device__ __noinline__ Cut find_by_key(Group& g, const Slice<V>& x, const Row& 
       if (k < lo || k > hi || !in_cut(within, k, i)) return;
       add_mass(s, (int)((hi - k) >> shift), kMass ? mass_of(weight(row, f)) : 1);
     });
-    g.cl.sync();
+    g.sync();
     Group::Bins c, m;
-    g.sum_bins(c, m);
+    g.sum_bins<true>(c, m, 0);
     uint64_t before, none, end;
     const int bin = g.find_bin(m, c, target - above, before, none, end);
     above += before;
@@ -474,76 +619,44 @@ __device__ __noinline__ Cut find_by_key(Group& g, const Slice<V>& x, const Row& 
     if (q >= r) b = mid; else a = mid;
   }
   c.last = min(b - 1, most);
-  return c;
+  return CutPar{c, g.par};
 }
 
-template <typename T>
-struct Four;
-template <>
-struct Four<float> { using V = float4; };
-template <>
-struct Four<uint16_t> { using V = uint2; };
-
-template <typename T>
+template <typename T, bool kKeep>
 __global__ void __launch_bounds__(kThreads, 2) k_sample(const SampleArgs a) {
-  using V = typename Four<T>::V;
   extern __shared__ __align__(16) uint8_t s_dynamic[];
-  V* s_values = reinterpret_cast<V*>(s_dynamic);
-  __shared__ Shared s;
+  Shared& s = *reinterpret_cast<Shared*>(s_dynamic);
   Group g{cg::this_cluster(), &s, 0, 0, 0};
-  auto started = g.cl.barrier_arrive();  // a rank's memory is there once it runs
   g.n = (int)g.cl.num_blocks();
   g.me = (int)g.cl.block_rank();
+  if (g.n > 1) cluster_arrive();  // a rank's memory is there once it runs
   const int64_t r = blockIdx.x / g.n;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const T* p = static_cast<const T*>(a.logits) + r * a.row_stride;
-  const Slice<V> x{s_values, a.levels, g.me};
-  uint64_t* s_level = reinterpret_cast<uint64_t*>(s_values + a.levels * kThreads);  // [levels][kWarps]
+  uint64_t* s_level = reinterpret_cast<uint64_t*>(s_dynamic + sizeof(Shared));  // [levels][kWarps]
+  const Slice<T, kKeep> x{reinterpret_cast<typename Four<T>::V*>(s_level + a.levels * kWarps),
+                          static_cast<const T*>(a.logits) + r * a.row_stride, a.levels, g.me, a.vocab, a.vec != 0};
   // Maximum with its lowest index, and the lowest value above -inf.
   float top = kNegInf, least = __builtin_huge_valf();
   int at_top = 0x7fffffff;
-#pragma unroll 4
-  for (int l = 0; l < a.levels; ++l) {
-    const int j = x.index(l);
-    float f[4] = {kNegInf, kNegInf, kNegInf, kNegInf};
-    if (a.vec && j + 3 < a.vocab) {
-      if constexpr (sizeof(T) == 4) {
-        const uint4 v = ldg_nc_v4(p + j);
-        f[0] = __uint_as_float(v.x); f[1] = __uint_as_float(v.y);
-        f[2] = __uint_as_float(v.z); f[3] = __uint_as_float(v.w);
-      } else {
-        const uint2 v = __ldg(reinterpret_cast<const uint2*>(p + j));
-        f[0] = bf16lo(v.x); f[1] = bf16hi(v.x);
-        f[2] = bf16lo(v.y); f[3] = bf16hi(v.y);
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (j + e < a.vocab) f[e] = load_scalar<T>(p, j + e);
+  x.template each<true>([&](float f, int i) {
+    if (f > top) {
+      top = f;
+      at_top = i;
     }
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      // NaN counts as -inf; -0 as 0 (equal numbers have equal keys).
-      f[e] = f[e] != f[e] ? kNegInf : f[e] + 0.f;
-      if (f[e] > top) {
-        top = f[e];
-        at_top = j + e;
-      }
-      if (f[e] > kNegInf) least = fminf(least, f[e]);
-    }
-    pack4(f, s_values[l * kThreads + tid]);
-  }
+    if (f > kNegInf) least = fminf(least, f);
+  });
   uint64_t best = ((uint64_t)key_of(top) << 32) | (0x7fffffffu - (uint32_t)at_top);
   uint64_t low = top > kNegInf ? (uint64_t)key_of(least) : ~0ull;
   if (tid < kTable) s.table[tid] = exp2((double)tid / kTable);
   if (tid == 0) s.listed = 0;
+  if (tid < 3) s.window[tid] = 0;
   clear_bins(s);
   const float temp = a.temperature ? a.temperature[r] : a.temperature1;
   const float top_p = a.top_p ? a.top_p[r] : a.top_p1;
   const float min_p = a.min_p ? a.min_p[r] : a.min_p1;
   const int top_k = a.top_k ? a.top_k[r] : a.top_k1;
 
-  g.cl.barrier_wait(std::move(started));
+  if (g.n > 1) cluster_wait();
   g.reduce(best, low, Max(), Min());
   const uint32_t kmax = (uint32_t)(best >> 32), klow = (uint32_t)low;
   const int imax = (int)(0x7fffffffu - (uint32_t)best);
@@ -565,47 +678,53 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const SampleArgs a) {
     const float scale = (float)kBins / (row.max - value_of(klow));
     const bool even = scale > 0.f && scale < 3e38f;  // not: one value, or an infinite span
     auto bin_of = [&](float f) { return min(kBins - 1, (int)((row.max - f) * scale)); };
-    // The first top_k as a rule fit one CTA's list, which then needs no masses
-    // of the others.
-    const bool small_k = by_k && top_k <= kList / 2;
-    Group::Bins cnt, mass;
+    Group::Bins cnt, mass;  // mass: about, in 2^-30
+    const float width = (row.max - value_of(klow)) / kBins;
+    auto about = [&](float b) { return exp2f((float)row.steps / kTable * -b * width) * 1073741824.f; };
     if (even) {
       x.each([&](float f, int) {
         if (!(f > kNegInf)) return;
-        const int b = bin_of(f);
-        if (by_k) atomicAdd(&s.count[b], 1u);
-        if (by_p && !small_k) add_mass(s, b, mass_of(weight(row, f)));
+        const float y = (row.max - f) * scale;
+        const int b = min(kBins - 1, (int)y);
+        atomicAdd(&s.count[b], 1u);
+        // the place inside the bin in 1/256 (at most 2^18 of them: 26 bits)
+        if (by_p) atomicAdd(&s.mass[0][b], (uint32_t)min(255, (int)((y - (float)b) * 256.f)));
+      });
+      g.sync();
+      // The mean place of a bin's values: their mean weight to 1e-5.
+      g.sum_bins<false>(cnt, mass, [&](int b, float n, float places) {
+        return (uint64_t)(n * about((float)b + (places / n + 0.5f) * (1.f / 256)));
       });
     } else {
-      uint64_t c = 0, m = 0;
-      x.each([&](float f, int) {
-        if (!(f > kNegInf)) return;
-        ++c;
-        m += mass_of(weight(row, f));
-      });
-      g.reduce(c, m, Add(), Add());
+      uint64_t c = 0, none = 0;
+      x.each([&](float f, int) { c += f > kNegInf; });
+      g.reduce(c, none, Add(), Add());
       cnt.whole = c;
-      mass.whole = m;
-    }
-    if (even) {
-      g.cl.sync();
-      g.sum_bins(cnt, mass);
     }
     if (by_k && (uint64_t)top_k >= cnt.whole) by_k = false;  // fewer values than that
-    int listed_bin = -1, listed = 0;
-    uint64_t whole = mass.whole;
+    auto take = [&](CutPar c) {
+      cut = c.cut;
+      g.par = c.par;
+    };
+    int listed = 0;
+    double share = 1.0;  // about, of the mass: what top_k leaves
+    // Without turning each into a whole number: (max - f) * scale is not
+    // negative, so its whole part is below b where it is.
+    auto in_bin = [&](float f, int b) {
+      const float y = (row.max - f) * scale;
+      return f > kNegInf && y >= (float)b && (y < (float)(b + 1) || b == kBins - 1);
+    };
     // The values of a bin, sorted, in rank 0's list; how many (on all ranks).
     auto gather = [&](int bin) {
       x.each([&](float f, int i) {
-        if (!(f > kNegInf) || bin_of(f) != bin) return;
-        Shared* o = g.cl.map_shared_rank(&s, 0);
+        if (!in_bin(f, bin) || !in_cut(cut, key_of(f), i)) return;
+        Shared* o = g.of(0);
         const uint32_t at = atomicAdd(&o->listed, 1u);
         if (at < (uint32_t)kList) o->list[at] = ((uint64_t)key_of(f) << 32) | (uint32_t)~i;
       });
-      g.cl.sync();
-      listed = (int)g.cl.map_shared_rank(&s, 0)->listed;
-      listed_bin = bin;
-      if (g.me == 0 && listed <= kList) sort_list(s.list, listed);
+      g.sync();
+      listed = (int)g.of(0)->listed;
+      if (g.me == 0 && listed <= kList) sort_list(s.list, s.rank, listed);
     };
     // Keys of a bin, for find_by_key.
     auto keys = [&](int bin, uint32_t& lo, uint32_t& hi) {
@@ -624,117 +743,123 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const SampleArgs a) {
       const int bin = g.find_bin(cnt, mass, (uint64_t)top_k, above, above_mass, end);
       if (end <= kList) {  // everything down to the border goes to one CTA, which ends the row
         x.each([&](float f, int i) {
-          if (f > kNegInf && bin_of(f) <= bin) {
-            Shared* o = g.cl.map_shared_rank(&s, 0);
+          if (f > kNegInf && ((row.max - f) * scale < (float)(bin + 1) || bin == kBins - 1)) {
+            Shared* o = g.of(0);
             o->list[atomicAdd(&o->listed, 1u)] = ((uint64_t)key_of(f) << 32) | (uint32_t)~i;
           }
         });
-        g.cl.sync();
+        g.sync();
         if (g.me == 0) finish_list(s, row, (int)end, top_k, top_p, min_p, a.uniforms[r], a.ids + r);
         return;
       }
-      if (by_p && small_k) {  // masses after all
-        x.each([&](float f, int) {
-          if (f > kNegInf) add_mass(s, bin_of(f), mass_of(weight(row, f)));
-        });
-        g.cl.sync();
-        g.sum_bins(cnt, mass);
-        above_mass = 0;
-        uint64_t again;
-        g.find_bin(cnt, mass, (uint64_t)top_k, again, above_mass, end);
-      }
+      if (mass.whole) share = fmin(1.0, ((double)above_mass + ((double)top_k - (double)above) * about((float)bin + 0.5f)) / (double)mass.whole);
       gather(bin);
       if (listed <= kList) {
         const int need = top_k - (int)above;  // of the bin
-        if (g.me == 0) {
-          uint64_t m = 0;
-          if (by_p)
-            for (int i = tid; i < need; i += kThreads) m += mass_of(weight(row, value_of((uint32_t)(s.list[i] >> 32))));
-          m = warp_reduce(m, Add());
-          if (lane == 0) s.warp64[warp] = m;
-          __syncthreads();
-          if (tid < g.n) {
-            m = above_mass;
-            for (int w = 0; w < kWarps; ++w) m += s.warp64[w];
-            Shared* o = g.cl.map_shared_rank(&s, tid);
-            o->found[g.par][0] = s.list[need - 1];
-            o->found[g.par][1] = m;
-          }
-        }
-        g.cl.sync();
+        if (g.me == 0 && tid < g.n) g.of(tid)->found[g.par][0] = s.list[need - 1];
+        g.sync();
         cut.key = (uint32_t)(s.found[g.par][0] >> 32);
         cut.last = (int)~(uint32_t)s.found[g.par][0];
-        whole = s.found[g.par][1];
         g.par ^= 1;
       } else {
         uint32_t lo, hi;
         keys(bin, lo, hi);
-        cut = find_by_key<false>(g, x, row, cut, lo, hi, above, (uint64_t)top_k);
+        take(find_by_key<false>(g, x, row, cut, lo, hi, above, (uint64_t)top_k));
       }
     } else if (by_k) {
-      cut = find_by_key<false>(g, x, row, cut, klow, kmax, 0, (uint64_t)top_k);
+      take(find_by_key<false>(g, x, row, cut, klow, kmax, 0, (uint64_t)top_k));
     }
-    if (by_p && (listed > kList || !even)) {  // the bins are gone: by key, among the first k
-      uint64_t m = 0, none = 0;
+    if (by_p) {
+      // The bin where the border of top_p lies, about; then the exact masses
+      // before and in the three bins around it, and of all.
+      const Cut within = cut;
+      int bin = -1;
+      uint64_t target = 0, above = 0;
+      bool exact = false;
+      uint64_t w[5] = {0, 0, 0, 0, 0};  // all, before the window, its three bins
+      if (even && mass.whole) {
+        uint64_t none1, none2, none3;
+        const uint64_t goal = (uint64_t)((double)mass.whole * share * (double)fmaxf(top_p, 0.f));
+        bin = g.find_bin(mass, cnt, min(mass.whole, goal + 1), none1, none2, none3) - 1;
+      }
+      const float low_f = within.key ? value_of(within.key) : kNegInf;
+      const float y0 = even ? (float)bin : -1.f, y1 = even ? (float)(bin + 3) : -1.f;
       x.each([&](float f, int i) {
-        if (f > kNegInf && in_cut(cut, key_of(f), i)) m += mass_of(weight(row, f));
+        if (!(f >= low_f) || (f == low_f && i > within.last)) return;
+        const uint64_t m = mass_of(weight(row, f));
+        w[0] += m;
+        const float y = (row.max - f) * scale;
+        if (y < y0) w[1] += m;
+        else if (y < y1 && m)  // few
+          atomicAdd(reinterpret_cast<unsigned long long*>(&s.window[min((int)(y - y0), 2)]), (unsigned long long)m);
       });
-      g.reduce(m, none, Add(), Add());
-      cut = find_by_key<true>(g, x, row, cut, max(cut.key, klow), kmax, 0, mass_target(top_p, m));
-    } else if (by_p) {
-      const uint64_t target = mass_target(top_p, whole);
-      uint64_t above = 0, none = 0, end = 0;
-      const int bin = g.find_bin(mass, cnt, target, above, none, end);
-      if (bin != listed_bin) {
+      g.reduce_window(w);
+      target = mass_target(top_p, w[0]);
+      above = w[1];
+#pragma unroll
+      for (int i = 2; i < 5; ++i) {
+        if (exact) continue;
+        if (even && above < target && above + w[i] >= target) {
+          exact = true;
+          bin += i - 2;
+        } else {
+          above += w[i];
+        }
+      }
+      if (exact) {
         if (g.me == 0 && tid == 0) s.listed = 0;
-        g.cl.sync();
+        g.sync();
         gather(bin);
       }
-      if (listed <= kList) {
-        // The last of the list whose preceding mass is below target; with a
-        // top_k in this bin target ends within the first k of it.
+      if (exact && listed <= kList) {
+        // The last of the list whose preceding mass is below target.
         if (g.me == 0) {
           const int per = (listed + kThreads - 1) / kThreads;
-          uint64_t sum = 0;
+          uint64_t sum = 0, all;
           for (int e = 0; e < per; ++e) {
             const int i = tid * per + e;
             if (i < listed) sum += mass_of(weight(row, value_of((uint32_t)(s.list[i] >> 32))));
           }
-          const uint64_t incl = warp_inclusive(sum, lane);
-          if (lane == 31) s.warp64[warp] = incl;
-          __syncthreads();
-          uint64_t before = above + incl - sum;
-          for (int w = 0; w < warp; ++w) before += s.warp64[w];
+          uint64_t before = above + cta_before(s, sum, all);
           for (int e = 0; e < per; ++e) {
             const int i = tid * per + e;
             if (i >= listed) break;
             const uint64_t m = mass_of(weight(row, value_of((uint32_t)(s.list[i] >> 32))));
             if (m && before < target && before + m >= target)
-              for (int o = 0; o < g.n; ++o) g.cl.map_shared_rank(&s, o)->found[g.par][0] = s.list[i];
+              for (int o = 0; o < g.n; ++o) g.of(o)->found[g.par][0] = s.list[i];
             before += m;
           }
         }
-        g.cl.sync();
+        g.sync();
         cut.key = (uint32_t)(s.found[g.par][0] >> 32);
         cut.last = (int)~(uint32_t)s.found[g.par][0];
         g.par ^= 1;
-      } else {
+      } else if (exact) {
         uint32_t lo, hi;
         keys(bin, lo, hi);
-        cut = find_by_key<true>(g, x, row, cut, max(lo, cut.key), hi, above, target);
+        take(find_by_key<true>(g, x, row, within, max(lo, within.key), hi, above, target));
+      } else {  // the estimate was off, or there were no bins
+        take(find_by_key<true>(g, x, row, within, max(within.key, klow), kmax, 0, target));
       }
     }
   }
 
   // Running sums by index: (rank, level, warp, lane, element).
+  // (min_p by the weight itself; below this by more than any rounding, not)
+  const float cut_f = cut.key ? value_of(cut.key) : kNegInf;
+  const float min_f = min_p > 0.f ? row.max + fminf(temp * (logf(min_p) - 0.01f), 0.f) - fabsf(row.max) * 1e-6f : kNegInf;
+  const float least_kept = fmaxf(cut_f, min_f <= row.max ? min_f : kNegInf);
+  auto candidate = [&](float f, int i) {
+    return f >= least_kept && f > kNegInf && (f > cut_f || i <= cut.last);
+  };
   auto kept_mass = [&](float f, int i) -> uint64_t {
-    if (!(f > kNegInf) || !in_cut(cut, key_of(f), i)) return 0;
+    if (!candidate(f, i)) return 0;
     const double w = weight(row, f);
     return w >= (double)min_p || i == imax ? mass_of(w) : 0;
   };
   auto level_mass = [&](int l) -> uint64_t {
     float q[4];
-    widen4(s_values[l * kThreads + tid], q);
+    x.four(l, q);
     const int i = x.index(l);
     return kept_mass(q[0], i) + kept_mass(q[1], i + 1) + kept_mass(q[2], i + 2) + kept_mass(q[3], i + 3);
   };
@@ -753,9 +878,9 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const SampleArgs a) {
     uint64_t t = 0;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) t += s.warp64[w];
-    g.cl.map_shared_rank(&s, tid)->all_a[g.par][g.me] = t;
+    g.of(tid)->all_a[g.par][g.me] = t;
   }
-  g.cl.sync();
+  g.sync();
   uint64_t whole = 0, start = 0;
   for (int i = 0; i < g.n; ++i) {
     if (i < g.me) start += s.all_a[g.par][i];
@@ -785,7 +910,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const SampleArgs a) {
   at += warp_inclusive(m, lane) - m;
   if (goal < at || goal >= at + m) return;
   float f[4];
-  widen4(s_values[l * kThreads + tid], f);
+  x.four(l, f);
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     const uint64_t t = kept_mass(f[e], x.index(l) + e);
@@ -794,12 +919,10 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const SampleArgs a) {
   }
 }
 
-template <typename T>
-cudaError_t launch_rows(const SampleArgs& a, int64_t rows, int cluster, cudaStream_t stream) {
-  const void* k = reinterpret_cast<const void*>(k_sample<T>);
-  constexpr int level = kThreads * (int)sizeof(typename Four<T>::V) + kWarps * 8;
-  const int smem = a.levels * level;
-  cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxLevels * level);
+template <typename T, bool kKeep>
+cudaError_t launch_rows(const SampleArgs& a, int64_t rows, int cluster, int smem, cudaStream_t stream) {
+  const void* k = reinterpret_cast<const void*>(k_sample<T, kKeep>);
+  cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(rows * cluster));
@@ -830,16 +953,22 @@ wr_status_t launch_sample(const SampleProblem& p, cudaStream_t stream) {
   a.temperature = p.temperatures; a.top_p = p.top_ps; a.min_p = p.min_ps; a.top_k = p.top_ks;
   a.temperature1 = p.temperature; a.top_p1 = p.top_p; a.min_p1 = p.min_p; a.top_k1 = p.top_k;
   a.ids = p.ids;
-  // The smallest cluster whose CTAs hold the row in 64 KB each (so that two
-  // share an SM; fewer exchanges than with more CTAs); with few rows, for
-  // their latency, one vector a thread or the largest cluster.
+  // As many CTAs as run at once (two an SM), but a vector a thread at least;
+  // more where the row would not stay in shared memory.
   const int64_t vectors = ((int64_t)p.vocab + 3) / 4;
-  const int64_t per = p.rows * kMaxCluster <= device_sm_count() ? kThreads : (elt == 2 ? 16 : 8) * kThreads;
   int cluster = 1;
-  while (cluster < kMaxCluster && vectors > cluster * per) cluster *= 2;
+  while (cluster < kMaxCluster && vectors > cluster * kThreads &&
+         (p.rows * cluster * 2 <= 2 * device_sm_count() || vectors * 4 * elt > (int64_t)cluster * kKeepBytes))
+    cluster *= 2;
   a.levels = (int)((vectors + (int64_t)cluster * kThreads - 1) / ((int64_t)cluster * kThreads));
-  const cudaError_t e = elt == 2 ? launch_rows<uint16_t>(a, p.rows, cluster, stream)
-                                 : launch_rows<float>(a, p.rows, cluster, stream);
+  const int sums = (int)sizeof(Shared) + a.levels * kWarps * 8, part = a.levels * kThreads * 4 * elt;
+  cudaError_t e;
+  if (part <= kKeepBytes)
+    e = elt == 2 ? launch_rows<uint16_t, true>(a, p.rows, cluster, sums + part, stream)
+                 : launch_rows<float, true>(a, p.rows, cluster, sums + part, stream);
+  else
+    e = elt == 2 ? launch_rows<uint16_t, false>(a, p.rows, cluster, sums, stream)
+                 : launch_rows<float, false>(a, p.rows, cluster, sums, stream);
   return e == cudaSuccess ? WR_OK : cuda_fail(e, "sample_tokens launch");
 }
 
