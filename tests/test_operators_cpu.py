@@ -157,3 +157,19 @@ def test_bad_samples(kw, status, word):
 
 def test_sample_of_no_rows_needs_no_gpu():
     assert sample(rows_=0, logits=None, u=None, ids=None) == _abi.WR_OK
+
+
+def test_python_entry_points_refuse_what_is_not_on_a_gpu():
+    import torch
+
+    import warp_route
+
+    c = torch.zeros(2, 2, 16, 64, dtype=torch.bfloat16)
+    k = torch.zeros(3, 2, 64, dtype=torch.bfloat16)
+    with pytest.raises(RuntimeError, match="k_cache must be a CUDA tensor"):
+        warp_route.append_paged_kv(k, k, c, c, torch.zeros(3, dtype=torch.int64))
+    with pytest.raises(RuntimeError, match="k_cache must be a CUDA tensor"):
+        warp_route.shared_prefix_attention(k, c, c, torch.zeros(3, 1, dtype=torch.int32),
+                                           torch.zeros(3, dtype=torch.int32))
+    with pytest.raises(RuntimeError, match="logits must be a CUDA tensor"):
+        warp_route.sample_tokens(torch.zeros(1, 10), torch.zeros(1))
