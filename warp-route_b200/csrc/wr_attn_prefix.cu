@@ -330,14 +330,24 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1)
       const int r = pc.pair * MR + t * kTileRows + rl;
       const int tok = r / a.group, g = r - tok * a.group;
       const bool in = tok < a.T;
-      if (!dead) {  // this row of Q
-        const uint16_t* src = static_cast<const uint16_t*>(a.q) + (int64_t)tok * a.q_ts +
-                              (int64_t)(pc.h * a.group + g) * a.q_hs;
-        uint8_t* dst = qbuf + t * C::kTileBytes + rl * 128;
+      if (!dead) {
+        // This warp's 32 rows of Q, a row of 16-byte chunks by D / 8 lanes.
+        constexpr int CPR = D / 8, RPP = 32 / CPR;
+        const int c = lane % CPR;
+        const uint16_t* q = static_cast<const uint16_t*>(a.q) + (int64_t)pc.h * a.group * a.q_hs + c * 8;
+        uint4 v[32 / RPP];
 #pragma unroll
-        for (int k = 0; k < D / 8; ++k) {
-          const uint4 v = in ? *reinterpret_cast<const uint4*>(src + k * 8) : make_uint4(0, 0, 0, 0);
-          *reinterpret_cast<uint4*>(dst + (k >> 3) * C::kPanelBytes + (((k & 7) ^ (rl & 7)) << 4)) = v;
+        for (int i = 0; i < 32 / RPP; ++i) {
+          const int rr = pc.pair * MR + t * kTileRows + (warp & 3) * 32 + i * RPP + lane / CPR;
+          const int tk = rr / a.group;
+          v[i] = make_uint4(0, 0, 0, 0);
+          if (tk < a.T) v[i] = *reinterpret_cast<const uint4*>(q + (int64_t)tk * a.q_ts + (int64_t)(rr - tk * a.group) * a.q_hs);
+        }
+#pragma unroll
+        for (int i = 0; i < 32 / RPP; ++i) {
+          const int row = (warp & 3) * 32 + i * RPP + lane / CPR;
+          *reinterpret_cast<uint4*>(qbuf + t * C::kTileBytes + (c >> 3) * C::kPanelBytes + row * 128 +
+                                    (((c & 7) ^ (row & 7)) << 4)) = v[i];
         }
         fence_proxy_async_smem();
         mbar_arrive(&q_full[t]);
@@ -438,19 +448,41 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1)
       const bool whole = pc.u == 0 && pc.n == p.us;
       const int64_t orow = (int64_t)tok * a.hq + pc.h * a.group + g;
       const int64_t prow = ((int64_t)blockIdx.x * 2 + (pc.u == 0 ? 1 : 0)) * MR + t * kTileRows + rl;
-      float* op = whole ? a.home + orow * D : a.part.piece + prow * D;
       if (!dead) {
+        // Sums of 64 columns at a time go through this warp's quarter of the
+        // tile's Q (whose last product has ended) to whole rows: a thread's own
+        // row would be 16 bytes here and there (10000 cycles against 2500).
         tc_fence_after();
+        __syncwarp();
+        uint8_t* stage = qbuf + t * C::kTileBytes + (warp & 3) * (C::kTileBytes / 4);
+        constexpr int kCols = D == 64 ? 32 : 64, CH = kCols / 4;  // chunks of 16 bytes a row
 #pragma unroll 1
-        for (int k = 0; k < D / 32; ++k) {
-          uint32_t o[32];
-          tmem_ld32(to + k * 32, o);
-          tmem_wait_lds();
-          reg_dep32(o);
-          if (in)
+        for (int k = 0; k < D / kCols; ++k) {
 #pragma unroll
-            for (int j = 0; j < 32; j += 4)
-              *reinterpret_cast<uint4*>(op + k * 32 + j) = make_uint4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+          for (int j = 0; j < kCols / 16; ++j) {
+            uint32_t o[16];
+            tmem_ld16(to + k * kCols + j * 16, o);
+            tmem_wait_ld(o);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              *reinterpret_cast<uint4*>(stage + lane * kCols * 4 + (((j * 4 + e) ^ (lane & 7)) << 4)) =
+                  make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+          }
+          __syncwarp();
+          const int c = lane % CH;
+#pragma unroll 4
+          for (int i = 0; i < 32; i += 32 / CH) {
+            const int rw = i + lane / CH;  // row of this warp
+            const int rr = pc.pair * MR + t * kTileRows + (warp & 3) * 32 + rw;
+            const int tk = rr / a.group;
+            if (tk < a.T) {
+              float* op = whole ? a.home + ((int64_t)tk * a.hq + pc.h * a.group + (rr - tk * a.group)) * D
+                                : a.part.piece + (prow - lane + rw) * D;
+              *reinterpret_cast<uint4*>(op + k * kCols + c * 4) =
+                  *reinterpret_cast<const uint4*>(stage + rw * kCols * 4 + ((c ^ (rw & 7)) << 4));
+            }
+          }
+          __syncwarp();
         }
         tc_fence_before();
       } else {
