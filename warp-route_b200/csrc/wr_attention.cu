@@ -459,8 +459,11 @@ __global__ void __launch_bounds__(kStreamWarps * 32) k_attn_stream(const AttnArg
 // ---------------------------------------------------------------------------
 // fp32
 // ---------------------------------------------------------------------------
+// Two stages: six warps an SM rather than four count for more than a third
+// stage (12 sequences, 16 heads: 39 us against 43).
 template <int DP, int MR>
 struct StreamF32Cfg {
+  static constexpr int kStages = 2;
   static constexpr int kMR = MR;
   static constexpr int kWarps = 1;
   static constexpr int kRowBytes = DP * 4;
@@ -478,7 +481,7 @@ struct StreamF32Cfg {
 template <int DP, int MR>
 __global__ void __launch_bounds__(32) k_attn_stream_f32(const AttnArgs a) {
   using C = StreamF32Cfg<DP, MR>;
-  constexpr int CPR = DP / 4, HR = MR / 2;  // rows whose statistics a half of the lanes keeps
+  constexpr int kStages = C::kStages, CPR = DP / 4, HR = MR / 2;  // rows whose statistics a half of the lanes keeps
   constexpr int VC = DP / 32;  // columns of O a lane has
   constexpr int VW = VC < 4 ? VC : 4;  // ... in runs of VW
   extern __shared__ __align__(128) uint8_t smem[];
@@ -723,168 +726,227 @@ WR_DEVINL PieceList piece_list(const AttnSplit& sp, int64_t unit0, int us, int r
   return p;
 }
 
-// A row's pieces, 32 at a time: lane i looks up piece i and its weight, then
-// all lanes add up the pieces' columns, whose loads do not wait for one
-// another.  kWarps 1: a warp a row; 8: a CTA a row, each warp an eighth of its
-// pieces (few rows with many pieces).
-template <typename T, int MR, int DP, int kWarps>
-__global__ void __launch_bounds__(kWarps == 1 ? 128 : kWarps * 32) k_attn_combine(const CombineArgs c) {
-  constexpr int VC = DP / 32;
-  constexpr int VW = VC < 4 ? VC : 4;
-  constexpr int kRowsCta = kWarps == 1 ? 4 : 1;
-  constexpr int kFlight = DP > 128 ? 4 : 8;
-  __shared__ float s_o[kWarps > 1 ? kWarps : 1][DP];
-  __shared__ float2 s_ml[kWarps > 1 ? kWarps : 1];
-  const AttnArgs& a = c.own;
-  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
-  const int64_t row = (int64_t)blockIdx.x * kRowsCta + (kWarps == 1 ? wid : 0);
-  if (row >= (int64_t)a.T * a.hq) return;  // uniform over a row's warps
-  const int t = (int)row / a.hq, hq = (int)row - t * a.hq;
-  const int h = hq / a.group, g = hq - h * a.group;
-  // Where the pieces are: few rows work it out from the lengths while the
-  // kernels before are still at it; many rows read what those wrote.
-  int b;
-  int64_t unit0 = 0, units = 0;
-  if (kWarps > 1) {
-    b = a.q_start ? seq_of(a, t) : t;
-    const int seg = b + (a.lead > 0);
-    for (int i0 = 0; i0 < segments(a); i0 += 32) {
-      const int64_t v = seg_units<MR>(a, i0 + lane);
-      units += v;
-      if (i0 + lane < seg) unit0 += v;
-    }
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) {
-      unit0 += __shfl_xor_sync(0xffffffffu, unit0, d);
-      units += __shfl_xor_sync(0xffffffffu, units, d);
-    }
-    griddep_wait();
-  } else {
-    griddep_wait();
-    b = a.q_start ? a.token_seq[t] : t;
-    if (b >= 0) unit0 = a.seg_unit[b + (a.lead > 0)];
-    units = a.seg_unit[segments(a)];
-  }
-  PieceList po{}, pp{};
-  if (b >= 0) {
-    const Segment s = segment(a, b + (a.lead > 0));
-    const int us = key_units(s), rts = row_tiles<MR>(a, s);
-    AttnSplit sp;
-    sp.units = units;
-    sp.ranges = min(c.own_warps, sp.units);
-    const int r = (t - s.q0) * a.group + g;
-    po = piece_list(sp, unit0 + ((int64_t)h * rts + r / MR) * us, us, r % MR);
-    if (po.whole && a.direct) return;  // written by the first kernel
-    if (c.has_pre) {
-      const int rp = t * a.group + g, rt = rp / c.pre_mr;
-      pp = piece_list(c.tiles ? c.pre_split : sp, ((int64_t)h * c.pre_rts + rt) * c.pre_us, c.pre_us,
-                      rp - rt * c.pre_mr);
-    }
-  }
-  const int total = po.n + pp.n;
-  const int lo = kWarps == 1 ? 0 : total * wid / kWarps, hi = kWarps == 1 ? total : total * (wid + 1) / kWarps;
-  float m = WR_NEG_INF, l = 0.f, o[VC];
-#pragma unroll
-  for (int i = 0; i < VC; ++i) o[i] = 0.f;
-  for (int c0 = lo; c0 < hi; c0 += 32) {
-    const int i = c0 + lane;
-    const float* src = nullptr;
-    float2 ml = make_float2(WR_NEG_INF, 0.f);
-    if (i < hi) {
-      const bool mine = i < po.n;
-      const PieceList& p = mine ? po : pp;
-      const int k = mine ? i : i - po.n;
-      const int64_t at = p.whole ? row : ((p.w0 + k) * 2 + (k == 0 ? 1 : 0)) * (mine ? MR : c.pre_mr) + p.rl;
-      src = (p.whole ? (mine ? a.home : c.pre_home) : (mine ? a.part.piece : c.pre.piece)) + at * a.dim;
-      ml = (p.whole ? (mine ? a.home_ml : c.pre_home_ml) : (mine ? a.part.piece_ml : c.pre.piece_ml))[at];
-    }
-    float nm = fmaxf(m, ml.x);
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) nm = fmaxf(nm, __shfl_xor_sync(0xffffffffu, nm, d));
-    const float base = nm == WR_NEG_INF ? 0.f : nm;
-    const float fo = ex2(m - base), w = ex2(ml.x - base);
-    float add = ml.y * w;
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) add += __shfl_xor_sync(0xffffffffu, add, d);
-    m = nm;
-    l = l * fo + add;
-#pragma unroll
-    for (int q = 0; q < VC; ++q) o[q] *= fo;
-    const int n = min(32, hi - c0);
-    for (int k0 = 0; k0 < n; k0 += kFlight) {  // kFlight pieces' loads at once
-      float v[kFlight][VC];
-#pragma unroll
-      for (int k = 0; k < kFlight; ++k) {
-        const float* p = reinterpret_cast<const float*>(
-            __shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(src), min(k0 + k, n - 1)));
-#pragma unroll
-        for (int q = 0; q < VC; q += VW) {
-          const int d = q * 32 + lane * VW;
-          if constexpr (VW == 4) {
-            const float4 x = d < a.dim ? *reinterpret_cast<const float4*>(p + d) : make_float4(0.f, 0.f, 0.f, 0.f);
-            v[k][q] = x.x; v[k][q + 1] = x.y; v[k][q + 2] = x.z; v[k][q + 3] = x.w;
-          } else {
-            const float2 x = d < a.dim ? *reinterpret_cast<const float2*>(p + d) : make_float2(0.f, 0.f);
-            v[k][q] = x.x; v[k][q + 1] = x.y;
-          }
-        }
-      }
-#pragma unroll
-      for (int k = 0; k < kFlight; ++k) {
-        const float f = __shfl_sync(0xffffffffu, w, min(k0 + k, n - 1));
-        if (k0 + k < n)
-#pragma unroll
-          for (int q = 0; q < VC; ++q) o[q] += f * v[k][q];
-      }
-    }
-  }
-  if constexpr (kWarps > 1) {
-#pragma unroll
-    for (int q = 0; q < VC; q += VW)
-#pragma unroll
-      for (int e = 0; e < VW; ++e) s_o[wid][q * 32 + lane * VW + e] = o[q + e];
-    if (lane == 0) s_ml[wid] = make_float2(m, l);
-    __syncthreads();
-    if (wid) return;
+// A row's pieces lo .. hi - 1, 32 at a time: lane i looks up piece i and its
+// weight, then all lanes add up the pieces' columns.  The loads of the first
+// few pieces are under way before any weight is known (the pieces have often
+// left L2 by now: one wait for HBM, not two).
+template <int MR, int DP>
+struct RowSum {
+  static constexpr int VC = DP / 32, VW = VC < 4 ? VC : 4;  // columns a lane has, in runs of VW
+  static constexpr int kFlight = DP > 128 ? 2 : 4;
+  float m, l, o[VC];
+
+  WR_DEVINL void add(const CombineArgs& c, const PieceList& po, const PieceList& pp, int64_t row, int lo, int hi,
+                     int lane) {
+    const AttnArgs& a = c.own;
     m = WR_NEG_INF;
-    for (int i = 0; i < kWarps; ++i) m = fmaxf(m, s_ml[i].x);
-    const float base = m == WR_NEG_INF ? 0.f : m;
     l = 0.f;
 #pragma unroll
-    for (int q = 0; q < VC; ++q) o[q] = 0.f;
-    for (int i = 0; i < kWarps; ++i) {
-      const float f = ex2(s_ml[i].x - base);
-      l += s_ml[i].y * f;
+    for (int i = 0; i < VC; ++i) o[i] = 0.f;
+    for (int c0 = lo; c0 < hi; c0 += 32) {
+      const int i = c0 + lane;
+      const float* src = nullptr;
+      float2 ml = make_float2(WR_NEG_INF, 0.f);
+      if (i < hi) {
+        const bool mine = i < po.n;
+        const PieceList& p = mine ? po : pp;
+        const int k = mine ? i : i - po.n;
+        const int64_t at = p.whole ? row : ((p.w0 + k) * 2 + (k == 0 ? 1 : 0)) * (mine ? MR : c.pre_mr) + p.rl;
+        src = (p.whole ? (mine ? a.home : c.pre_home) : (mine ? a.part.piece : c.pre.piece)) + at * a.dim;
+        ml = (p.whole ? (mine ? a.home_ml : c.pre_home_ml) : (mine ? a.part.piece_ml : c.pre.piece_ml))[at];
+      }
+      const int n = min(32, hi - c0);
+      float v[kFlight][VC];
+      auto fetch = [&](int k0) {
 #pragma unroll
-      for (int q = 0; q < VC; q += VW)
+        for (int k = 0; k < kFlight; ++k) {
+          const float* p = reinterpret_cast<const float*>(
+              __shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(src), min(k0 + k, n - 1)));
 #pragma unroll
-        for (int e = 0; e < VW; ++e) o[q + e] += s_o[i][q * 32 + lane * VW + e] * f;
+          for (int q = 0; q < VC; q += VW) {
+            const int d = q * 32 + lane * VW;
+            const bool in = d < a.dim && k0 + k < n;
+            if constexpr (VW == 4) {
+              const float4 x = in ? *reinterpret_cast<const float4*>(p + d) : make_float4(0.f, 0.f, 0.f, 0.f);
+              v[k][q] = x.x; v[k][q + 1] = x.y; v[k][q + 2] = x.z; v[k][q + 3] = x.w;
+            } else {
+              const float2 x = in ? *reinterpret_cast<const float2*>(p + d) : make_float2(0.f, 0.f);
+              v[k][q] = x.x; v[k][q + 1] = x.y;
+            }
+          }
+        }
+      };
+      fetch(0);
+      float nm = fmaxf(m, ml.x);
+#pragma unroll
+      for (int d = 16; d > 0; d >>= 1) nm = fmaxf(nm, __shfl_xor_sync(0xffffffffu, nm, d));
+      const float base = nm == WR_NEG_INF ? 0.f : nm;
+      const float fo = ex2(m - base), w = ex2(ml.x - base);
+      float add = ml.y * w;
+#pragma unroll
+      for (int d = 16; d > 0; d >>= 1) add += __shfl_xor_sync(0xffffffffu, add, d);
+      m = nm;
+      l = l * fo + add;
+#pragma unroll
+      for (int q = 0; q < VC; ++q) o[q] *= fo;
+#pragma unroll 1
+      for (int k0 = 0;;) {
+#pragma unroll
+        for (int k = 0; k < kFlight; ++k) {
+          const float f = __shfl_sync(0xffffffffu, w, min(k0 + k, n - 1));
+          if (k0 + k < n)
+#pragma unroll
+            for (int q = 0; q < VC; ++q) o[q] += f * v[k][q];
+        }
+        k0 += kFlight;
+        if (k0 >= n) break;
+        fetch(k0);
+      }
     }
   }
-  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+
+  template <typename T>
+  WR_DEVINL void store(const AttnArgs& a, int64_t row, int lane) const {
+    const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // NaN stays
 #pragma unroll
-  for (int q = 0; q < VC; q += VW) {
-    const int d = q * 32 + lane * VW;
-    if (d >= a.dim) continue;
-    if constexpr (sizeof(T) == 2) {
+    for (int q = 0; q < VC; q += VW) {
+      const int d = q * 32 + lane * VW;
+      if (d >= a.dim) continue;
+      if constexpr (sizeof(T) == 2) {
 #pragma unroll
-      for (int e = 0; e < VW; e += 2)
-        *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.out) + row * a.dim + d + e) =
-            pack_bf16(o[q + e] * inv, o[q + e + 1] * inv);
-    } else {
+        for (int e = 0; e < VW; e += 2)
+          *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.out) + row * a.dim + d + e) =
+              pack_bf16(o[q + e] * inv, o[q + e + 1] * inv);
+      } else {
 #pragma unroll
-      for (int e = 0; e < VW; ++e) static_cast<float*>(a.out)[row * a.dim + d + e] = o[q + e] * inv;
+        for (int e = 0; e < VW; ++e) static_cast<float*>(a.out)[row * a.dim + d + e] = o[q + e] * inv;
+      }
     }
+    if (a.lse && lane == 0) a.lse[row] = l == 0.f ? WR_NEG_INF : (m + log2f(l)) * kLn2;
   }
-  if (a.lse && lane == 0) a.lse[row] = l == 0.f ? WR_NEG_INF : (m + log2f(l)) * kLn2;
+};
+
+// The pieces of row g of token t and key head h.
+struct RowPlace {
+  Segment s;
+  int us, rts;
+  int64_t unit0;
+  AttnSplit sp;
+};
+template <int MR>
+WR_DEVINL bool row_pieces(const CombineArgs& c, const RowPlace& x, int t, int h, int g, PieceList& po, PieceList& pp) {
+  const AttnArgs& a = c.own;
+  const int r = (t - x.s.q0) * a.group + g;
+  po = piece_list(x.sp, x.unit0 + ((int64_t)h * x.rts + r / MR) * x.us, x.us, r % MR);
+  if (po.whole && a.direct) return false;  // written by the first kernel
+  if (c.has_pre) {
+    const int rp = t * a.group + g, rt = rp / c.pre_mr;
+    pp = piece_list(c.tiles ? c.pre_split : x.sp, ((int64_t)h * c.pre_rts + rt) * c.pre_us, c.pre_us,
+                    rp - rt * c.pre_mr);
+  }
+  return true;
+}
+
+// Few rows with many pieces: a CTA a row, each of its 8 warps an eighth of the
+// pieces.  Where they are it works out from the lengths while the kernels
+// before are still at it.
+template <typename T, int MR, int DP>
+__global__ void __launch_bounds__(256) k_attn_combine_wide(const CombineArgs c) {
+  using R = RowSum<MR, DP>;
+  constexpr int kWarps = 8;
+  __shared__ float s_o[kWarps][DP];
+  __shared__ float2 s_ml[kWarps];
+  const AttnArgs& a = c.own;
+  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
+  const int64_t row = blockIdx.x;
+  const int t = (int)row / a.hq, hq = (int)row - t * a.hq;
+  const int h = hq / a.group, g = hq - h * a.group;
+  RowPlace x{};
+  const int b = a.q_start ? seq_of(a, t) : t, seg = b + (a.lead > 0);
+  for (int i0 = 0; i0 < segments(a); i0 += 32) {
+    const int64_t v = seg_units<MR>(a, i0 + lane);
+    x.sp.units += v;
+    if (i0 + lane < seg) x.unit0 += v;
+  }
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) {
+    x.unit0 += __shfl_xor_sync(0xffffffffu, x.unit0, d);
+    x.sp.units += __shfl_xor_sync(0xffffffffu, x.sp.units, d);
+  }
+  x.sp.ranges = min(c.own_warps, x.sp.units);
+  PieceList po{}, pp{};
+  bool work = true;
+  if (b >= 0) {
+    x.s = segment(a, seg);
+    x.us = key_units(x.s);
+    x.rts = row_tiles<MR>(a, x.s);
+    work = row_pieces<MR>(c, x, t, h, g, po, pp);
+  }
+  griddep_wait();
+  if (!work) return;
+  const int total = po.n + pp.n;
+  R sum;
+  sum.add(c, po, pp, row, total * wid / kWarps, total * (wid + 1) / kWarps, lane);
+#pragma unroll
+  for (int q = 0; q < R::VC; q += R::VW)
+#pragma unroll
+    for (int e = 0; e < R::VW; ++e) s_o[wid][q * 32 + lane * R::VW + e] = sum.o[q + e];
+  if (lane == 0) s_ml[wid] = make_float2(sum.m, sum.l);
+  __syncthreads();
+  if (wid) return;
+  sum.m = WR_NEG_INF;
+  for (int i = 0; i < kWarps; ++i) sum.m = fmaxf(sum.m, s_ml[i].x);
+  const float base = sum.m == WR_NEG_INF ? 0.f : sum.m;
+  sum.l = 0.f;
+#pragma unroll
+  for (int q = 0; q < R::VC; ++q) sum.o[q] = 0.f;
+  for (int i = 0; i < kWarps; ++i) {
+    const float f = ex2(s_ml[i].x - base);
+    sum.l += s_ml[i].y * f;
+#pragma unroll
+    for (int q = 0; q < R::VC; q += R::VW)
+#pragma unroll
+      for (int e = 0; e < R::VW; ++e) sum.o[q + e] += s_o[i][q * 32 + lane * R::VW + e] * f;
+  }
+  sum.template store<T>(a, row, lane);
+}
+
+// Many rows: a warp a row.
+template <typename T, int MR, int DP>
+__global__ void __launch_bounds__(128) k_attn_combine(const CombineArgs c) {
+  const AttnArgs& a = c.own;
+  const int lane = threadIdx.x & 31;
+  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+  griddep_wait();
+  if (row >= (int64_t)a.T * a.hq) return;
+  const int t = (int)row / a.hq, hq = (int)row - t * a.hq;
+  const int h = hq / a.group, g = hq - h * a.group;
+  const int b = a.q_start ? a.token_seq[t] : t;
+  PieceList po{}, pp{};
+  if (b >= 0) {
+    RowPlace x;
+    x.unit0 = a.seg_unit[b + (a.lead > 0)];
+    x.sp.units = a.seg_unit[segments(a)];
+    x.sp.ranges = min(c.own_warps, x.sp.units);
+    x.s = segment(a, b + (a.lead > 0));
+    x.us = key_units(x.s);
+    x.rts = row_tiles<MR>(a, x.s);
+    if (!row_pieces<MR>(c, x, t, h, g, po, pp)) return;
+  }
+  RowSum<MR, DP> sum;
+  sum.add(c, po, pp, row, 0, po.n + pp.n, lane);
+  sum.template store<T>(a, row, lane);
 }
 
 // ---------------------------------------------------------------------------
 // Host
 // ---------------------------------------------------------------------------
-// From this many rows a key head the prefix goes to the tensor cores; the
-// warps of k_attn_stream take 16 rows each and read the keys again for every 16.
+// The prefix goes to the tensor cores from 33 rows a key head where the warps
+// of k_attn_stream, which read the keys again for every 16 rows, would read
+// more than this: below, that kernel's launch and set-up cost more (64 rows a
+// head and 2055 keys of 8 heads, 34 MB: 29 us with it, 26 without).
 constexpr int kTileMinRows = 32;
+constexpr int64_t kTileMinBytes = 64 << 20;
 
 struct Plan {
   int dp, mr, smem;
@@ -929,7 +991,8 @@ Plan make_plan(const AttnProblem& p) {
   pl.inline_prefix = p.prefix_len > 0 && p.B == 1;
   pl.has_pre = p.prefix_len > 0 && !pl.inline_prefix;
   const int64_t group_rows = (int64_t)p.T * group;  // rows that meet the prefix, a key head
-  pl.tiles = pl.has_pre && group_rows > kTileMinRows && prefix_tiles_ok(p);
+  const int64_t again = (group_rows + 15) / 16 * p.c.hkv * p.prefix_len * p.c.dim * 4;  // K and V in bf16
+  pl.tiles = pl.has_pre && group_rows > kTileMinRows && again > kTileMinBytes && prefix_tiles_ok(p);
   // An upper bound of the units: the lengths are on the device.
   const int64_t keys = (int64_t)p.table_width * p.c.page_size + (pl.inline_prefix ? p.prefix_len : 0);
   const int64_t tiles = (group_rows + pl.mr - 1) / pl.mr + (p.B > 0 ? p.B : 0);
@@ -999,12 +1062,17 @@ cudaError_t launch_stream(const Plan& pl, bool f32, const AttnArgs& a, bool pdl,
   return pl.dp == 64 ? go(k_attn_stream<64>) : pl.dp == 128 ? go(k_attn_stream<128>) : go(k_attn_stream<256>);
 }
 
-template <typename T, int MR, int W>
-cudaError_t launch_combine_dp(int dp, const CombineArgs& c, int64_t grid, cudaStream_t s) {
-  constexpr int th = W == 1 ? 128 : W * 32;
-  if (dp == 64) return launch_one(k_attn_combine<T, MR, 64, W>, grid, th, 0, true, s, &c);
-  if (dp == 128) return launch_one(k_attn_combine<T, MR, 128, W>, grid, th, 0, true, s, &c);
-  return launch_one(k_attn_combine<T, MR, 256, W>, grid, th, 0, true, s, &c);
+template <typename T, int MR>
+cudaError_t launch_combine(int dp, const CombineArgs& c, cudaStream_t s) {
+  const int64_t rows = (int64_t)c.own.T * c.own.hq;
+  if (rows <= (int64_t)device_sm_count() * 8) {
+    auto go = [&](auto kernel) { return launch_one(kernel, rows, 256, 0, true, s, &c); };
+    return dp == 64 ? go(k_attn_combine_wide<T, MR, 64>) : dp == 128 ? go(k_attn_combine_wide<T, MR, 128>)
+                                                                     : go(k_attn_combine_wide<T, MR, 256>);
+  }
+  auto go = [&](auto kernel) { return launch_one(kernel, (rows + 3) / 4, 128, 0, true, s, &c); };
+  return dp == 64 ? go(k_attn_combine<T, MR, 64>) : dp == 128 ? go(k_attn_combine<T, MR, 128>)
+                                                              : go(k_attn_combine<T, MR, 256>);
 }
 
 }  // namespace
@@ -1068,18 +1136,8 @@ wr_status_t launch_attn(const AttnProblem& p, void* ws, cudaStream_t stream) {
   }
   e = launch_stream(pl, f32, a, pl.tiles, stream);
   if (e != cudaSuccess) return cuda_fail(e, "shared_prefix_attention launch");
-  // Few rows: 8 warps a row read its many pieces; many rows: a warp each.
-  const bool wide = pl.rows <= (int64_t)device_sm_count() * 8;
-  const int64_t grid = wide ? pl.rows : (pl.rows + 3) / 4;
-  if (!f32)
-    e = wide ? launch_combine_dp<uint16_t, 16, 8>(pl.dp, c, grid, stream)
-             : launch_combine_dp<uint16_t, 16, 1>(pl.dp, c, grid, stream);
-  else if (pl.mr == 8)
-    e = wide ? launch_combine_dp<float, 8, 8>(pl.dp, c, grid, stream)
-             : launch_combine_dp<float, 8, 1>(pl.dp, c, grid, stream);
-  else
-    e = wide ? launch_combine_dp<float, 4, 8>(pl.dp, c, grid, stream)
-             : launch_combine_dp<float, 4, 1>(pl.dp, c, grid, stream);
+  e = !f32 ? launch_combine<uint16_t, 16>(pl.dp, c, stream)
+           : pl.mr == 8 ? launch_combine<float, 8>(pl.dp, c, stream) : launch_combine<float, 4>(pl.dp, c, stream);
   return e == cudaSuccess ? WR_OK : cuda_fail(e, "shared_prefix_attention (join) launch");
 }
 

@@ -59,7 +59,13 @@ struct PrefixArgs {
   int us;     // units of 128 keys
   AttnSplit sp;
   int box;    // keys of one TMA copy
+  uint32_t group_inv;  // ceil(2^32 / group), 0 for a group of one
 };
+
+// Token of a row: its quotient by the group, exact while row * group < 2^32.
+WR_DEVINL int token_of(const PrefixArgs& p, int row) {
+  return p.group_inv ? (int)__umulhi((uint32_t)row, p.group_inv) : row;
+}
 
 WR_DEVINL float ex2p(float x) {
   float r;
@@ -96,9 +102,9 @@ struct Piece {
 };
 WR_DEVINL Piece piece_at(const PrefixArgs& p, int64_t unit, int64_t end) {
   Piece x;
-  const int64_t tile = unit / p.us;
+  const int64_t tile = quotient(unit, p.us);
   x.u = (int)(unit - tile * p.us);
-  x.h = (int)(tile / p.pairs);
+  x.h = (int)quotient(tile, p.pairs);
   x.pair = (int)(tile - (int64_t)x.h * p.pairs);
   x.n = (int)min((int64_t)(p.us - x.u), end - unit);
   return x;
@@ -328,7 +334,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1)
     while (unit < u1) {
       const Piece pc = piece_at(p, unit, u1);
       const int r = pc.pair * MR + t * kTileRows + rl;
-      const int tok = r / a.group, g = r - tok * a.group;
+      const int tok = token_of(p, r), g = r - tok * a.group;
       const bool in = tok < a.T;
       if (!dead) {
         // This warp's 32 rows of Q, a row of 16-byte chunks by D / 8 lanes.
@@ -339,7 +345,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1)
 #pragma unroll
         for (int i = 0; i < 32 / RPP; ++i) {
           const int rr = pc.pair * MR + t * kTileRows + (warp & 3) * 32 + i * RPP + lane / CPR;
-          const int tk = rr / a.group;
+          const int tk = token_of(p, rr);
           v[i] = make_uint4(0, 0, 0, 0);
           if (tk < a.T) v[i] = *reinterpret_cast<const uint4*>(q + (int64_t)tk * a.q_ts + (int64_t)(rr - tk * a.group) * a.q_hs);
         }
@@ -474,7 +480,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1)
           for (int i = 0; i < 32; i += 32 / CH) {
             const int rw = i + lane / CH;  // row of this warp
             const int rr = pc.pair * MR + t * kTileRows + (warp & 3) * 32 + rw;
-            const int tk = rr / a.group;
+            const int tk = token_of(p, rr);
             if (tk < a.T) {
               float* op = whole ? a.home + ((int64_t)tk * a.hq + pc.h * a.group + (rr - tk * a.group)) * D
                                 : a.part.piece + (prow - lane + rw) * D;
@@ -529,7 +535,7 @@ bool prefix_tiles_ok(const AttnProblem& p) {
   const int64_t most = (int64_t)1 << 38;  // elements; tensor maps hold strides below 2^40 bytes
   return c.dtype == WR_DTYPE_BF16 && (c.dim == 64 || c.dim == 128) && p.scale > 1e-30f && p.scale < 1e30f && c.page_size >= 16 &&
          (c.page_size & (c.page_size - 1)) == 0 && strides && c.page_stride < most && c.head_stride < most &&
-         c.slot_stride < most;
+         c.slot_stride < most && (int64_t)p.T * (p.hq / c.hkv) * (p.hq / c.hkv) < (int64_t)1 << 31;
 }
 
 wr_status_t launch_attn_prefix(const AttnProblem& p, const AttnArgs& a, int row_tile, int grid,
@@ -552,6 +558,7 @@ wr_status_t launch_attn_prefix(const AttnProblem& p, const AttnArgs& a, int row_
   x.sp.units = (int64_t)a.hkv * x.pairs * x.us;
   x.sp.ranges = grid < x.sp.units ? grid : x.sp.units;
   x.box = box_keys;
+  x.group_inv = a.group == 1 ? 0 : (uint32_t)((((uint64_t)1 << 32) + a.group - 1) / a.group);
   cudaError_t e;
   const int g = (int)x.sp.ranges;
   if (c.dim == 64)
