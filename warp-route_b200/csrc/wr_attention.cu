@@ -1120,8 +1120,11 @@ wr_status_t launch_attn(const AttnProblem& p, void* ws, cudaStream_t stream) {
     c.pre_rts = (int)(((int64_t)p.T * a.group + c.pre_mr - 1) / c.pre_mr);
     c.pre_us = (p.prefix_len + unit - 1) / unit;
   }
-  cudaError_t e;
+  cudaError_t e = launch_stream(pl, f32, a, false, stream);
+  if (e != cudaSuccess) return cuda_fail(e, "shared_prefix_attention launch");
   if (pl.tiles) {
+    // After the own keys, so that the prefix's partial results, the larger
+    // part, are still in L2 when they are joined.
     AttnArgs x = a;
     x.prefix = p.prefix_len;
     x.part.piece = reinterpret_cast<float*>(base + pl.off_tpiece);
@@ -1134,8 +1137,6 @@ wr_status_t launch_attn(const AttnProblem& p, void* ws, cudaStream_t stream) {
     const wr_status_t st = launch_attn_prefix(p, x, pl.tile_mr, pl.tile_grid, stream);
     if (st != WR_OK) return st;
   }
-  e = launch_stream(pl, f32, a, pl.tiles, stream);
-  if (e != cudaSuccess) return cuda_fail(e, "shared_prefix_attention launch");
   e = !f32 ? launch_combine<uint16_t, 16>(pl.dp, c, stream)
            : pl.mr == 8 ? launch_combine<float, 8>(pl.dp, c, stream) : launch_combine<float, 4>(pl.dp, c, stream);
   return e == cudaSuccess ? WR_OK : cuda_fail(e, "shared_prefix_attention (join) launch");

@@ -505,6 +505,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1)
     tc_fence_after();
     tmem_dealloc(tmem, C::kTmemCols);
   }
+  griddep_wait();  // this launch counts as complete only after the one before it
 }
 
 template <int D, int NT>
@@ -520,6 +521,11 @@ cudaError_t launch_tiles(const CUtensorMap& km, const CUtensorMap& vm, const Pre
   cfg.blockDim = dim3(C::kThreads);
   cfg.dynamicSmemBytes = C::kSmem;
   cfg.stream = stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
   return cudaLaunchKernelExC(&cfg, k, args);
 }
 
