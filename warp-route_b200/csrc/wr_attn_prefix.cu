@@ -16,12 +16,14 @@
 // columns a tile (with O of both tiles TMEM is full), so the next scores are
 // there when a softmax ends; with one of 128 columns, whose P has to be
 // consumed before the next S, softmax and products of a tile took turns
-// (145 us for 1536 rows and 16384 keys of 8 heads).  m follows the true maximum
+// (145 us for 1536 rows and 16384 keys of 8 heads; now 100 us, 1.05 PFLOP/s, at
+// the 1.5 GHz that the power limit leaves).  m follows the true maximum
 // only when it has grown by more than 8 (a factor of 256, harmless in fp32
 // sums and bf16 weights), so O is rescaled rarely.  Warp 4 * NT brings K and V
 // by TMA, a copy a page and 64 columns, into two rings; the warps behind it
-// issue the MMAs, one for each tile.  Keys in pages outside the cache, and those behind the prefix's
-// end in its last page, are masked in S and their rows of V set to zero.
+// issue the MMAs, for each tile one the scores' and one the sums'.  Keys in
+// pages outside the cache, and those behind the prefix's end in its last page,
+// are masked in S and their rows of V set to zero.
 //
 // The (key head, row tiles, 128 keys) units are dealt to the CTAs in ranges of
 // equal length, their pieces joined by k_attn_combine (wr_attention.cu).
@@ -74,16 +76,16 @@ WR_DEVINL float ex2p(float x) {
 }
 
 // A wait on the critical path, of a converged warp: few instructions (the MMA
-// warps spend their time on them), each try suspended by the hardware for up
-// to 10 ms and 200 of them at most, which is the bound of 2 s.  False: it gave
-// up.
+// warps spend their time on them), each try suspended by the hardware; the
+// clock comes in only when many have failed.  False: it gave up.
+__device__ __noinline__ bool wait_long(uint64_t* bar, uint32_t parity) { return mbar_wait(bar, parity, nullptr); }
 WR_DEVINL bool wait_lean(uint64_t* bar, uint32_t parity) {
   uint32_t ok;
   asm volatile(
       "{\n\t.reg .pred P;\n\t.reg .u32 n;\n\t"
       "mov.u32 n, 200;\n\t"
       "WAIT_%=:\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 P, [%1], %2, 10000000;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 P, [%1], %2;\n\t"
       "@P bra DONE_%=;\n\t"
       "sub.u32 n, n, 1;\n\t"
       "setp.ne.u32 P, n, 0;\n\t"
@@ -93,7 +95,7 @@ WR_DEVINL bool wait_lean(uint64_t* bar, uint32_t parity) {
       : "=r"(ok)
       : "r"(smem_u32(bar)), "r"(parity)
       : "memory");
-  return ok != 0;
+  return ok != 0 || wait_long(bar, parity);
 }
 
 // A CTA's pieces in order: the units of one (key head, row tiles) in its range.
@@ -455,12 +457,15 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1)
       const int64_t orow = (int64_t)tok * a.hq + pc.h * a.group + g;
       const int64_t prow = ((int64_t)blockIdx.x * 2 + (pc.u == 0 ? 1 : 0)) * MR + t * kTileRows + rl;
       if (!dead) {
-        // Sums of 64 columns at a time go through this warp's quarter of the
-        // tile's Q (whose last product has ended) to whole rows: a thread's own
-        // row would be 16 bytes here and there (10000 cycles against 2500).
+        // Sums of 64 columns at a time (32 where D is 64) go through the place
+        // of this warp's own 32 rows of Q, whose last product has ended (and
+        // which no other warp writes its next rows to), to whole rows: a
+        // thread's own row would be 16 bytes here and there.
         tc_fence_after();
         __syncwarp();
-        uint8_t* stage = qbuf + t * C::kTileBytes + (warp & 3) * (C::kTileBytes / 4);
+        uint8_t* stage = qbuf + t * C::kTileBytes + (warp & 3) * 32 * 128;
+        // 32 rows of kCols sums: all in this panel, or 16 in each of two.
+        auto place = [](int rw) { return D == 64 ? rw * 128 : (rw >> 4) * C::kPanelBytes + (rw & 15) * 256; };
         constexpr int kCols = D == 64 ? 32 : 64, CH = kCols / 4;  // chunks of 16 bytes a row
 #pragma unroll 1
         for (int k = 0; k < D / kCols; ++k) {
@@ -471,7 +476,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1)
             tmem_wait_ld(o);
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-              *reinterpret_cast<uint4*>(stage + lane * kCols * 4 + (((j * 4 + e) ^ (lane & 7)) << 4)) =
+              *reinterpret_cast<uint4*>(stage + place(lane) + (((j * 4 + e) ^ (lane & 7)) << 4)) =
                   make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
           }
           __syncwarp();
@@ -485,7 +490,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1)
               float* op = whole ? a.home + ((int64_t)tk * a.hq + pc.h * a.group + (rr - tk * a.group)) * D
                                 : a.part.piece + (prow - lane + rw) * D;
               *reinterpret_cast<uint4*>(op + k * kCols + c * 4) =
-                  *reinterpret_cast<const uint4*>(stage + rw * kCols * 4 + ((c ^ (rw & 7)) << 4));
+                  *reinterpret_cast<const uint4*>(stage + place(rw) + ((c ^ (rw & 7)) << 4));
             }
           }
           __syncwarp();

@@ -14,7 +14,7 @@
 //
 // A row belongs to one cluster of 1 to 8 CTAs: as many as run at once for all
 // rows (two an SM), and enough to keep the row in shared memory with two CTAs
-// an SM (256 rows of 131072: 8 CTAs a row 240 us, one that reads the row again
+// an SM (256 rows of 131072: 8 CTAs a row 214 us, one that reads the row again
 // for each pass 345 us); only what 8 CTAs do not hold is read again for each
 // pass, from L2 as a rule.  The border of the first k, and that of the mass
 // top_p, are found without sorting the row: a histogram of the values over
@@ -45,7 +45,6 @@ constexpr int kBins = 1024;
 constexpr int kMaxCluster = 8;
 constexpr int kList = 1024;  // values that one CTA sorts
 constexpr int kTable = 128;  // steps of the exponential's table per factor of two
-// 16 vectors a thread hold kSampleMaxVocab values.
 constexpr int kKeepBytes = 76 * 1024;  // of a row's part in shared memory, at most
 constexpr int kFlight = 4;             // vectors a thread has in flight
 constexpr double kMassOne = 35184372088832.0;  // 2^45: with up to 2^18 values sums stay below 2^63
@@ -83,7 +82,7 @@ WR_DEVINL bool in_cut(const Cut& c, uint32_t key, int idx) {
   return key > c.key || (key == c.key && idx <= c.last);
 }
 
-struct Shared {
+struct alignas(16) Shared {
   uint32_t count[kBins];
   // Masses in parts of 14 bits, each added with a native 32-bit atomic (a
   // 64-bit one is a loop of compare and swap): at most 2^18 values, so no part
@@ -96,8 +95,7 @@ struct Shared {
   // written by every rank of the cluster into every rank's copy
   uint64_t all_a[2][kMaxCluster], all_b[2][kMaxCluster];
   uint64_t all_w[kMaxCluster][5];
-  uint64_t warp_w[kWarps][2];
-  uint64_t window[3];
+  uint64_t warp_w[kWarps][5];
   uint32_t rank[256];
   uint64_t found[2][4];
   uint32_t listed;
@@ -123,23 +121,32 @@ static_assert(sizeof(Shared) % 16 == 0 && sizeof(Shared) + kKeepBytes < 113 * 10
 
 struct Row {
   float max;
+  float low;            // values below this weigh nothing: their weight rounds to 0, or they are -inf
   double maxd;
   double steps;         // table steps per unit of x: kTable * log2(e) / temperature
   const double* table;  // 2^(i / kTable)
 };
 
+// The same value in 64 bits, by its bits (the conversion is one of the slow
+// instructions).  A number below 2^-126 in size comes out as some other one
+// below 2^-126, an infinity as 2^128: no difference to x - max where it counts.
+WR_DEVINL double wider(float x) {
+  const uint32_t b = __float_as_uint(x);
+  return __hiloint2double((int)((((b & 0x7fffffffu) >> 3) + 0x38000000u) | (b & 0x80000000u)), (int)(b << 29));
+}
+
 // w = 2^(steps (x - max) / kTable): the whole steps by the table and the
-// exponent, the rest of at most half a step (|u| <= ln 2 / 256) by the
-// exponential's series up to u^4 (the next term is below 2^-49).  Table-driven
-// reduction as in P. T. P. Tang, ACM TOMS 15 (1989).
+// exponent, the rest r of at most half a step by the series of the exponential
+// of u = r ln 2 / kTable (|u| <= ln 2 / 256) up to u^4 (the next term is below
+// 2^-49).  Table-driven reduction as in P. T. P. Tang, ACM TOMS 15 (1989).
 WR_DEVINL double weight(const Row& r, float x) {
-  if (x == r.max) return 1.0;  // +inf among them
-  const double t = ((double)x - r.maxd) * r.steps;
-  if (!(t > -60.0 * kTable)) return 0.0;  // far below 2^-46, which rounds to nothing
+  if (!(x >= r.low)) return 0.0;
+  constexpr double c = 0.69314718055994530942 / kTable;
+  const double t = (wider(x) - r.maxd) * r.steps;
   const double m = t + kMagic;
   const int k = __double2loint(m);
-  const double u = (t - (m - kMagic)) * (0.69314718055994530942 / kTable);
-  const double e = fma(fma(fma(fma(u, 1.0 / 24, 1.0 / 6), u, 0.5), u, 1.0), u, 1.0);
+  const double u = t - (m - kMagic);
+  const double e = fma(fma(fma(fma(u, c * c * c * c / 24, c * c * c / 6), u, c * c / 2), u, c), u, 1.0);
   const double w = r.table[k & (kTable - 1)] * e;
   return __hiloint2double(__double2hiint(w) + ((k >> 7) << 20), __double2loint(w));
 }
@@ -258,6 +265,19 @@ struct Group {
   }
   WR_DEVINL Shared* of(int rank) { return n == 1 ? s : cl.map_shared_rank(s, rank); }
 
+  // A value for rank 0's list, from the lanes that have one (one atomic a
+  // warp); all lanes of the warp call it.
+  WR_DEVINL void push(bool have, float f, int i) {
+    const uint32_t who = __ballot_sync(0xffffffffu, have);
+    if (!who) return;
+    const int lane = threadIdx.x & 31, first = __ffs(who) - 1;
+    Shared* o = of(0);
+    uint32_t at = 0;
+    if (lane == first) at = atomicAdd(&o->listed, (uint32_t)__popc(who));
+    at = __shfl_sync(0xffffffffu, at, first) + __popc(who & ((1u << lane) - 1));
+    if (have && at < (uint32_t)kList) o->list[at] = ((uint64_t)key_of(f) << 32) | (uint32_t)~i;
+  }
+
   // Two values of the CTA's threads reduced over the cluster (fa, fb
   // associative and commutative); every thread gets both.
   template <typename FA, typename FB>
@@ -294,12 +314,11 @@ struct Group {
     par ^= 1;
   }
 
-  // Over the cluster: the sums of two values of the threads, and of the
-  // window's three (complete at the call's barrier).
-  WR_DEVINL void reduce_window(uint64_t (&v)[5]) {
+  // Five sums over the cluster.
+  WR_DEVINL void reduce5(uint64_t (&v)[5]) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < 5; ++i) {
       v[i] = warp_reduce(v[i], Add());
       if (lane == 0) s->warp_w[warp][i] = v[i];
     }
@@ -307,11 +326,7 @@ struct Group {
     if (threadIdx.x < 5 * n) {
       const int i = threadIdx.x % 5;
       uint64_t t = 0;
-      if (i < 2) {
-        for (int w = 0; w < kWarps; ++w) t += s->warp_w[w][i];
-      } else {
-        t = s->window[i - 2];
-      }
+      for (int w = 0; w < kWarps; ++w) t += s->warp_w[w][i];
       of(threadIdx.x / 5)->all_w[me][i] = t;
     }
     sync();
@@ -649,7 +664,6 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const SampleArgs a) {
   uint64_t low = top > kNegInf ? (uint64_t)key_of(least) : ~0ull;
   if (tid < kTable) s.table[tid] = exp2((double)tid / kTable);
   if (tid == 0) s.listed = 0;
-  if (tid < 3) s.window[tid] = 0;
   clear_bins(s);
   const float temp = a.temperature ? a.temperature[r] : a.temperature1;
   const float top_p = a.top_p ? a.top_p[r] : a.top_p1;
@@ -666,7 +680,10 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const SampleArgs a) {
   }
   Row row;
   row.max = value_of(kmax);
-  row.maxd = (double)row.max;
+  row.maxd = wider(row.max);
+  // e^-41.6 is 2^-60, far below the 2^-46 that rounds to nothing
+  const float lowest = value_of((uint32_t)low);
+  row.low = row.max > 3.4e38f ? row.max : fmaxf(row.max - 41.6f * temp, lowest);
   row.steps = kTable * 1.4426950408889634074 / (double)temp;
   row.table = s.table;
 
@@ -677,13 +694,12 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const SampleArgs a) {
     // Even bins over the values (monotone in x, whatever it rounds to).
     const float scale = (float)kBins / (row.max - value_of(klow));
     const bool even = scale > 0.f && scale < 3e38f;  // not: one value, or an infinite span
-    auto bin_of = [&](float f) { return min(kBins - 1, (int)((row.max - f) * scale)); };
     Group::Bins cnt, mass;  // mass: about, in 2^-30
     const float width = (row.max - value_of(klow)) / kBins;
     auto about = [&](float b) { return exp2f((float)row.steps / kTable * -b * width) * 1073741824.f; };
     if (even) {
       x.each([&](float f, int) {
-        if (!(f > kNegInf)) return;
+        if (!(f >= lowest)) return;
         const float y = (row.max - f) * scale;
         const int b = min(kBins - 1, (int)y);
         atomicAdd(&s.count[b], 1u);
@@ -710,17 +726,15 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const SampleArgs a) {
     double share = 1.0;  // about, of the mass: what top_k leaves
     // Without turning each into a whole number: (max - f) * scale is not
     // negative, so its whole part is below b where it is.
+    auto bin_end = [](int b) { return b == kBins - 1 ? 3e38f : (float)(b + 1); };
     auto in_bin = [&](float f, int b) {
       const float y = (row.max - f) * scale;
-      return f > kNegInf && y >= (float)b && (y < (float)(b + 1) || b == kBins - 1);
+      return y >= (float)b && y < bin_end(b);
     };
     // The values of a bin, sorted, in rank 0's list; how many (on all ranks).
     auto gather = [&](int bin) {
       x.each([&](float f, int i) {
-        if (!in_bin(f, bin) || !in_cut(cut, key_of(f), i)) return;
-        Shared* o = g.of(0);
-        const uint32_t at = atomicAdd(&o->listed, 1u);
-        if (at < (uint32_t)kList) o->list[at] = ((uint64_t)key_of(f) << 32) | (uint32_t)~i;
+        g.push(in_bin(f, bin) && in_cut(cut, key_of(f), i), f, i);
       });
       g.sync();
       listed = (int)g.of(0)->listed;
@@ -730,7 +744,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const SampleArgs a) {
     auto keys = [&](int bin, uint32_t& lo, uint32_t& hi) {
       uint64_t l = 0xffffffffull, h = 0;
       x.each([&](float f, int) {
-        if (!(f > kNegInf) || bin_of(f) != bin) return;
+        if (!in_bin(f, bin)) return;
         l = min(l, (uint64_t)key_of(f));
         h = max(h, (uint64_t)key_of(f));
       });
@@ -743,10 +757,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const SampleArgs a) {
       const int bin = g.find_bin(cnt, mass, (uint64_t)top_k, above, above_mass, end);
       if (end <= kList) {  // everything down to the border goes to one CTA, which ends the row
         x.each([&](float f, int i) {
-          if (f > kNegInf && ((row.max - f) * scale < (float)(bin + 1) || bin == kBins - 1)) {
-            Shared* o = g.of(0);
-            o->list[atomicAdd(&o->listed, 1u)] = ((uint64_t)key_of(f) << 32) | (uint32_t)~i;
-          }
+          g.push((row.max - f) * scale < bin_end(bin), f, i);
         });
         g.sync();
         if (g.me == 0) finish_list(s, row, (int)end, top_k, top_p, min_p, a.uniforms[r], a.ids + r);
@@ -782,18 +793,23 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const SampleArgs a) {
         const uint64_t goal = (uint64_t)((double)mass.whole * share * (double)fmaxf(top_p, 0.f));
         bin = g.find_bin(mass, cnt, min(mass.whole, goal + 1), none1, none2, none3) - 1;
       }
-      const float low_f = within.key ? value_of(within.key) : kNegInf;
+      const float low_f = fmaxf(within.key ? value_of(within.key) : kNegInf, row.low);
+      const float cut_f = within.key ? value_of(within.key) : kNegInf;
       const float y0 = even ? (float)bin : -1.f, y1 = even ? (float)(bin + 3) : -1.f;
       x.each([&](float f, int i) {
-        if (!(f >= low_f) || (f == low_f && i > within.last)) return;
+        if (!(f >= low_f) || (f == cut_f && i > within.last)) return;
         const uint64_t m = mass_of(weight(row, f));
         w[0] += m;
         const float y = (row.max - f) * scale;
         if (y < y0) w[1] += m;
-        else if (y < y1 && m)  // few
-          atomicAdd(reinterpret_cast<unsigned long long*>(&s.window[min((int)(y - y0), 2)]), (unsigned long long)m);
+        else if (y < y1) {  // few (in registers: hundreds of 64-bit atomics on three words took longer than the pass)
+          const float b = y - y0;
+          if (b < 1.f) w[2] += m;
+          else if (b < 2.f) w[3] += m;
+          else w[4] += m;
+        }
       });
-      g.reduce_window(w);
+      g.reduce5(w);
       target = mass_target(top_p, w[0]);
       above = w[1];
 #pragma unroll
@@ -849,9 +865,8 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const SampleArgs a) {
   const float cut_f = cut.key ? value_of(cut.key) : kNegInf;
   const float min_f = min_p > 0.f ? row.max + fminf(temp * (logf(min_p) - 0.01f), 0.f) - fabsf(row.max) * 1e-6f : kNegInf;
   const float least_kept = fmaxf(cut_f, min_f <= row.max ? min_f : kNegInf);
-  auto candidate = [&](float f, int i) {
-    return f >= least_kept && f > kNegInf && (f > cut_f || i <= cut.last);
-  };
+  const float floor_f = fmaxf(least_kept, row.low);
+  auto candidate = [&](float f, int i) { return f >= floor_f && (f > cut_f || i <= cut.last); };
   auto kept_mass = [&](float f, int i) -> uint64_t {
     if (!candidate(f, i)) return 0;
     const double w = weight(row, f);
