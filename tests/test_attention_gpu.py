@@ -146,6 +146,12 @@ def test_several_tokens_a_sequence(nq, lens, prefix, dtype):
     (40, 4, 4, 128, 8, 300, "heads"),         # pages too small for TMA copies of tiles
     (40, 4, 4, 96, 16, 300, "heads"),
     (40, 4, 4, 128, 24, 300, "heads"),
+    (700, 16, 2, 96, 16, 1500, "heads"),      # columns behind the head
+    (300, 24, 2, 72, 32, 2000, "tokens"),
+    (200, 32, 4, 128, 256, 2700, "heads"),    # enough bytes for the tensor cores
+    (150, 32, 4, 64, 16, 6000, "tokens"),
+    (90, 32, 16, 128, 32, 3100, "heads"),
+    (60, 16, 8, 64, 64, 9000, "heads"),       # 120 rows a head: one tile
 ])
 def test_many_rows_behind_a_prefix(n, hq, hk, d, page, prefix, layout):
     s = make([(i * 37) % 90 for i in range(n)], [1] * n, hq, hk, d, page, prefix, torch.bfloat16, layout=layout)
@@ -158,7 +164,7 @@ def test_many_rows_behind_a_prefix(n, hq, hk, d, page, prefix, layout):
 def test_scores_that_grow_along_the_prefix():
     """The running maximum moves by more than the kernels tolerate without
     rescaling, again and again, for some rows and not for others."""
-    s = make([5] * 80, [1] * 80, 4, 2, 128, 16, 2000, torch.bfloat16)
+    s = make([5] * 80, [1] * 80, 16, 8, 128, 16, 2000, torch.bfloat16)
     ramp = torch.linspace(0.05, 3.0, 2000, device="cuda")
     pages = s["prefix_pages"].long()
     for i, p in enumerate(pages.tolist()):
@@ -170,7 +176,7 @@ def test_scores_that_grow_along_the_prefix():
 
 
 def test_bad_pages_hide_a_tile_of_the_prefix():
-    s = make([9] * 50, [1] * 50, 4, 2, 128, 16, 500, torch.bfloat16)
+    s = make([9] * 50, [1] * 50, 256, 16, 128, 16, 500, torch.bfloat16)
     s["prefix_pages"][3] = -1
     s["prefix_pages"][8:16] = 2 ** 31 - 1   # a whole tile of 128 keys
     s["prefix_pages"][-1] = s["k_cache"].shape[0]
@@ -182,7 +188,7 @@ def test_bad_pages_hide_a_tile_of_the_prefix():
 
 
 def test_several_tokens_and_many_rows():
-    s = make([(i * 53) % 200 + 9 for i in range(24)], [i % 9 + 1 for i in range(24)], 8, 2, 128, 32, 1111,
+    s = make([(i * 53) % 200 + 9 for i in range(24)], [i % 9 + 1 for i in range(24)], 64, 8, 128, 32, 1111,
              torch.bfloat16)
     out, lse = call(s, return_lse=True)
     check(s, out, lse)

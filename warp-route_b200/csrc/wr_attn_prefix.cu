@@ -349,7 +349,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1)
           const int rr = pc.pair * MR + t * kTileRows + (warp & 3) * 32 + i * RPP + lane / CPR;
           const int tk = token_of(p, rr);
           v[i] = make_uint4(0, 0, 0, 0);
-          if (tk < a.T) v[i] = *reinterpret_cast<const uint4*>(q + (int64_t)tk * a.q_ts + (int64_t)(rr - tk * a.group) * a.q_hs);
+          if (tk < a.T && c * 8 < a.dim) v[i] = *reinterpret_cast<const uint4*>(q + (int64_t)tk * a.q_ts + (int64_t)(rr - tk * a.group) * a.q_hs);
         }
 #pragma unroll
         for (int i = 0; i < 32 / RPP; ++i) {
@@ -486,9 +486,9 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1)
             const int rw = i + lane / CH;  // row of this warp
             const int rr = pc.pair * MR + t * kTileRows + (warp & 3) * 32 + rw;
             const int tk = token_of(p, rr);
-            if (tk < a.T) {
-              float* op = whole ? a.home + ((int64_t)tk * a.hq + pc.h * a.group + (rr - tk * a.group)) * D
-                                : a.part.piece + (prow - lane + rw) * D;
+            if (tk < a.T && k * kCols + c * 4 < a.dim) {
+              float* op = whole ? a.home + ((int64_t)tk * a.hq + pc.h * a.group + (rr - tk * a.group)) * a.dim
+                                : a.part.piece + (prow - lane + rw) * a.dim;
               *reinterpret_cast<uint4*>(op + k * kCols + c * 4) =
                   *reinterpret_cast<const uint4*>(stage + place(rw) + ((c ^ (rw & 7)) << 4));
             }
@@ -536,7 +536,8 @@ cudaError_t launch_tiles(const CUtensorMap& km, const CUtensorMap& vm, const Pre
 
 }  // namespace
 
-// TMA copies want pages that cut a tile of 128 keys evenly (or the reverse),
+// Heads of 64, or of up to 128 columns, of which those behind the head arrive
+// as zeros.  TMA copies want pages that cut a tile of 128 keys evenly (or the reverse),
 // 16 keys at least so that a warp's 32 lanes issue a tile's copies at once,
 // and strides other than 0.
 bool prefix_tiles_ok(const AttnProblem& p) {
@@ -544,7 +545,7 @@ bool prefix_tiles_ok(const AttnProblem& p) {
   const bool strides = (c.num_pages == 1 || c.page_stride > 0) && (c.hkv == 1 || c.head_stride > 0) &&
                        (c.page_size == 1 || c.slot_stride > 0);
   const int64_t most = (int64_t)1 << 38;  // elements; tensor maps hold strides below 2^40 bytes
-  return c.dtype == WR_DTYPE_BF16 && (c.dim == 64 || c.dim == 128) && p.scale > 1e-30f && p.scale < 1e30f && c.page_size >= 16 &&
+  return c.dtype == WR_DTYPE_BF16 && c.dim >= 64 && c.dim <= 128 && p.scale > 1e-30f && p.scale < 1e30f && c.page_size >= 16 &&
          (c.page_size & (c.page_size - 1)) == 0 && strides && c.page_stride < most && c.head_stride < most &&
          c.slot_stride < most && (int64_t)p.T * (p.hq / c.hkv) * (p.hq / c.hkv) < (int64_t)1 << 31;
 }
