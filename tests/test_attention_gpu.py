@@ -297,3 +297,55 @@ def test_cache_beyond_32_bits():
     want = warp_route.shared_prefix_attention(q, kc, vc, t - (pages - 3), lens, prefix_pages=pp - (pages - 3),
                                               prefix_len=100)
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_no_own_pages_at_all(dtype):
+    s = make([0] * 5, [1] * 5, 8, 2, 128, 16, 75, dtype)
+    s["tables"] = s["tables"][:, :0]
+    out, lse = call(s, return_lse=True)
+    check(s, out, lse)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("n,c,prefix", [(1, 40, 500), (7, 7, 33), (50, 130, 700), (3, 1, 18)])
+def test_one_sequence_with_several_tokens_behind_a_prefix(n, c, prefix, dtype):
+    s = make([c], [n], 6, 2, 128, 16, prefix, dtype)
+    if n == 1:
+        s["q_start"] = torch.tensor([0, 1], dtype=torch.int32, device="cuda")
+    out, lse = call(s, return_lse=True)
+    check(s, out, lse)
+
+
+def test_pages_that_several_sequences_name():
+    """A page may stand in several tables, several times, and in the prefix."""
+    s = make([64, 64, 30], [1, 1, 1], 8, 2, 128, 16, 64, torch.bfloat16, junk=0.5)
+    s["tables"][1] = s["tables"][0]
+    s["tables"][0, 2] = s["tables"][0, 1]
+    s["prefix_pages"][3] = s["tables"][2, 0]
+    s["prefix_pages"][1] = s["prefix_pages"][0]
+    out, lse = call(s, return_lse=True)
+    check(s, out, lse)
+
+
+def test_two_calls_at_once():
+    a = make([700 + 90 * i for i in range(20)], [1] * 20, 16, 2, 128, 16, 3000, torch.bfloat16)
+    b = make([50] * 300, [1] * 300, 32, 4, 128, 16, 2048, torch.bfloat16, seed=3)
+    want = [call(a), call(b)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for _ in range(6):
+        for i, (s, st) in enumerate(zip((a, b), streams)):
+            with torch.cuda.stream(st):
+                got[i].append(call(s))
+    torch.cuda.synchronize()
+    for i in (0, 1):
+        assert all(torch.equal(g, want[i]) for g in got[i])
+
+
+def test_many_sequences():
+    n = 3000
+    s = make([(i * 7) % 20 for i in range(n)], [1] * n, 2, 1, 64, 16, 40, torch.bfloat16)
+    out, lse = call(s, return_lse=True)
+    check(s, out, lse)

@@ -179,3 +179,41 @@ def test_frequencies_follow_the_probabilities():
     share = torch.softmax(torch.where(x == -3.0, float("-inf"), x).double(), 0)
     count = torch.bincount(ids, minlength=6).double()
     assert ((count - share * n).abs() <= 1.0 + 1e-6).all()
+
+
+def test_two_calls_at_once_and_again():
+    a, ua = rows(64, 60000, torch.bfloat16, seed=1)
+    b, ub = rows(7, 131072, seed=2)
+    want = [warp_route.sample_tokens(a, ua, top_p=0.9), warp_route.sample_tokens(b, ub, top_k=60, top_p=0.8)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = []
+    for _ in range(8):
+        with torch.cuda.stream(streams[0]):
+            got.append((0, warp_route.sample_tokens(a, ua, top_p=0.9)))
+        with torch.cuda.stream(streams[1]):
+            got.append((1, warp_route.sample_tokens(b, ub, top_k=60, top_p=0.8)))
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, want[i]) for i, g in got)
+
+
+def test_many_rows():
+    x, u = rows(5000, 300, seed=8)
+    check(x, u, top_k=30, top_p=0.9)
+
+
+@pytest.mark.parametrize("shift", [-1e6, -3000.0, 3000.0, 1e6])
+def test_logits_far_from_zero(shift):
+    """Only differences count: far from zero they are coarse, not wrong."""
+    x, u = rows(4, 20000, seed=4)
+    check(x + shift, u, top_p=0.9)
+    check(x + shift, u, top_k=77)
+    check((x + shift), u, temperature=0.7, min_p=0.02)
+
+
+@pytest.mark.parametrize("t", [1e-30, 1e-3, 50.0, 1e30, float("inf")])
+def test_extreme_temperatures(t):
+    x, u = rows(4, 20000, seed=5)
+    check(x, u, temperature=t)
+    check(x, u, temperature=t, top_k=100, top_p=0.7)
+    check(x, u, temperature=t, top_p=0.7)
