@@ -349,3 +349,32 @@ def test_many_sequences():
     s = make([(i * 7) % 20 for i in range(n)], [1] * n, 2, 1, 64, 16, 40, torch.bfloat16)
     out, lse = call(s, return_lse=True)
     check(s, out, lse)
+
+
+@pytest.mark.parametrize("dtype,d", [(torch.bfloat16, 64), (torch.bfloat16, 128), (torch.bfloat16, 256),
+                                     (torch.float32, 64), (torch.float32, 128), (torch.float32, 256)])
+@pytest.mark.parametrize("group", [1, 5, 8])
+def test_many_tokens_of_many_sequences(group, dtype, d):
+    """More rows than the warps of a launch could leave unfinished, with rows
+    of no sequence behind them; most units lie behind some row's own key."""
+    hk = 4 if d > 64 else 8
+    n = 2 + 60000 // (hk * group * 30)
+    nq = [(i * 13) % 61 for i in range(n)]
+    lens = [c + (i * 7) % 40 if i % 9 else c // 2 for i, c in enumerate(nq)]
+    s = make(lens, nq, hk * group, hk, d, 16, 0, dtype, seed=group)
+    tail = torch.randn(9, hk * group, d, device="cuda").to(dtype)
+    s["q"] = torch.cat([s["q"], tail])
+    out, lse = call(s, return_lse=True)
+    check(s, out, lse)
+    assert not out[-9:].any() and (lse[-9:] == float("-inf")).all()
+    again = call(s)
+    assert torch.equal(out, again)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_long_sequences_of_many_tokens(dtype):
+    """Tiles cut by several ranges, of which the first rows see only a part."""
+    nq, lens = [700, 1, 300, 700], [700, 900, 2500, 650]
+    s = make(lens, nq, 16, 2, 128, 16, 0, dtype)
+    out, lse = call(s, return_lse=True)
+    check(s, out, lse)

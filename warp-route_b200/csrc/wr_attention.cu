@@ -449,6 +449,8 @@ __global__ void __launch_bounds__(kStreamWarps * 32) k_attn_stream(const AttnArg
         }
       }
       if (it + 1 < n) cc.next(a);
+      else if (a.ends && lane == 0)
+        a.ends[w] = make_int4(cc.b, cc.h, cc.rt, tile_end || first > 0 ? -1 : cc.u);
     }
     cp_async_wait<0>();
   } else {
@@ -686,6 +688,8 @@ __global__ void __launch_bounds__(32) k_attn_stream_f32(const AttnArgs a) {
         }
       }
       if (it + 1 < n) cc.next(a);
+      else if (a.ends && lane == 0)
+        a.ends[w] = make_int4(cc.b, cc.h, cc.rt, tile_end || first > 0 ? -1 : cc.u);
     }
     cp_async_wait<0>();
   } else {
@@ -939,6 +943,41 @@ __global__ void __launch_bounds__(128) k_attn_combine(const CombineArgs c) {
   sum.template store<T>(a, row, lane);
 }
 
+// More rows than the warps of a launch can leave unfinished, and no prefix
+// beside them: a warp a row of the tiles that a range's end cuts (209
+// sequences of 1 to 64 tokens, their own keys and 64 heads of 96 columns: the
+// call takes 226 us so, 341 with a look at every row).  The warp whose range
+// begins a tile names it.
+template <typename T, int MR, int DP>
+__global__ void __launch_bounds__(128) k_attn_combine_ends(const CombineArgs c) {
+  const AttnArgs& a = c.own;
+  const int lane = threadIdx.x & 31;
+  const int64_t at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5), w = at / MR;
+  const int rl = (int)(at % MR);
+  griddep_wait();
+  RowSum<MR, DP> sum;
+  if (a.q_start)
+    for (int64_t t = at; t < a.T; t += (int64_t)gridDim.x * 4)
+      if (a.token_seq[t] < 0)
+        for (int h = 0; h < a.hq; ++h) {
+          sum.add(c, PieceList{}, PieceList{}, t * a.hq + h, 0, 0, lane);
+          sum.template store<T>(a, t * a.hq + h, lane);
+        }
+  AttnSplit sp;
+  sp.units = a.seg_unit[segments(a)];
+  sp.ranges = min(c.own_warps, sp.units);
+  if (w >= sp.ranges) return;
+  const int4 e = a.ends[w];
+  if (e.w < 0) return;
+  const Segment s = segment(a, e.x);
+  const int r = e.z * MR + rl, i = r / a.group;
+  if (i >= s.nq) return;
+  const int64_t row = (int64_t)(s.q0 + i) * a.hq + e.y * a.group + (r - i * a.group);
+  const PieceList po = piece_list(sp, range_start(sp, w + 1) - 1 - e.w, key_units(s), rl);
+  sum.add(c, po, PieceList{}, row, 0, po.n, lane);
+  sum.template store<T>(a, row, lane);
+}
+
 // ---------------------------------------------------------------------------
 // Host
 // ---------------------------------------------------------------------------
@@ -957,7 +996,8 @@ struct Plan {
   int tiles;         // on the tensor cores
   int tile_mr;
   int64_t rows;      // T * hq: of the output
-  size_t off_piece, off_piece_ml, off_home, off_home_ml, off_seg, off_tok;
+  int ends;          // the join takes the tiles that the ranges' ends cut, not all rows
+  size_t off_piece, off_piece_ml, off_home, off_home_ml, off_seg, off_tok, off_ends;
   size_t off_tpiece, off_tpiece_ml, off_phome, off_phome_ml;
   size_t bytes;
 };
@@ -1011,6 +1051,8 @@ Plan make_plan(const AttnProblem& p) {
   pl.off_piece_ml = take(own_rows * 8);
   pl.off_seg = take((size_t)(p.B + 2) * 8);
   pl.off_tok = take((size_t)(p.q_start ? p.T : 0) * 4);
+  pl.ends = !pl.has_pre && pl.rows > (int64_t)pl.own_grid * pl.mr;
+  pl.off_ends = take(pl.ends ? (size_t)pl.own_grid * 16 : 0);
   if (pl.has_pre) {
     pl.off_home = take((size_t)pl.rows * p.c.dim * 4);
     pl.off_home_ml = take((size_t)pl.rows * 8);
@@ -1066,6 +1108,11 @@ cudaError_t launch_stream(const Plan& pl, bool f32, const AttnArgs& a, bool pdl,
 template <typename T, int MR>
 cudaError_t launch_combine(int dp, const CombineArgs& c, cudaStream_t s) {
   const int64_t rows = (int64_t)c.own.T * c.own.hq;
+  if (c.own.ends) {
+    auto go = [&](auto kernel) { return launch_one(kernel, c.own_warps * MR / 4, 128, 0, true, s, &c); };
+    return dp == 64 ? go(k_attn_combine_ends<T, MR, 64>) : dp == 128 ? go(k_attn_combine_ends<T, MR, 128>)
+                                                                     : go(k_attn_combine_ends<T, MR, 256>);
+  }
   if (rows <= (int64_t)device_sm_count() * 8) {
     auto go = [&](auto kernel) { return launch_one(kernel, rows, 256, 0, true, s, &c); };
     return dp == 64 ? go(k_attn_combine_wide<T, MR, 64>) : dp == 128 ? go(k_attn_combine_wide<T, MR, 128>)
@@ -1106,6 +1153,7 @@ wr_status_t launch_attn(const AttnProblem& p, void* ws, cudaStream_t stream) {
   a.lead_home_ml = reinterpret_cast<float2*>(base + pl.off_phome_ml);
   a.seg_unit = reinterpret_cast<int64_t*>(base + pl.off_seg);
   a.token_seq = reinterpret_cast<int32_t*>(base + pl.off_tok);
+  a.ends = pl.ends ? reinterpret_cast<int4*>(base + pl.off_ends) : nullptr;
   a.out = p.out; a.lse = p.lse;
   CombineArgs c{};
   c.own = a;

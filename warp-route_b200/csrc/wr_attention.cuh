@@ -68,6 +68,8 @@ struct AttnArgs {
   float2* lead_home_ml;
   int64_t* seg_unit; // [segments + 1] first unit of each segment, and all of them
   int32_t* token_seq;  // [T] sequence of each token, -1: none
+  int4* ends;        // null, or [warps] the tile that a warp begins and leaves to the next: segment,
+                     // key head, row tile and its last unit there (-1: it leaves none)
   void* out;
   float* lse;
 };
