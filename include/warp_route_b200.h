@@ -362,8 +362,9 @@ WR_API wr_status_t wr_append_paged_kv(const wr_paged_kv_t* cache, int32_t num_to
  *
  * out: contiguous [num_tokens][num_q_heads][head_dim] of the cache's type;
  * lse: fp32 [num_tokens][num_q_heads], or NULL.  A row that sees no key, and
- * a token that belongs to no sequence, gets out = 0 and lse = -inf.  A page
- * index outside the cache hides its keys.  Lengths, tables and q_start are
+ * a token that belongs to no sequence, gets out = 0 and lse = -inf.  A key
+ * that a token does not see does not reach it, infinities and NaN included.
+ * A page index outside the cache hides its keys.  Lengths, tables and q_start are
  * read on the device, so a captured graph follows them; prefix_len is fixed
  * in the call.  The workspace needs no initial content; calls that share one
  * must not overlap on the GPU.  No counterpart in warp-route. */

@@ -378,3 +378,44 @@ def test_long_sequences_of_many_tokens(dtype):
     s = make(lens, nq, 16, 2, 128, 16, 0, dtype)
     out, lse = call(s, return_lse=True)
     check(s, out, lse)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("d,group,prefix", [(64, 8, 0), (128, 4, 0), (256, 3, 0), (96, 1, 70), (128, 20, 300)])
+@pytest.mark.parametrize("bad", [float("inf"), float("-inf"), float("nan")])
+def test_later_keys_that_are_not_finite(bad, d, group, prefix, dtype):
+    """Keys and values of a sequence's last tokens: no row before them sees
+    them, whatever they hold."""
+    nq, lens = [1, 20, 7, 40, 33], [50, 20, 90, 47, 200]
+    s = make(lens, nq, 2 * group, 2, d, 16, prefix, dtype)
+    clean, lse = call(s, return_lse=True)
+    check(s, clean, lse)
+    hit = torch.zeros(sum(nq), dtype=torch.bool, device="cuda")
+    starts = [sum(nq[:i]) for i in range(6)]
+    # 3 late keys of each longer sequence: in the last unit, and one before it
+    for b, back in ((1, 1), (2, 3), (3, 20), (4, 2)):
+        for j in (lens[b] - back, lens[b] - 1):
+            page = s["tables"][b, j // 16]
+            s["k_cache"][page, :, j % 16] = bad
+            s["v_cache"][page, :, j % 16, ::3] = bad
+        hit[starts[b] + nq[b] - back:starts[b + 1]] = True
+    out, got = call(s, return_lse=True)
+    assert torch.isfinite(out[~hit]).all() and torch.isfinite(got[~hit]).all()
+    # only the order of a unit's sums, and the rounding of its weights, differ
+    tol = (2.0 ** -6 if dtype == torch.bfloat16 else 2.0 ** -14)
+    assert ((out[~hit].double() - clean[~hit].double()).abs() <= tol * (1 + clean[~hit].double().abs())).all()
+    assert torch.equal(got[~hit], lse[~hit])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_a_value_that_is_not_finite_reaches_who_sees_it(dtype):
+    nq, lens = [20], [20]
+    s = make(lens, nq, 4, 2, 128, 16, 0, dtype)
+    s["v_cache"][s["tables"][0, 0], :, 9, 5] = float("inf")
+    out = call(s)
+    assert torch.isfinite(out[:9]).all()
+    seen = out[9:, :, 5]
+    assert (seen == float("inf")).all()
+    rest = torch.ones(128, dtype=torch.bool, device="cuda")
+    rest[5] = False
+    assert torch.isfinite(out[:, :, rest]).all()

@@ -25,6 +25,8 @@
 // segment of its own, whose partial results k_attn_combine joins to those of
 // the own keys: m = max m_s, l = sum l_s 2^(m_s - m), O = sum O_s 2^(m_s - m),
 // in the order of the pieces, so that a call's result is the same each time.
+#include <climits>
+
 #include "wr_attention.cuh"
 
 namespace wr {
@@ -215,6 +217,17 @@ WR_DEVINL int row_limit(const AttnArgs& a, const Cursor<MR>& c, int i) {
   return c.s.prefix + max(0, c.s.len - c.s.nq + i + 1);
 }
 
+// The first unit with a key that some row of the tile does not see, because a
+// later token of its sequence put it there.  A weight of zero does not hide an
+// infinity or a NaN in that key's value: from here on the values are looked
+// through, and a unit that holds one is added up key by key, by the rows that
+// see the key.
+template <int MR>
+WR_DEVINL int first_cut(const AttnArgs& a, const Cursor<MR>& c) {
+  if (c.s.nq <= 1) return INT_MAX;
+  return (c.s.prefix + max(0, c.s.len - c.s.nq + c.rt * MR / a.group + 1)) / kUnitTokens;
+}
+
 // ---------------------------------------------------------------------------
 // bf16
 // ---------------------------------------------------------------------------
@@ -228,8 +241,12 @@ struct StreamCfg {
   static constexpr int kSmem = kStreamWarps * kWarpBytes;
 };
 
-template <int DP>
-__global__ void __launch_bounds__(kStreamWarps * 32) k_attn_stream(const AttnArgs a) {
+// Registers for as many warps an SM as the rings leave room for.
+// kSeveral: some sequence may have several tokens.  The look at their later
+// values costs such calls 2 to 14 % (24 sequences of 1 to 9: 67.8 us, 66.1
+// without; the 209 sequences of 1 to 64 below: 257, 226).
+template <int DP, bool kSeveral>
+__global__ void __launch_bounds__(kStreamWarps * 32) __maxnreg__(DP == 64 ? 128 : DP == 128 ? 224 : 255) k_attn_stream(const AttnArgs a) {
   using C = StreamCfg<DP>;
   constexpr int MR = 16, CPR = DP / 8, RPP = 32 / CPR;  // chunks a row, rows a pass of the warp
   extern __shared__ __align__(128) uint8_t smem[];
@@ -285,13 +302,14 @@ __global__ void __launch_bounds__(kStreamWarps * 32) k_attn_stream(const AttnArg
     uint32_t qf[C::kQSmem ? 1 : DP / 16][4];
     float o[DP / 8][4];
     float m0 = WR_NEG_INF, m1 = WR_NEG_INF, l0 = 0.f, l1 = 0.f;
-    int lim0 = 0, lim1 = 0, first = 0;
+    int lim0 = 0, lim1 = 0, first = 0, cut = 0;
     const int g8 = lane >> 2, c2 = (lane & 3) * 2;
     for (int it = 0; it < n; ++it) {
       __syncwarp();  // every lane has read what the next copies overwrite
       load();
       if (it == 0 || cc.u == 0) {  // a new piece
         first = cc.u;
+        if constexpr (kSeveral) cut = first_cut(a, cc);
         m0 = m1 = WR_NEG_INF;
         l0 = l1 = 0.f;
 #pragma unroll
@@ -399,7 +417,39 @@ __global__ void __launch_bounds__(kStreamWarps * 32) k_attn_stream(const AttnArg
         }
       const uint32_t p[4] = {pack_bf16(s[0][0], s[0][1]), pack_bf16(s[0][2], s[0][3]),
                              pack_bf16(s[1][0], s[1][1]), pack_bf16(s[1][2], s[1][3])};
-      {
+      bool odd = false;
+      if (kSeveral && cc.u >= cut) {
+        uint32_t x = 0;  // an exponent of ones plus one carries into the sign
+        auto look = [&](uint32_t v) { x |= (v & 0x7f807f80u) + 0x00800080u; };
+#pragma unroll 4
+        for (int i = lane; i < C::kTile / 16; i += 32) {
+          const uint4 v = *reinterpret_cast<const uint4*>(ring + (st * 2 + 1) * C::kTile + i * 16);
+          look(v.x); look(v.y); look(v.z); look(v.w);
+        }
+        odd = __any_sync(0xffffffffu, x & 0x80008000u);
+      }
+      if (odd) {
+#pragma unroll 1
+        for (int j = 0; j < kUnitTokens; ++j) {
+          const int src = (lane & ~3) | ((j & 7) >> 1);
+          const float p0 = __shfl_sync(0xffffffffu, j & 8 ? (j & 1 ? s[1][1] : s[1][0]) : (j & 1 ? s[0][1] : s[0][0]), src);
+          const float p1 = __shfl_sync(0xffffffffu, j & 8 ? (j & 1 ? s[1][3] : s[1][2]) : (j & 1 ? s[0][3] : s[0][2]), src);
+          const uint8_t* vr = ring + (st * 2 + 1) * C::kTile + j * C::kRowBytes + c2 * 2;
+#pragma unroll
+          for (int d = 0; d < DP / 8; ++d) {
+            const uint32_t x = *reinterpret_cast<const uint32_t*>(vr + ((d ^ (j & 7)) << 4));
+            const float lo = __uint_as_float(x << 16), hi = __uint_as_float(x & 0xffff0000u);
+            if (j0 + j < lim0) {
+              o[d][0] += p0 * lo;
+              o[d][1] += p0 * hi;
+            }
+            if (j0 + j < lim1) {
+              o[d][2] += p1 * lo;
+              o[d][3] += p1 * hi;
+            }
+          }
+        }
+      } else {
         const int r = (((lane >> 3) & 1) << 3) + (lane & 7);
         const uint32_t row = vb + r * C::kRowBytes;
 #pragma unroll
@@ -449,10 +499,10 @@ __global__ void __launch_bounds__(kStreamWarps * 32) k_attn_stream(const AttnArg
         }
       }
       if (it + 1 < n) cc.next(a);
-      else if (a.ends && lane == 0)
-        a.ends[w] = make_int4(cc.b, cc.h, cc.rt, tile_end || first > 0 ? -1 : cc.u);
     }
     cp_async_wait<0>();
+    if (kSeveral && a.ends && lane == 0)
+      a.ends[w] = make_int4(cc.b, cc.h, cc.rt, cc.u == cc.us - 1 || first > 0 ? -1 : cc.u);
   } else {
     write_index<MR>(a, lane);
   }
@@ -481,7 +531,7 @@ struct StreamF32Cfg {
 // of the second: DP / 32 columns, all keys.  K chunks are swizzled by key, so
 // that the 8 lanes of a 16-byte read phase meet 8 different banks; Q and the
 // weights are read by all lanes at once.
-template <int DP, int MR>
+template <int DP, int MR, bool kSeveral>
 __global__ void __launch_bounds__(32) k_attn_stream_f32(const AttnArgs a) {
   using C = StreamF32Cfg<DP, MR>;
   constexpr int kStages = C::kStages, CPR = DP / 4, HR = MR / 2;  // rows whose statistics a half of the lanes keeps
@@ -539,13 +589,14 @@ __global__ void __launch_bounds__(32) k_attn_stream_f32(const AttnArgs a) {
 
     const int t = lane & 15, hf = lane >> 4;
     float o[MR][VC], m[HR], l[HR];  // m, l: rows hf * HR + 0 .. HR - 1
-    int lim[HR], first = 0;
+    int lim[HR], first = 0, cut = 0;
     for (int it = 0; it < n; ++it) {
       __syncwarp();
       load();
       const int rows = cc.s.nq * a.group;
       if (it == 0 || cc.u == 0) {
         first = cc.u;
+        if constexpr (kSeveral) cut = first_cut(a, cc);
 #pragma unroll
         for (int r = 0; r < MR; ++r)
 #pragma unroll
@@ -621,15 +672,25 @@ __global__ void __launch_bounds__(32) k_attn_stream_f32(const AttnArgs a) {
           for (int c = 0; c < VC; ++c) o[r][c] *= fr;
         }
       }
+      bool odd = false;
+      if (kSeveral && cc.u >= cut) {
+        uint32_t x = 0;
+        auto look = [&](uint32_t v) { x |= (v & 0x7f800000u) + 0x00800000u; };
+#pragma unroll 4
+        for (int i = lane; i < C::kTile / 16; i += 32) {
+          const uint4 v = reinterpret_cast<const uint4*>(vb)[i];
+          look(v.x); look(v.y); look(v.z); look(v.w);
+        }
+        odd = __any_sync(0xffffffffu, x >> 31);
+      }
 #pragma unroll
       for (int e = 0; e < HR; ++e) {
         const float w = ex2(x[e] - (m[e] == WR_NEG_INF ? 0.f : m[e]));
         l[e] += w;
-        ps[t * MR + hf * HR + e] = w;
+        ps[t * MR + hf * HR + e] = odd && j >= lim[e] ? -1.f : w;  // below zero: not seen
       }
       __syncwarp();
-#pragma unroll 4
-      for (int k = 0; k < kUnitTokens; ++k) {
+      auto key = [&](int k, auto seen) {
         float p[MR];
 #pragma unroll
         for (int r = 0; r < MR; r += 4)
@@ -648,8 +709,16 @@ __global__ void __launch_bounds__(32) k_attn_stream_f32(const AttnArgs a) {
         }
 #pragma unroll
         for (int r = 0; r < MR; ++r)
+          if (seen(p[r]))
 #pragma unroll
-          for (int c = 0; c < VC; ++c) o[r][c] = fmaf(p[r], v[c], o[r][c]);
+            for (int c = 0; c < VC; ++c) o[r][c] = fmaf(p[r], v[c], o[r][c]);
+      };
+      if (!odd) {
+#pragma unroll 4
+        for (int k = 0; k < kUnitTokens; ++k) key(k, [](float) { return true; });
+      } else {
+#pragma unroll 1
+        for (int k = 0; k < kUnitTokens; ++k) key(k, [](float w) { return !(w < 0.f); });
       }
       const bool tile_end = cc.u == cc.us - 1;
       if (tile_end || it == n - 1) {
@@ -688,10 +757,10 @@ __global__ void __launch_bounds__(32) k_attn_stream_f32(const AttnArgs a) {
         }
       }
       if (it + 1 < n) cc.next(a);
-      else if (a.ends && lane == 0)
-        a.ends[w] = make_int4(cc.b, cc.h, cc.rt, tile_end || first > 0 ? -1 : cc.u);
     }
     cp_async_wait<0>();
+    if (kSeveral && a.ends && lane == 0)
+      a.ends[w] = make_int4(cc.b, cc.h, cc.rt, cc.u == cc.us - 1 || first > 0 ? -1 : cc.u);
   } else {
     write_index<MR>(a, lane);
   }
@@ -945,9 +1014,11 @@ __global__ void __launch_bounds__(128) k_attn_combine(const CombineArgs c) {
 
 // More rows than the warps of a launch can leave unfinished, and no prefix
 // beside them: a warp a row of the tiles that a range's end cuts (209
-// sequences of 1 to 64 tokens, their own keys and 64 heads of 96 columns: the
-// call takes 226 us so, 341 with a look at every row).  The warp whose range
-// begins a tile names it.
+// sequences of 1 to 64 tokens, their own keys and 64 heads of 96 columns: 13 us
+// behind the first kernel's 244, and 126 with a look at every row).  The warp
+// whose range begins a tile names it.  Only calls with several tokens a
+// sequence have that many rows to make up for the naming (12 sequences of one
+// token, 16 heads, fp32: 37.1 us without, 39.2 with).
 template <typename T, int MR, int DP>
 __global__ void __launch_bounds__(128) k_attn_combine_ends(const CombineArgs c) {
   const AttnArgs& a = c.own;
@@ -1051,7 +1122,7 @@ Plan make_plan(const AttnProblem& p) {
   pl.off_piece_ml = take(own_rows * 8);
   pl.off_seg = take((size_t)(p.B + 2) * 8);
   pl.off_tok = take((size_t)(p.q_start ? p.T : 0) * 4);
-  pl.ends = !pl.has_pre && pl.rows > (int64_t)pl.own_grid * pl.mr;
+  pl.ends = p.q_start && !pl.has_pre && pl.rows > (int64_t)pl.own_grid * pl.mr;
   pl.off_ends = take(pl.ends ? (size_t)pl.own_grid * 16 : 0);
   if (pl.has_pre) {
     pl.off_home = take((size_t)pl.rows * p.c.dim * 4);
@@ -1094,15 +1165,20 @@ cudaError_t launch_one(K kernel, int64_t grid, int threads, int smem, bool pdl, 
   return cudaLaunchKernelExC(&cfg, reinterpret_cast<const void*>(kernel), ptrs);
 }
 
-cudaError_t launch_stream(const Plan& pl, bool f32, const AttnArgs& a, bool pdl, cudaStream_t s) {
-  auto go = [&](auto kernel) { return launch_one(kernel, pl.own_grid, 32, pl.smem, pdl, s, &a); };
+template <bool kSeveral>
+cudaError_t launch_stream(const Plan& pl, bool f32, const AttnArgs& a, cudaStream_t s) {
+  auto go = [&](auto kernel) { return launch_one(kernel, pl.own_grid, 32, pl.smem, false, s, &a); };
   if (f32 && pl.mr == 8)
-    return pl.dp == 64 ? go(k_attn_stream_f32<64, 8>) : pl.dp == 128 ? go(k_attn_stream_f32<128, 8>)
-                                                                     : go(k_attn_stream_f32<256, 8>);
+    return pl.dp == 64    ? go(k_attn_stream_f32<64, 8, kSeveral>)
+           : pl.dp == 128 ? go(k_attn_stream_f32<128, 8, kSeveral>)
+                          : go(k_attn_stream_f32<256, 8, kSeveral>);
   if (f32)
-    return pl.dp == 64 ? go(k_attn_stream_f32<64, 4>) : pl.dp == 128 ? go(k_attn_stream_f32<128, 4>)
-                                                                     : go(k_attn_stream_f32<256, 4>);
-  return pl.dp == 64 ? go(k_attn_stream<64>) : pl.dp == 128 ? go(k_attn_stream<128>) : go(k_attn_stream<256>);
+    return pl.dp == 64    ? go(k_attn_stream_f32<64, 4, kSeveral>)
+           : pl.dp == 128 ? go(k_attn_stream_f32<128, 4, kSeveral>)
+                          : go(k_attn_stream_f32<256, 4, kSeveral>);
+  return pl.dp == 64    ? go(k_attn_stream<64, kSeveral>)
+         : pl.dp == 128 ? go(k_attn_stream<128, kSeveral>)
+                        : go(k_attn_stream<256, kSeveral>);
 }
 
 template <typename T, int MR>
@@ -1169,7 +1245,9 @@ wr_status_t launch_attn(const AttnProblem& p, void* ws, cudaStream_t stream) {
     c.pre_rts = (int)(((int64_t)p.T * a.group + c.pre_mr - 1) / c.pre_mr);
     c.pre_us = (p.prefix_len + unit - 1) / unit;
   }
-  cudaError_t e = launch_stream(pl, f32, a, false, stream);
+  // With one token a sequence the look for values that are not finite falls
+  // away (12 sequences, 16 heads, fp32: 37 us without it, 41 with).
+  cudaError_t e = p.q_start ? launch_stream<true>(pl, f32, a, stream) : launch_stream<false>(pl, f32, a, stream);
   if (e != cudaSuccess) return cuda_fail(e, "shared_prefix_attention launch");
   if (pl.tiles) {
     // After the own keys, so that the prefix's partial results, the larger

@@ -295,8 +295,9 @@ def shared_prefix_attention(
 
     Returns out [T, num_q_heads, head_dim] in q's dtype, or (out, lse) with
     the fp32 log of the sum of exponentials [T, num_q_heads].  A row that
-    sees no key (and a token of no sequence) gets 0 and -inf.  Lengths and
-    tables are read on the device: a captured graph follows them."""
+    sees no key (and a token of no sequence) gets 0 and -inf.  Keys that a
+    token does not see do not reach it, infinities and NaN included.  Lengths
+    and tables are read on the device: a captured graph follows them."""
     _C = _load_extension()
     out, lse = _C.shared_prefix_attention(q, k_cache, v_cache, block_tables, context_lens,
                                           prefix_pages, prefix_len, q_start,
