@@ -217,3 +217,50 @@ def test_extreme_temperatures(t):
     check(x, u, temperature=t)
     check(x, u, temperature=t, top_k=100, top_p=0.7)
     check(x, u, temperature=t, top_p=0.7)
+
+
+def _edge_rows(dtype):
+    """Rows with a value just inside a bin's end: 1024 even bins over the
+    row's span R have their first edge at R / 1024 below the maximum, and the
+    product (max - x) * (1024 / R) comes out as 1 - 2^-24 for some of them."""
+    kept = []
+    for n in range(1, 4000):
+        span = np.float32(n / 8)
+        x = np.float32(-n / 8192)
+        y = np.float32(-x) * np.float32(np.float32(1024) / span)
+        if y == np.nextafter(np.float32(1), np.float32(0)):
+            r = torch.tensor([0.0, float(x), -float(span)])
+            if torch.equal(r.to(dtype).float(), r):
+                kept.append(r)
+    return torch.stack(kept).to(dtype).cuda()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_values_at_the_end_of_a_bin(dtype):
+    """Every pass of top_p has to put such a value into the same bin."""
+    x = _edge_rows(dtype)
+    assert x.shape[0] >= (500 if dtype == torch.float32 else 20)
+    assert (x.float() == torch.tensor([0.0, -41 / 8192, -5.125], device="cuda")).all(1).any()
+    for u in (0.0, 0.3, 0.7, 1 - 2.0 ** -24):
+        uu = torch.full((x.shape[0],), u, device="cuda")
+        for p in (0.3, 0.5, 0.6, 0.9):
+            check(x, uu, top_p=p)
+    check(x, uu, top_p=0.6, top_k=2)
+
+
+@pytest.mark.parametrize("v", [700, 6000, 40000])
+def test_values_at_the_end_of_a_bin_before_a_full_one(v):
+    """The next bin holds few values, more than one CTA sorts, or most of the row."""
+    u = torch.tensor([0.0, 0.31, 0.68, 1 - 2.0 ** -24], device="cuda")
+    x = torch.full((4, v), -5.125, device="cuda")
+    for i in range(4):
+        g = torch.Generator(device="cuda").manual_seed(i)
+        at = torch.randperm(v, generator=g, device="cuda")
+        x[i, at[:2]] = torch.tensor([0.0, -41 / 8192], device="cuda")
+        # from the second bin's first value to its last
+        n = v // 2
+        x[i, at[2:2 + n]] = -(41 / 8192) * (1.01 + 0.98 * torch.arange(n, device="cuda") / n)
+    for p in (0.5 / v, 1.5 / v, 2.5 / v, 0.2, 0.5, 0.97, 0.999):
+        check(x, u, top_p=p)
+    check(x.bfloat16(), u, top_p=0.4)
+    check(x, u, top_p=0.4, top_k=v // 3)

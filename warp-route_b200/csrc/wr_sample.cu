@@ -581,7 +581,8 @@ __device__ __noinline__ void finish_list(Shared& s, const Row row, int n, int to
 // A border inside keys [lo, hi] (all of them within `within`), where `above`
 // lies before them in the order: the last value whose preceding sum is below
 // target, sums of 1 (kMass false) or of mass.  For bins too full to sort:
-// binned by key until one key is left, whose values go by index.
+// binned by key until one key is left, whose values go by index.  Four passes
+// of 1024 bins tell any two keys apart.
 // (By value, and `par` back by value: nothing of the kernel's hot loops may
 // have its address taken, or they would read it from memory each time.)
 struct CutPar {
@@ -592,7 +593,7 @@ template <bool kMass, typename X>
 __device__ __noinline__ CutPar find_by_key(Group g, const X x, const Row row, const Cut within,
                                         uint32_t lo, uint32_t hi, uint64_t above, uint64_t target) {
   Shared& s = *g.s;
-  while (lo != hi) {
+  for (int pass = 0; pass < 4 && lo < hi; ++pass) {
     int shift = 0;
     while (((hi - lo) >> shift) >= (uint32_t)kBins) ++shift;
     clear_bins(s);
@@ -691,16 +692,19 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const SampleArgs a) {
   bool by_k = top_k >= 1 && top_k < a.vocab;
   const bool by_p = top_p < 1.f;
   if (by_k || by_p) {
-    // Even bins over the values (monotone in x, whatever it rounds to).
+    // Even bins over the values (monotone in x, whatever it rounds to).  A
+    // value's bin is the whole part of its rounded place, in every pass: places
+    // are compared with whole numbers only, never shifted and rounded again.
     const float scale = (float)kBins / (row.max - value_of(klow));
     const bool even = scale > 0.f && scale < 3e38f;  // not: one value, or an infinite span
     Group::Bins cnt, mass;  // mass: about, in 2^-30
     const float width = (row.max - value_of(klow)) / kBins;
+    auto place = [&](float f) { return __fmul_rn(__fsub_rn(row.max, f), scale); };
     auto about = [&](float b) { return exp2f((float)row.steps / kTable * -b * width) * 1073741824.f; };
     if (even) {
       x.each([&](float f, int) {
         if (!(f >= lowest)) return;
-        const float y = (row.max - f) * scale;
+        const float y = place(f);
         const int b = min(kBins - 1, (int)y);
         atomicAdd(&s.count[b], 1u);
         // the place inside the bin in 1/256 (at most 2^18 of them: 26 bits)
@@ -724,11 +728,11 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const SampleArgs a) {
     };
     int listed = 0;
     double share = 1.0;  // about, of the mass: what top_k leaves
-    // Without turning each into a whole number: (max - f) * scale is not
-    // negative, so its whole part is below b where it is.
+    // Without turning each into a whole number: a place is not negative, so
+    // its whole part is below b where it is.
     auto bin_end = [](int b) { return b == kBins - 1 ? 3e38f : (float)(b + 1); };
     auto in_bin = [&](float f, int b) {
-      const float y = (row.max - f) * scale;
+      const float y = place(f);
       return y >= (float)b && y < bin_end(b);
     };
     // The values of a bin, sorted, in rank 0's list; how many (on all ranks).
@@ -757,7 +761,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const SampleArgs a) {
       const int bin = g.find_bin(cnt, mass, (uint64_t)top_k, above, above_mass, end);
       if (end <= kList) {  // everything down to the border goes to one CTA, which ends the row
         x.each([&](float f, int i) {
-          g.push((row.max - f) * scale < bin_end(bin), f, i);
+          g.push(place(f) < bin_end(bin), f, i);
         });
         g.sync();
         if (g.me == 0) finish_list(s, row, (int)end, top_k, top_p, min_p, a.uniforms[r], a.ids + r);
@@ -795,17 +799,17 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const SampleArgs a) {
       }
       const float low_f = fmaxf(within.key ? value_of(within.key) : kNegInf, row.low);
       const float cut_f = within.key ? value_of(within.key) : kNegInf;
-      const float y0 = even ? (float)bin : -1.f, y1 = even ? (float)(bin + 3) : -1.f;
+      const float y0 = even ? (float)bin : -1.f, y3 = even ? y0 + 3.f : -1.f;
+      const float y1 = y0 + 1.f, y2 = y0 + 2.f;  // (bin -1 is empty)
       x.each([&](float f, int i) {
         if (!(f >= low_f) || (f == cut_f && i > within.last)) return;
         const uint64_t m = mass_of(weight(row, f));
         w[0] += m;
-        const float y = (row.max - f) * scale;
+        const float y = place(f);
         if (y < y0) w[1] += m;
-        else if (y < y1) {  // few (in registers: hundreds of 64-bit atomics on three words took longer than the pass)
-          const float b = y - y0;
-          if (b < 1.f) w[2] += m;
-          else if (b < 2.f) w[3] += m;
+        else if (y < y3) {  // few (in registers: hundreds of 64-bit atomics on three words took longer than the pass)
+          if (y < y1) w[2] += m;
+          else if (y < y2) w[3] += m;
           else w[4] += m;
         }
       });
