@@ -173,3 +173,9 @@ def test_python_entry_points_refuse_what_is_not_on_a_gpu():
                                            torch.zeros(3, dtype=torch.int32))
     with pytest.raises(RuntimeError, match="logits must be a CUDA tensor"):
         warp_route.sample_tokens(torch.zeros(1, 10), torch.zeros(1))
+
+
+def test_append_with_queries_of_no_heads():
+    # an empty tensor's pointer is NULL: the heads are what is wrong with it
+    assert append(q=rows(ptr=FAKE + 4096), q_out=None, hq=0) == _abi.WR_ERR_INVALID
+    assert "num_q_heads must be positive" in message()

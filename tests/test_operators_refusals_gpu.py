@@ -96,3 +96,12 @@ def test_sampling(kw, word):
         warp_route.sample_tokens(logits, uniforms, **opt)
     with pytest.raises(RuntimeError, match="float32 or bfloat16"):
         warp_route.sample_tokens(_z(3, 10, dtype=torch.float16), _z(3, dtype=torch.float32))
+
+
+def test_append_with_queries_of_no_heads():
+    """Refused: it must not return as if the keys had been written."""
+    with pytest.raises(RuntimeError, match="num_q_heads must be positive"):
+        _append(q=_z(3, 0, 64))
+    # no tokens is another matter: nothing to write
+    out = _append(k=_z(0, 2, 64), v=_z(0, 2, 64), slots=_z(0, dtype=torch.int64), q=_z(0, 4, 64))
+    assert out.shape == (0, 4, 64)

@@ -388,9 +388,9 @@ wr_status_t wr_append_paged_kv(const wr_paged_kv_t* cache, int32_t num_tokens, c
     return fail(WR_ERR_INVALID, "rot_dim must be even and in [0, head_dim=%d], got %d", p.c.dim, rot_dim);
   if (rot_dim > 0 && (!positions || !inv_freq))
     return fail(WR_ERR_INVALID, "positions and inv_freq must not be NULL when rot_dim > 0");
+  if (q && num_q_heads < 1) return fail(WR_ERR_INVALID, "num_q_heads must be positive, got %d", num_q_heads);
   if ((q == nullptr) != (q_out == nullptr))
     return fail(WR_ERR_INVALID, "q and q_out go together");
-  if (q && num_q_heads < 1) return fail(WR_ERR_INVALID, "num_q_heads must be positive, got %d", num_q_heads);
   if ((int64_t)(q ? num_q_heads : 0) + 2 * (int64_t)p.c.hkv > 16384)
     return fail(WR_ERR_UNSUPPORTED, "more than 16384 heads");
   if (num_tokens == 0) return WR_OK;

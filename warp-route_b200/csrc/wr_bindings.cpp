@@ -496,7 +496,7 @@ c10::optional<torch::Tensor> append_paged_kv(torch::Tensor k, torch::Tensor v, t
     qr = make_rows(*q, "q", T, -1, k_cache);
     hq = narrow(q->size(1), "num_q_heads");
     out = torch::empty({T, hq, k_cache.size(3)}, k_cache.options());
-    if (out.numel() == 0) return out;
+    if (T == 0) return out;
   }
   check_status(wr_append_paged_kv(&cache, narrow(T, "num_tokens"), &kr, &vr, slots.data_ptr<int64_t>(),
                                   rot ? positions->data_ptr<int64_t>() : nullptr,
