@@ -144,3 +144,37 @@ def test_attention_without_a_context_is_refused():
         MoEStack(stack.layers, stack.E, stack.H, stack.I, stack.K, 2)
     with pytest.raises(ValueError, match="tokens"):
         MoEStack(stack.layers, stack.E, stack.H, stack.I, stack.K, 3, context=stack.context)
+
+
+def test_a_captured_step_refuses_another_prefix_or_context():
+    """The graph holds prefix_len by value and the tensors by address: a step
+    with others must not run on the old ones."""
+    stack, normal, H = build(3, torch.bfloat16, prefix=37)
+    ctx, A = stack.context, stack.layers[1].attention
+    x = normal(3, H, std=1)
+    advance(ctx, 0)
+    first = stack.step(x).clone()
+    ctx.prefix_len = 20
+    with pytest.raises(ValueError, match="prefix_len"):
+        stack.step(x)
+    ctx.prefix_len = 37
+    assert torch.equal(stack.step(x), first)
+    for field in ("slots", "positions", "context_lens", "block_tables", "prefix_pages"):
+        old = getattr(ctx, field)
+        setattr(ctx, field, old.clone())
+        with pytest.raises(ValueError, match="in place"):
+            stack.step(x)
+        setattr(ctx, field, old)
+    caches = A.k_cache, A.v_cache
+    A.k_cache = A.k_cache.clone()
+    with pytest.raises(ValueError, match="caches"):
+        stack.step(x)
+    A.k_cache = caches[0]
+    assert torch.equal(stack.step(x), first)
+    # released, it captures the new prefix
+    stack.close()
+    ctx.prefix_len = 20
+    ctx.slots = ctx.slots.clone()
+    shorter = stack.step(x).clone()
+    assert torch.equal(shorter, stack.eager(x)) and not torch.equal(shorter, first)
+    stack.close()

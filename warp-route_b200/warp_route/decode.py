@@ -63,8 +63,11 @@ class StackContext:
     positions int64 [T], context_lens int32 [T] (own keys, this step's token
     among them), block_tables int32 [T, pages]; prefix_pages int32 of the
     prefix_len tokens that all sequences share.  The tensors are read when a
-    step runs: write them in place between steps.  A slot of -1 (and a length
-    of 0) is a sequence that does not take part."""
+    step runs: write them in place between steps.  prefix_len is a number and
+    part of the captured step: a `step` with another one, or with another
+    tensor in a field's place, is refused until `close` has released the graph
+    (the next step captures anew).  A slot of -1 (and a length of 0) is a
+    sequence that does not take part."""
     slots: torch.Tensor
     positions: torch.Tensor
     context_lens: torch.Tensor
@@ -124,6 +127,18 @@ class MoEStack:
         self.h = [torch.zeros(shape, dtype=self.dtype, device=dev) for _ in range(2)]
         self.stream = torch.cuda.Stream(device=dev)
         self.graph: Optional[torch.cuda.CUDAGraph] = None
+        self.captured: tuple = ()
+
+    def _fixed(self) -> tuple:
+        """What a captured step has by reference or by value besides weights:
+        the context's fields and the caches."""
+        c = self.context
+        if c is None:
+            return ()
+        caches = [t for L in self.layers if L.attention is not None
+                  for t in (L.attention.k_cache, L.attention.v_cache)]
+        return (c.prefix_len, c.slots, c.positions, c.context_lens, c.block_tables, c.prefix_pages,
+                *caches)
 
     def layer(self, i: int, h: torch.Tensor, nxt: torch.Tensor) -> torch.Tensor:
         """Layer i on input h: writes the next input into nxt and returns the
@@ -188,6 +203,7 @@ class MoEStack:
         g = torch.cuda.CUDAGraph()
         with torch.cuda.graph(g, stream=self.stream):
             self.out = self._forward()
+        self.captured = self._fixed()  # and keeps the tensors for as long as the graph reads them
         self.graph = g
 
     def step(self, x: torch.Tensor) -> torch.Tensor:
@@ -195,6 +211,10 @@ class MoEStack:
         next step overwrites)."""
         if self.graph is None:
             self.capture()
+        now, then = self._fixed(), self.captured
+        if now[:1] != then[:1] or any(a is not b for a, b in zip(now[1:], then[1:])):
+            raise ValueError("prefix_len, the context's tensors and the caches are part of the captured "
+                             "step: write the tensors in place, or close() the stack before a change")
         self.x_in.copy_(x)
         self.graph.replay()
         return self.out
@@ -212,3 +232,4 @@ class MoEStack:
         """Release the graph (before destroying a process group it captured
         collectives of)."""
         self.graph = None
+        self.captured = ()
