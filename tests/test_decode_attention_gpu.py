@@ -178,3 +178,22 @@ def test_a_captured_step_refuses_another_prefix_or_context():
     shorter = stack.step(x).clone()
     assert torch.equal(shorter, stack.eager(x)) and not torch.equal(shorter, first)
     stack.close()
+
+
+def test_capture_writes_no_cache():
+    """The warm-up runs on whatever input is there: it must not reach slots
+    that the context already names."""
+    stack, normal, H = build(3, torch.bfloat16)
+    x = normal(3, H, std=1)
+    advance(stack.context, 0)
+    stack.eager(x)
+    stack.x_in.zero_()  # as another step's input would be
+    slots = stack.context.slots.clone()
+    before = [t.clone() for L in stack.layers for t in (L.attention.k_cache, L.attention.v_cache)]
+    stack.capture()
+    torch.cuda.synchronize()
+    after = [t for L in stack.layers for t in (L.attention.k_cache, L.attention.v_cache)]
+    assert all(torch.equal(torch.nan_to_num(a), torch.nan_to_num(b)) for a, b in zip(after, before))
+    assert torch.equal(stack.context.slots, slots)
+    assert torch.equal(stack.step(x), stack.eager(x))
+    stack.close()

@@ -192,13 +192,22 @@ class MoEStack:
 
     def capture(self, warmup: int = 2) -> None:
         """Capture the stack into a CUDA graph (warm-up calls run first, on the
-        capture stream, so the per-stream workspaces exist before capture)."""
+        capture stream, so the per-stream workspaces exist before capture).
+        The caches stay as they are: the warm-up calls write no slot."""
+        slots = None if self.context is None else self.context.slots
+        kept = None if slots is None else slots.clone()
         # the capture stream's warm-up writes the same static buffers as any
         # call already queued on the caller's stream: run it after them
         self.stream.wait_stream(torch.cuda.current_stream())
         with torch.cuda.stream(self.stream):
-            for _ in range(warmup):
-                self._forward()
+            try:
+                if slots is not None:
+                    slots.fill_(-1)
+                for _ in range(warmup):
+                    self._forward()
+            finally:
+                if slots is not None:
+                    slots.copy_(kept)
         torch.cuda.synchronize()
         g = torch.cuda.CUDAGraph()
         with torch.cuda.graph(g, stream=self.stream):
