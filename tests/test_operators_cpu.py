@@ -179,3 +179,23 @@ def test_append_with_queries_of_no_heads():
     # an empty tensor's pointer is NULL: the heads are what is wrong with it
     assert append(q=rows(ptr=FAKE + 4096), q_out=None, hq=0) == _abi.WR_ERR_INVALID
     assert "num_q_heads must be positive" in message()
+
+
+def test_prefix_waits_have_one_answer_for_a_warp():
+    """k_attn_prefix branches on its waits around warp-wide instructions: each
+    wait whose answer counts goes through a vote, and so does the word by
+    which one warp tells the others that it gave up."""
+    import os
+    import re
+
+    repo = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    with open(os.path.join(repo, "warp-route_b200", "csrc", "wr_attn_prefix.cu")) as f:
+        text = f.read()
+    lines = [ln.split("//")[0].strip() for ln in text.splitlines()]
+    for ln in lines:
+        if "mbar_wait(" in ln or "mbar_try_wait(" in ln or "wait_long(" in ln:
+            dropped = ln.startswith("mbar_wait(")  # its answer is not used
+            itself = re.match(r"(__device__|return mbar_wait\(bar, parity, abort, )", ln)
+            assert dropped or itself or "__all_sync(0xffffffffu," in ln, ln
+        if "*abort" in ln and not re.search(r"\*abort = 1;|volatile int\* abort", ln):
+            assert "__any_sync(0xffffffffu, *abort)" in ln, ln

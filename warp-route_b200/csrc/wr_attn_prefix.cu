@@ -30,6 +30,8 @@
 //
 // Every wait is bounded.  One that runs out ends the CTA's work and leaves NaN
 // in the rows of its pieces, in their sums, so that it shows in the output.
+// Whether a wait ran out is one answer for all lanes of a warp (wait_warp),
+// since what follows is done by whole warps (tcgen05.ld and st, votes, elect).
 #include "wr_attention.cuh"
 #include "wr_tcgen05.cuh"
 
@@ -75,11 +77,25 @@ WR_DEVINL float ex2p(float x) {
   return r;
 }
 
-// A wait on the critical path, of a converged warp: few instructions (the MMA
-// warps spend their time on them), each try suspended by the hardware; the
-// clock comes in only when many have failed.  False: it gave up.
-__device__ __noinline__ bool wait_long(uint64_t* bar, uint32_t parity) { return mbar_wait(bar, parity, nullptr); }
-WR_DEVINL bool wait_lean(uint64_t* bar, uint32_t parity) {
+// Bound of the waits that the work hangs on, in ns; with 0 each gives up at
+// once.  The waits for what is still in flight when a CTA ends are not among
+// them: those always have the whole kWaitLimitNs.
+#ifndef WR_PREFIX_WAIT_NS
+#define WR_PREFIX_WAIT_NS kWaitLimitNs
+#endif
+constexpr uint64_t kPrefixWaitNs = WR_PREFIX_WAIT_NS;
+
+// A wait of a whole converged warp: few instructions (the MMA warps spend
+// their time on them), each try suspended by the hardware; the clock comes in
+// only when many have failed.  False, for all lanes: it gave up, or another
+// warp had.  (The vote costs 1 % of a call bound by this kernel: 191.1 us
+// without, 193.0 with, for 256 sequences of 6 rows a key head behind 16384
+// keys.)
+__device__ __noinline__ bool wait_long(uint64_t* bar, uint32_t parity, const volatile int* abort) {
+  return mbar_wait(bar, parity, abort, kPrefixWaitNs);
+}
+WR_DEVINL bool wait_warp(uint64_t* bar, uint32_t parity, const volatile int* abort = nullptr) {
+  if (kPrefixWaitNs == 0) return false;
   uint32_t ok;
   asm volatile(
       "{\n\t.reg .pred P;\n\t.reg .u32 n;\n\t"
@@ -95,7 +111,7 @@ WR_DEVINL bool wait_lean(uint64_t* bar, uint32_t parity) {
       : "=r"(ok)
       : "r"(smem_u32(bar)), "r"(parity)
       : "memory");
-  return ok != 0 || wait_long(bar, parity);
+  return __all_sync(0xffffffffu, ok != 0 || wait_long(bar, parity, abort));
 }
 
 // A CTA's pieces in order: the units of one (key head, row tiles) in its range.
@@ -176,9 +192,10 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1)
     uint32_t aux_phase = 0;
     int64_t unit = u0;
     int it = 0;
-    while (it < total && !*abort) {
+    bool dead = false;  // this warp or another gave up
+    while (it < total && !dead) {
       const Piece pc = piece_at(p, unit, u1);
-      for (int i = 0; i < pc.n && !*abort; ++i, ++it) {
+      for (int i = 0; i < pc.n; ++i, ++it) {
         const int st = it % S;
         const uint32_t ph = (it / S) & 1;
         const int key0 = (pc.u + i) * kTileKeys;
@@ -204,9 +221,8 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1)
             word |= (uint32_t)in << j;
           }
         }
-        if (it >= S && !mbar_wait(&k_empty[st], ph ^ 1, abort)) *abort = 1;
-        __syncwarp();
-        if (*abort) break;
+        dead = __any_sync(0xffffffffu, *abort) || (it >= S && !wait_warp(&k_empty[st], ph ^ 1, abort));
+        if (dead) break;
         if (lane < 4) s_mask[it % kMaskRing][lane] = word;
         if (lane == 0) s_special[it % kMaskRing] = special;
         __syncwarp();
@@ -217,9 +233,8 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1)
         uint8_t* dst = kbuf + st * C::kTileBytes + panel * C::kPanelBytes + pi * p.box * 128;
         if (ok) tma_load_4d(dst, &kmap, panel * 64, row, pc.h, page, &k_full[st], policy);
         issued_k = it + 1;
-        if (it >= S && !mbar_wait(&v_empty[st], ph ^ 1, abort)) *abort = 1;
-        __syncwarp();
-        if (*abort) break;
+        dead = it >= S && !wait_warp(&v_empty[st], ph ^ 1, abort);
+        if (dead) break;
         dst += vbuf - kbuf;
         uint64_t* bar = special ? &aux : &v_full[st];
         if (lane == 0) {
@@ -229,7 +244,10 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1)
         if (ok) tma_load_4d(dst, &vmap, panel * 64, row, pc.h, page, bar, policy);
         if (special) {
           // What the copies left behind the prefix, or did not bring, becomes 0.
-          if (!mbar_wait(&aux, aux_phase, nullptr)) *abort = 1;
+          // (Copies of this warp's: the whole limit.  Without them V never
+          // becomes full, and the warps that wait for it give up too.)
+          dead = !__all_sync(0xffffffffu, mbar_wait(&aux, aux_phase, nullptr));
+          if (dead) break;
           aux_phase ^= 1;
           for (int key = 0; key < kTileKeys; ++key) {
             const uint32_t w = __shfl_sync(0xffffffffu, word, key >> 5);
@@ -248,10 +266,12 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1)
     }
     // Nothing of this CTA's is in flight when it ends: copies have landed, and
     // (unless it gave up) the MMAs have released the stages.
+    if (dead) *abort = 1;
+    dead = __any_sync(0xffffffffu, *abort);
     for (int i = max(0, issued_k - S); i < issued_k; ++i)
-      mbar_wait(*abort ? &k_full[i % S] : &k_empty[i % S], (i / S) & 1, nullptr);
+      mbar_wait(dead ? &k_full[i % S] : &k_empty[i % S], (i / S) & 1, nullptr);
     for (int i = max(0, issued_v - S); i < issued_v; ++i)
-      mbar_wait(*abort ? &v_full[i % S] : &v_empty[i % S], (i / S) & 1, nullptr);
+      mbar_wait(dead ? &v_full[i % S] : &v_empty[i % S], (i / S) & 1, nullptr);
   } else if (warp > NT * 4) {
     // ---- the MMAs ---------------------------------------------------------
     // A warp for each tile's scores and one for its sums: what one waits for
@@ -265,7 +285,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1)
     const int t = which % NT;
     const uint32_t st = tmem_s + t * 2 * kHalf;
     bool dead = false;
-    auto wait = [&](uint64_t* bar, uint32_t parity) { dead |= !wait_lean(bar, parity); };
+    auto wait = [&](uint64_t* bar, uint32_t parity) { dead |= !wait_warp(bar, parity); };
     int64_t unit = u0;
     int j = 0, piece = 0;
     if (which < NT) {  // S = Q K^T
@@ -364,7 +384,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1)
       for (int i = 0; i < 2 * pc.n && !dead; ++i, ++it) {  // it: half tiles of this CTA
         const int b = it & 1;
         const uint32_t sb = ts + b * kHalf;
-        if (!wait_lean(&s_full[t][b], (it >> 1) & 1)) {
+        if (!wait_warp(&s_full[t][b], (it >> 1) & 1)) {
           *abort = 1;
           dead = true;
           break;
@@ -399,7 +419,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1)
           const bool up = top > m + kRescale;
           if (__any_sync(0xffffffffu, up)) {
             // O stands still once the last PV issued has ended.
-            if (!wait_lean(&pv_done[t][b ^ 1], ((it - 1) >> 1) & 1)) {
+            if (!wait_warp(&pv_done[t][b ^ 1], ((it - 1) >> 1) & 1)) {
               *abort = 1;
               dead = true;
               break;
@@ -424,7 +444,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1)
         float ls[4] = {0.f, 0.f, 0.f, 0.f};
         // The tiles' exponentials take turns: side by side both tiles wait for
         // the SFUs, then both for the rest, and the SFUs for them.
-        if (NT == 2 && (t == 1 || it > 0) && !wait_lean(&turn[t], (t == 1 ? it : it - 1) & 1)) {
+        if (NT == 2 && (t == 1 || it > 0) && !wait_warp(&turn[t], (t == 1 ? it : it - 1) & 1)) {
           *abort = 1;
           dead = true;
           break;
@@ -448,7 +468,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1)
         tc_fence_before();
         mbar_arrive(&p_full[t][b]);
       }
-      if (!dead && !wait_lean(&pv_done[t][(it - 1) & 1], ((it - 1) >> 1) & 1)) {
+      if (!dead && !wait_warp(&pv_done[t][(it - 1) & 1], ((it - 1) >> 1) & 1)) {
         *abort = 1;
         dead = true;
       }

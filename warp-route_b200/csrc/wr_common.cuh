@@ -106,17 +106,19 @@ WR_DEVINL bool mbar_test_wait(uint64_t* bar, uint32_t parity) {
   return ok != 0;
 }
 
-// Waits for the phase with `parity` to complete.  Gives up after
-// kWaitLimitNs, or as soon as *abort is set by another warp; returns false
-// then.  `abort` may be null (drain waits ignore it).
-WR_DEVINL bool mbar_wait(uint64_t* bar, uint32_t parity, const volatile int* abort) {
+// Waits for the phase with `parity` to complete.  Gives up after limit_ns, or
+// as soon as *abort is set by another warp; returns false then.  `abort` may be
+// null (drain waits ignore it).  The answer is this thread's own: the lanes of a
+// warp may get different ones where the phase completes just as time runs out.
+WR_DEVINL bool mbar_wait(uint64_t* bar, uint32_t parity, const volatile int* abort,
+                         uint64_t limit_ns = kWaitLimitNs) {
   if (mbar_try_wait(bar, parity)) return true;
   const uint64_t t0 = globaltimer_ns();
   for (uint32_t it = 1;; ++it) {
     if (mbar_try_wait(bar, parity)) return true;
     if ((it & 63u) == 0) {
       if (abort && *abort) return false;
-      if (globaltimer_ns() - t0 > kWaitLimitNs) return false;
+      if (globaltimer_ns() - t0 > limit_ns) return false;
     }
   }
 }
