@@ -36,7 +36,6 @@ namespace {
 // as many as it has room for.  (Beside a CTA of the prefix's kernel a warp of
 // this one gained nothing: its mma.sync wait for the tensor core, 184 us for
 // keys that take 60 alone.)
-constexpr int kStreamWarps = 1;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 #define WR_NEG_INF (-__int_as_float(0x7f800000))
@@ -237,8 +236,7 @@ struct StreamCfg {
   static constexpr int kRowBytes = DP * 2;
   static constexpr int kTile = kUnitTokens * kRowBytes;  // K (or V) of a unit
   static constexpr bool kQSmem = DP > 128;  // the fragments of 256 columns do not fit beside O
-  static constexpr int kWarpBytes = kStages * 2 * kTile + (kQSmem ? kTile : 0);
-  static constexpr int kSmem = kStreamWarps * kWarpBytes;
+  static constexpr int kSmem = kStages * 2 * kTile + (kQSmem ? kTile : 0);
 };
 
 // Registers for as many warps an SM as the rings leave room for.
@@ -246,20 +244,19 @@ struct StreamCfg {
 // values costs such calls 2 to 14 % (24 sequences of 1 to 9: 67.8 us, 66.1
 // without; the 209 sequences of 1 to 64 below: 257, 226).
 template <int DP, bool kSeveral>
-__global__ void __launch_bounds__(kStreamWarps * 32) __maxnreg__(DP == 64 ? 128 : DP == 128 ? 224 : 255) k_attn_stream(const AttnArgs a) {
+__global__ void __launch_bounds__(32) __maxnreg__(DP == 64 ? 128 : DP == 128 ? 224 : 255) k_attn_stream(const AttnArgs a) {
   using C = StreamCfg<DP>;
   constexpr int MR = 16, CPR = DP / 8, RPP = 32 / CPR;  // chunks a row, rows a pass of the warp
-  extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ uint32_t s_bits[kStreamWarps][kStages];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  extern __shared__ __align__(128) uint8_t ring[];
+  __shared__ uint32_t s_bits[kStages];
+  const int lane = threadIdx.x;
   griddep_launch_dependents();
   AttnSplit sp;
   sp.units = all_units<MR>(a, lane);
-  sp.ranges = min((int64_t)gridDim.x * kStreamWarps, sp.units);
-  const int64_t w = (int64_t)warp * gridDim.x + blockIdx.x;
+  sp.ranges = min((int64_t)gridDim.x, sp.units);
+  const int64_t w = blockIdx.x;
   if (w < sp.ranges) {
     const int64_t u0 = range_start(sp, w), u1 = range_start(sp, w + 1);
-    uint8_t* ring = smem + warp * C::kWarpBytes;
     const uint32_t ring_s = smem_u32(ring);
     const uint32_t q_s = ring_s + kStages * 2 * C::kTile;
     Cursor<MR> cl, cc;  // the copies' and the products' position
@@ -274,7 +271,7 @@ __global__ void __launch_bounds__(kStreamWarps * 32) __maxnreg__(DP == 64 ? 128 
         bool ok;
         const int64_t off = lane_offset(a, cl, page, lane, ok);
         const uint32_t bits = __ballot_sync(0xffffffffu, ok) & 0xffffu;
-        if (lane == 0) s_bits[warp][st] = bits;
+        if (lane == 0) s_bits[st] = bits;
         const uint32_t base = ring_s + st * 2 * C::kTile;
         const int c = lane % CPR;
         const bool in = c * 8 < a.dim;
@@ -353,7 +350,7 @@ __global__ void __launch_bounds__(kStreamWarps * 32) __maxnreg__(DP == 64 ? 128 
       __syncwarp();
       const int st = it % kStages;
       const uint32_t kb = ring_s + st * 2 * C::kTile, vb = kb + C::kTile;
-      const uint32_t bits = s_bits[warp][st];
+      const uint32_t bits = s_bits[st];
       float s[2][4] = {};
       {
         const int r = ((lane >> 4) << 3) + (lane & 7);
@@ -518,13 +515,11 @@ template <int DP, int MR>
 struct StreamF32Cfg {
   static constexpr int kStages = 2;
   static constexpr int kMR = MR;
-  static constexpr int kWarps = 1;
   static constexpr int kRowBytes = DP * 4;
   static constexpr int kTile = kUnitTokens * kRowBytes;
   static constexpr int kQBytes = kMR * kRowBytes;
   static constexpr int kPBytes = kUnitTokens * kMR * 4;
-  static constexpr int kWarpBytes = kStages * 2 * kTile + kQBytes + kPBytes;
-  static constexpr int kSmem = kWarps * kWarpBytes;
+  static constexpr int kSmem = kStages * 2 * kTile + kQBytes + kPBytes;
 };
 
 // Lane (t, half) of the first product: key t of the unit, half the columns;
@@ -537,17 +532,16 @@ __global__ void __launch_bounds__(32) k_attn_stream_f32(const AttnArgs a) {
   constexpr int kStages = C::kStages, CPR = DP / 4, HR = MR / 2;  // rows whose statistics a half of the lanes keeps
   constexpr int VC = DP / 32;  // columns of O a lane has
   constexpr int VW = VC < 4 ? VC : 4;  // ... in runs of VW
-  extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ uint32_t s_bits[C::kWarps][kStages];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  extern __shared__ __align__(128) uint8_t ring[];
+  __shared__ uint32_t s_bits[kStages];
+  const int lane = threadIdx.x;
   griddep_launch_dependents();
   AttnSplit sp;
   sp.units = all_units<MR>(a, lane);
-  sp.ranges = min((int64_t)gridDim.x * C::kWarps, sp.units);
-  const int64_t w = (int64_t)warp * gridDim.x + blockIdx.x;
+  sp.ranges = min((int64_t)gridDim.x, sp.units);
+  const int64_t w = blockIdx.x;
   if (w < sp.ranges) {
     const int64_t u0 = range_start(sp, w), u1 = range_start(sp, w + 1);
-    uint8_t* ring = smem + warp * C::kWarpBytes;
     const uint32_t ring_s = smem_u32(ring);
     float* qs = reinterpret_cast<float*>(ring + kStages * 2 * C::kTile);
     float* ps = qs + MR * DP;
@@ -563,7 +557,7 @@ __global__ void __launch_bounds__(32) k_attn_stream_f32(const AttnArgs a) {
         bool ok;
         const int64_t off = lane_offset(a, cl, page, lane, ok);
         const uint32_t bits = __ballot_sync(0xffffffffu, ok) & 0xffffu;
-        if (lane == 0) s_bits[warp][st] = bits;
+        if (lane == 0) s_bits[st] = bits;
         const uint32_t base = ring_s + st * 2 * C::kTile;
 #pragma unroll
         for (int i = 0; i < kUnitTokens * CPR / 32; ++i) {
@@ -623,7 +617,7 @@ __global__ void __launch_bounds__(32) k_attn_stream_f32(const AttnArgs a) {
       const int st = it % kStages;
       const uint8_t* kb = ring + st * 2 * C::kTile;
       const uint8_t* vb = kb + C::kTile;
-      const uint32_t bits = s_bits[warp][st];
+      const uint32_t bits = s_bits[st];
       float s[MR] = {};
       {
         const uint8_t* row = kb + t * C::kRowBytes;

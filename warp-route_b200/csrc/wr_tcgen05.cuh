@@ -132,7 +132,7 @@ WR_DEVINL void reg_dep16(uint32_t (&v)[16]) {
                : "memory");
 }
 
-// 32 consecutive columns of this warp's 32 lanes, in and out.
+// 32 consecutive columns of this warp's 32 lanes.
 WR_DEVINL void tmem_ld32(uint32_t taddr, uint32_t (&v)[32]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
@@ -160,6 +160,7 @@ WR_DEVINL void reg_dep32(uint32_t (&v)[32]) {
 // Waits for all of this thread's tcgen05.ld; follow with reg_dep32 of each
 // result before it is used.
 WR_DEVINL void tmem_wait_lds() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// 16 consecutive columns to this warp's 32 lanes; tmem_wait_st before they are used.
 WR_DEVINL void tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], "
