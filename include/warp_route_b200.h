@@ -339,7 +339,9 @@ typedef struct wr_rows {
  * [num_tokens][num_q_heads][head_dim], the queries of all tokens, those
  * without a slot too, turn by the same angles into q_out, which must not
  * overlap q.  rot_dim: even, in [0, head_dim]; positions and inv_freq may be
- * NULL when it is 0.  No counterpart in warp-route. */
+ * NULL when it is 0.  k, v and q must not overlap the rows that are written,
+ * nor these one another (a stride of 0 is refused).  No counterpart in
+ * warp-route. */
 WR_API wr_status_t wr_append_paged_kv(const wr_paged_kv_t* cache, int32_t num_tokens,
                                       const wr_rows_t* k, const wr_rows_t* v,
                                       const int64_t* slots, const int64_t* positions,

@@ -181,6 +181,18 @@ def test_append_with_queries_of_no_heads():
     assert "num_q_heads must be positive" in message()
 
 
+@pytest.mark.parametrize("kw", [dict(page_stride=0), dict(head_stride=0), dict(slot_stride=0)])
+def test_append_into_an_expanded_cache(kw):
+    """Heads (rows, pages) that are one memory cannot hold keys of their own."""
+    assert append(cache(**kw)) == _abi.WR_ERR_INVALID and "strides" in message()
+    # read, such a cache is as good as any; a dimension of one has no stride that counts
+    d = _abi.AttnDesc(3, 3, 4, 2, 2, 0, 0.1)
+    lib = _abi.load()
+    assert lib.wr_shared_prefix_attention_workspace_size(ctypes.byref(cache(**kw)), ctypes.byref(d), 0) > 0
+    one = dict(num_pages=1, num_kv_heads=1, page_size=1, page_stride=0, head_stride=0, slot_stride=0)
+    assert append(cache(**one), T=0) == _abi.WR_OK
+
+
 def test_prefix_waits_have_one_answer_for_a_warp():
     """k_attn_prefix branches on its waits around warp-wide instructions: each
     wait whose answer counts goes through a vote, and so does the word by

@@ -383,6 +383,9 @@ wr_status_t wr_append_paged_kv(const wr_paged_kv_t* cache, int32_t num_tokens, c
   AppendProblem p{};
   wr_status_t st = make_cache(cache, &p.c);
   if (st != WR_OK) return st;
+  if ((p.c.num_pages > 1 && p.c.page_stride == 0) || (p.c.hkv > 1 && p.c.head_stride == 0) ||
+      (p.c.page_size > 1 && p.c.slot_stride == 0))
+    return fail(WR_ERR_INVALID, "the strides of a cache that is written must not be 0 (an expanded tensor)");
   if (num_tokens < 0) return fail(WR_ERR_INVALID, "num_tokens must be >= 0, got %d", num_tokens);
   if (rot_dim < 0 || rot_dim > p.c.dim || rot_dim % 2 != 0)
     return fail(WR_ERR_INVALID, "rot_dim must be even and in [0, head_dim=%d], got %d", p.c.dim, rot_dim);

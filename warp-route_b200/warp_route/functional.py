@@ -257,7 +257,8 @@ def append_paged_kv(
     s // page_size) of k_cache, v_cache [num_pages, num_kv_heads, page_size,
     head_dim] (any strides of multiples of 16 bytes, the same for both).  A
     slot that is negative or outside the cache drops its token: the padding
-    of a batch.  Two tokens with one slot leave its content undefined.
+    of a batch.  Two tokens with one slot leave its content undefined, and k,
+    v and q must not share memory with the rows that are written.
 
     With positions [T] (int64) and inv_freq [rot_dim / 2] (float32) the first
     rot_dim columns of every key turn by the angles position * inv_freq:
