@@ -264,3 +264,16 @@ def test_values_at_the_end_of_a_bin_before_a_full_one(v):
         check(x, u, top_p=p)
     check(x.bfloat16(), u, top_p=0.4)
     check(x, u, top_p=0.4, top_k=v // 3)
+
+
+@pytest.mark.parametrize("kw", [dict(), dict(top_k=3), dict(top_p=0.7), dict(min_p=0.4), dict(top_k=900, top_p=0.9)])
+@pytest.mark.parametrize("t", [1e36, 1e38, float("inf")])
+def test_the_largest_finite_logits(t, kw):
+    """Only an infinite maximum leaves the finite values without weight."""
+    big = torch.finfo(torch.float32).max
+    x = big * (1 - torch.rand(6, 1000, device="cuda", generator=torch.Generator("cuda").manual_seed(1)) / 100)
+    x[:, 17] = big
+    x[1, ::2] = -big  # a span beyond the type
+    x[2, 3] = float("inf")
+    u = torch.tensor([0.1, 0.3, 0.5, 0.7, 0.9, 0.99], device="cuda")
+    check(x, u, temperature=t, **kw)

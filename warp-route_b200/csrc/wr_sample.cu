@@ -684,7 +684,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const SampleArgs a) {
   row.maxd = wider(row.max);
   // e^-41.6 is 2^-60, far below the 2^-46 that rounds to nothing
   const float lowest = value_of((uint32_t)low);
-  row.low = row.max > 3.4e38f ? row.max : fmaxf(row.max - 41.6f * temp, lowest);
+  row.low = row.max == __builtin_huge_valf() ? row.max : fmaxf(row.max - 41.6f * temp, lowest);
   row.steps = kTable * 1.4426950408889634074 / (double)temp;
   row.table = s.table;
 
