@@ -170,3 +170,24 @@ def test_later_keys_that_are_not_finite_against_the_plain_form(d, group, prefix,
     # rows that see none of those keys: as if they were not there
     out[hit], lse[hit] = clean[0][hit], clean[1][hit]
     check(s, out, lse)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("hq,prefix,several", [(8, 0, False), (8, 0, True), (8, 70, False), (8, 70, True),
+                                               (32, 5000, False), (32, 5000, True)])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_a_query_that_is_not_finite_stays_alone(bad, hq, prefix, several, dtype):
+    """Rows share tiles of products: one token's query must not reach another's output."""
+    nq = [3, 1, 4, 2, 7] if several else [1] * 17
+    if prefix == 5000 and dtype == torch.bfloat16:
+        assert tiles(sum(nq), hq, 8, 128, prefix) == 1
+    s = make([(i * 31) % 90 + 7 for i in range(len(nq))], nq, hq, 8, 128, 16, prefix, dtype)
+    out, lse = call(s, return_lse=True)
+    check(s, out, lse)
+    q = s["q"].clone()
+    q[5, ::2] = bad
+    got, gl = call(dict(s, q=q), return_lse=True)
+    keep = torch.ones(q.shape[:2], dtype=torch.bool, device="cuda")
+    keep[5, ::2] = False
+    assert torch.equal(got[keep], out[keep]) and torch.equal(gl[keep], lse[keep])
+    assert torch.isnan(got[~keep]).all()

@@ -197,3 +197,21 @@ def test_capture_writes_no_cache():
     assert torch.equal(stack.context.slots, slots)
     assert torch.equal(stack.step(x), stack.eager(x))
     stack.close()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_the_stack_samples_the_plain_forms_tokens(dtype):
+    from decode_reference import sample
+
+    stack, normal, H = build(4, dtype)
+    for n in range(6):
+        advance(stack.context, n)
+        out = stack.step(normal(4, H, std=1))
+        u = torch.rand(4, device="cuda", generator=torch.Generator("cuda").manual_seed(n))
+        for kw in (dict(), dict(temperature=0.8, top_k=20, top_p=0.9), dict(top_p=0.5, min_p=0.02)):
+            ids = stack.sample(out, u, **kw)
+            logits = torch.nn.functional.linear(out.view(4, H), stack.head).double().cpu().numpy()
+            full = dict(dict(temperature=1.0, top_k=0, top_p=1.0, min_p=0.0), **kw)
+            full = {k: v if k == "top_k" else float(torch.tensor(v)) for k, v in full.items()}
+            assert ids.tolist() == [sample(logits[r], u[r].item(), **full) for r in range(4)]
+    stack.close()

@@ -277,3 +277,20 @@ def test_the_largest_finite_logits(t, kw):
     x[2, 3] = float("inf")
     u = torch.tensor([0.1, 0.3, 0.5, 0.7, 0.9, 0.99], device="cuda")
     check(x, u, temperature=t, **kw)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_masks_of_the_lowest_value(dtype):
+    """Masked logits are the type's lowest finite value: all others share one
+    of the even bins, and masked ones only come in where nothing else is left."""
+    x, u = rows(5, 30000, dtype, seed=2)
+    low = torch.finfo(dtype).min
+    x[0, ::2] = low
+    x[1, 40:] = low
+    x[2, :-3] = low
+    x[3] = low
+    for kw in (dict(), dict(top_k=7), dict(top_k=20000), dict(top_p=0.8), dict(top_k=5000, top_p=0.3),
+               dict(top_p=0.9, temperature=2.5), dict(min_p=0.1), dict(temperature=0.0)):
+        ids = check(x, u, **kw)
+        if kw.get("top_k") != 20000:
+            assert ids[1] < 40 and ids[2] >= 30000 - 3
