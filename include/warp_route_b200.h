@@ -368,8 +368,10 @@ WR_API wr_status_t wr_append_paged_kv(const wr_paged_kv_t* cache, int32_t num_to
  * that a token does not see does not reach it, infinities and NaN included.
  * A page index outside the cache hides its keys.  Lengths, tables and q_start are
  * read on the device, so a captured graph follows them; prefix_len is fixed
- * in the call.  The workspace needs no initial content; calls that share one
- * must not overlap on the GPU.  No counterpart in warp-route. */
+ * in the call.  Scores, maxima and sums are fp32; with bf16 caches the weights
+ * e^(score - max) are rounded to bf16 before they meet the values.  The
+ * workspace needs no initial content; calls that share one must not overlap on
+ * the GPU.  No counterpart in warp-route. */
 typedef struct wr_attn_desc {
   int32_t num_tokens;
   int32_t num_seqs;

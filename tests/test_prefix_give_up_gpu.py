@@ -27,13 +27,22 @@ pytestmark = pytest.mark.gpu
 def gives_up(tmp_path_factory):
     if not torch.cuda.is_available():
         pytest.skip("needs a CUDA device")
-    wr_build.build_library()  # the objects of the other sources
     d = tmp_path_factory.mktemp("give_up")
-    obj, lib = str(d / "prefix.o"), str(d / "libgive_up.so")
-    src = os.path.join(wr_build.CSRC, "wr_attn_prefix.cu")
-    subprocess.run([wr_build.NVCC] + wr_build.NVCC_FLAGS + ["-DWR_PREFIX_WAIT_NS=0", "-c", src, "-o", obj], check=True)
-    objs = [obj if s == "wr_attn_prefix.cu" else os.path.join(wr_build.OBJ_DIR, s + ".o")
-            for s in wr_build.KERNEL_SOURCES]
+
+    def compiled(source, *flags):
+        obj = str(d / (source + ".o"))
+        subprocess.run([wr_build.NVCC] + wr_build.NVCC_FLAGS + [*flags, "-c", os.path.join(wr_build.CSRC, source),
+                                                                "-o", obj], check=True)
+        return obj
+
+    objs = []
+    for source in wr_build.KERNEL_SOURCES:  # the usual library's objects, but for one
+        usual = os.path.join(wr_build.OBJ_DIR, source + ".o")
+        if source == "wr_attn_prefix.cu":
+            objs.append(compiled(source, "-DWR_PREFIX_WAIT_NS=0"))
+        else:
+            objs.append(usual if os.path.exists(usual) else compiled(source))
+    lib = str(d / "libgive_up.so")
     subprocess.run([wr_build.NVCC] + wr_build.ARCH + ["-shared", "-o", lib] + objs + ["-lcudart"], check=True)
     return _abi.load(lib)
 

@@ -1048,8 +1048,16 @@ __global__ void __launch_bounds__(128) k_attn_combine_ends(const CombineArgs c) 
 // ---------------------------------------------------------------------------
 // The prefix goes to the tensor cores from 33 rows a key head where the warps
 // of k_attn_stream, which read the keys again for every 16 rows, would read
-// more than this: below, that kernel's launch and set-up cost more (64 rows a
-// head and 2055 keys of 8 heads, 34 MB: 29 us with it, 26 without).
+// more than this: below, that kernel's launch and set-up cost more.  Whole
+// calls, us, without / with it, by the MB read so (8 key heads, 4 query heads
+// each, 200 own keys a sequence, caches that are not in L2):
+//   head  rows        16           34           64           128          256
+//    64     64   15.8 / 19.7  18.7 / 21.3  23.4 / 24.5  34.2 / 30.3  53.7 / 40.3
+//    64    256   20.3 / 23.7  24.4 / 31.2  28.6 / 29.8  39.4 / 32.7  58.4 / 39.0
+//   128     64   15.4 / 22.1  18.1 / 22.8  23.1 / 24.8  32.0 / 30.5  50.1 / 38.4
+//   128    128   21.2 / 27.1  23.7 / 32.9  27.7 / 28.8  37.2 / 30.9  55.1 / 38.3
+//   128    256   24.1 / 30.8  26.4 / 36.3  29.8 / 33.3  38.9 / 37.2  57.4 / 41.3
+//   128   1024   56.8 / 68.8  56.6 / 66.6  60.4 / 65.0  67.7 / 67.9  84.2 / 79.2
 constexpr int kTileMinRows = 32;
 constexpr int64_t kTileMinBytes = 64 << 20;
 

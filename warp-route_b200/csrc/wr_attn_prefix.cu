@@ -17,7 +17,7 @@
 // there when a softmax ends; with one of 128 columns, whose P has to be
 // consumed before the next S, softmax and products of a tile took turns
 // (145 us for 1536 rows and 16384 keys of 8 heads; now 100 us, 1.05 PFLOP/s, at
-// the 1.5 GHz that the power limit leaves).  m follows the true maximum
+// the 1.5 GHz that the power limit leaves, and 2 us more for the votes on waits).  m follows the true maximum
 // only when it has grown by more than 8 (a factor of 256, harmless in fp32
 // sums and bf16 weights), so O is rescaled rarely.  Warp 4 * NT brings K and V
 // by TMA, a copy a page and 64 columns, into two rings; the warps behind it

@@ -45,7 +45,9 @@ class StackAttention:
     """One layer's attention: wqkv [(num_heads + 2 num_kv_heads) head_dim, H]
     (rows of q, then k, then v), wo [H, num_heads head_dim], its caches
     [num_pages, num_kv_heads, page_size, head_dim], and the frequencies
-    inv_freq (float32 [rot_dim / 2], None: no rotation)."""
+    inv_freq (float32 [rot_dim / 2], None: no rotation).  With a stack's
+    `comm` or `all_reduce` only the MoE layers are sharded: every rank
+    computes the whole attention and holds the whole caches."""
     wqkv: torch.Tensor
     wo: torch.Tensor
     num_heads: int

@@ -283,7 +283,10 @@ def shared_prefix_attention(
     return_lse: bool = False,
 ):
     """Attention of a batch over a paged cache, where all sequences share a
-    prefix, whose keys and values are read once for all of them.
+    prefix, which is read for tiles of all their rows rather than for each
+    sequence: tiles of 128 or 256 rows on the tensor cores where it is long
+    and the rows are many (bfloat16, heads of 64 to 128, pages of a power of
+    two from 16), else tiles of 16 rows (4 or 8 in float32).
 
     Every sequence sees the prefix_len keys in the pages prefix_pages (int32)
     and then its own context_lens[b] (int32 [B]) keys in the pages of row b
@@ -298,7 +301,10 @@ def shared_prefix_attention(
     the fp32 log of the sum of exponentials [T, num_q_heads].  A row that
     sees no key (and a token of no sequence) gets 0 and -inf.  Keys that a
     token does not see do not reach it, infinities and NaN included.  Lengths
-    and tables are read on the device: a captured graph follows them."""
+    and tables are read on the device: a captured graph follows them, but
+    keeps its prefix_len.  Scores, maxima and sums are fp32; with bfloat16
+    caches the weights exp(score - max) are rounded to bfloat16 (2^-8 at most)
+    before they meet the values, and the output once more."""
     _C = _load_extension()
     out, lse = _C.shared_prefix_attention(q, k_cache, v_cache, block_tables, context_lens,
                                           prefix_pages, prefix_len, q_start,
