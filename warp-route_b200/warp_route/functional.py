@@ -331,8 +331,10 @@ def sample_tokens(
     largest; the token is the first whose running sum of kept w, by index,
     exceeds uniform * sum.  Each setting is a number or a tensor with one for
     each row (float32, top_k int32); temperature 0 takes the maximum, top_k
-    0, top_p 1 and min_p 0 are off.  The result is the same every time.  NaN
-    counts as -inf; a row with nothing above -inf gets -1."""
+    0, top_p 1 and min_p 0 are off.  Sums are of w in whole numbers of 2^-45,
+    in which a weight below 2^-46 is nothing, so the result is the same every
+    time.  NaN counts as -inf; a row with nothing above -inf gets -1; at most
+    262144 values a row."""
     _C = _load_extension()
 
     def split(value, off):
